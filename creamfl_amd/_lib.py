@@ -57,6 +57,15 @@ SIGNATURES = {
     'cfl_bias_gelu_bwd': (c_int, [_P, _P, c_int, _P, c_longlong, c_int, _P, _P, c_int, _P, _P]),
     'cfl_dropout_mask': (c_int, [c_uint, c_float, c_longlong, _P, _P]),
     'cfl_set_dropout_tick': (c_int, [_P]),
+    'cfl_dropout': (c_int, [_P, c_int, c_longlong, c_double, c_uint, _P, _P, _P, _P]),
+    'cfl_gn_ws_bytes': (c_size_t, [c_int, c_int, c_int, c_int]),
+    'cfl_gn_fwd': (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, _P, _P, _P, _P]),
+    'cfl_gn_bwd': (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P]),
+    'cfl_relpos_ws_bytes': (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    'cfl_relpos_fwd': (c_int, [_P, c_longlong, _P, _P, c_longlong, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_int,
+                               c_int, _P, c_int, _P, c_longlong, _P, _P]),
+    'cfl_relpos_bwd': (c_int, [_P, c_longlong, _P, _P, c_longlong, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_int,
+                               c_int, _P, c_int, _P, _P, c_longlong, _P, _P, _P, c_longlong, _P, _P, c_longlong, _P, _P, _P]),
     'cfl_attn_small_fwd': (c_int, [_P, _P, _P, c_longlong, c_longlong, _P, c_int, c_int, c_int, c_int, _P, c_longlong, c_longlong, _P]),
     'cfl_attn_small_bwd': (c_int, [_P, _P, _P, c_longlong, c_longlong, _P, c_int, c_int, c_int, c_int, _P, c_longlong, c_longlong,
                                    _P, _P, _P, c_longlong, c_longlong, _P]),

@@ -1218,6 +1218,106 @@ def bn_act_eval(x, weight, bias, running_mean, running_var, eps, relu=False, res
     return y
 
 
+# --------------------------------------------------------------------------- trunk glue: group norm (+ residual) (+ activation)
+_GN_ACTS = {'none': 0, None: 0, 'relu': 1, 'silu': 2}
+
+
+def _on_device(t):
+    """Context in which a launch for `t` may be issued: its device is the current one (launches go to the current device)."""
+    idx = t.device.index
+    return contextlib.nullcontext() if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(idx)
+
+
+def _aligned16(t):
+    """`t`, or a copy of it where its first element does not lie on a 16-byte border (a view into the middle of a buffer)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format)
+
+
+def gn_act_supported(x, num_channels, groups):
+    """True when `gn_act` takes `x`: [N, C, H, W] on the GPU, channels_last, bf16 or fp32, C a multiple of 8 and of `groups`, C <= 2048."""
+    return (torch.is_tensor(x) and x.is_cuda and x.dim() == 4 and x.dtype in (torch.bfloat16, torch.float32) and x.numel() > 0
+            and x.shape[1] == num_channels and num_channels % 8 == 0 and num_channels <= 2048 and groups >= 1
+            and num_channels % groups == 0 and x.shape[0] <= 65535 and x.is_contiguous(memory_format=torch.channels_last))
+
+
+class _GNActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, groups, eps, act, need):
+        lib = _lib.load()
+        N, C, H, W = x.shape
+        y = torch.empty_like(x)                           # keeps channels_last
+        stats = torch.empty(2, N, groups, dtype=torch.float32, device=x.device) if need else None
+        ws = _ws(lib.cfl_gn_ws_bytes(N, H * W, C, groups), x.device)
+        with _on_device(x):
+            _lib.check(lib.cfl_gn_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), int(x.dtype == torch.bfloat16), N, H * W, C, groups,
+                                      eps, act, _ptr(y), _ptr(stats), _ptr(stats[1]) if need else None, _ptr(ws), _stream(x)), 'cfl_gn_fwd')
+        if need:
+            # (without an activation dz = dy: the residual is not read again)
+            ctx.save_for_backward(x, residual if act else None, weight, bias, stats)
+            ctx.hyper = (groups, act, residual is not None)
+        ctx.set_materialize_grads(False)                  # an unused alias must arrive as None, not as a zero tensor
+        return y, _alias(y)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dy2):
+        lib = _lib.load()
+        x, residual, weight, bias, stats = ctx.saved_tensors
+        groups, act, has_res = ctx.hyper
+        if dy is None:
+            dy, dy2 = dy2, None
+        if dy is None:
+            return (None,) * 8
+        N, C, H, W = x.shape
+        from . import streams
+        streams.flush(x.device)                           # a long HBM-bound phase: let the queued weight gradients run beside it
+
+        def prep(t):
+            return _aligned16(t.to(x.dtype).contiguous(memory_format=torch.channels_last))
+        dy = prep(dy)
+        dy2 = prep(dy2) if dy2 is not None else None
+        dx = torch.empty_like(x)
+        want = has_res and ctx.needs_input_grad[1]
+        # without an activation the residual's gradient is dy itself, unless two gradients have to be added
+        own = want and (act != 0 or dy2 is not None)
+        dres = torch.empty_like(x) if own else dy if want else None
+        dgb = torch.empty(2, C, dtype=torch.float32, device=x.device)
+        ws = _ws(lib.cfl_gn_ws_bytes(N, H * W, C, groups), x.device)
+        with _on_device(x):
+            _lib.check(lib.cfl_gn_bwd(_ptr(dy), _ptr(dy2), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(stats), _ptr(stats[1]),
+                                      int(x.dtype == torch.bfloat16), N, H * W, C, groups, act, int(own), _ptr(dx),
+                                      _ptr(dres) if own else None, _ptr(dgb), _ptr(dgb[1]), _ptr(ws), _stream(x)), 'cfl_gn_bwd')
+        return dx, dres, dgb[0], dgb[1], None, None, None, None
+
+
+def gn_act(x, weight, bias, groups, eps=1e-5, act='none', residual=None, two=False):
+    """act(GroupNorm(x) (+ residual)) of a channels_last feature map (csrc/gnorm.hip): statistics over a sample's C / groups channels and
+    all positions; act 'none', 'relu' or 'silu'.  x [N, C, H, W] bf16 or fp32 (`gn_act_supported`), weight and bias [C]; residual of x's
+    shape.  Differentiable in x, residual, weight and bias (once).  `two=True` returns the output as two tensor objects on one buffer, as
+    `bn_act_train` does: their two gradients are summed inside the backward."""
+    if act not in _GN_ACTS:
+        raise _lib.CreamflHipError(f"gn_act: act must be 'none', 'relu' or 'silu', got {act!r}")
+    if not (torch.is_tensor(x) and x.is_cuda):
+        raise _lib.CreamflHipError('gn_act: expected a CUDA/HIP tensor (no CPU fallback in creamfl_amd)')
+    groups = int(groups)
+    if not gn_act_supported(x, x.shape[1] if x.dim() == 4 else 0, groups):
+        raise _lib.CreamflHipError(f'gn_act: expected a channels_last bf16 / fp32 [N, C, H, W] map with C % 8 == 0, C % groups == 0, C <= 2048; '
+                                   f'got {tuple(x.shape)} {x.dtype} with {groups} groups')
+    for t, name in ((weight, 'weight'), (bias, 'bias')):
+        if not torch.is_tensor(t) or tuple(t.shape) != (x.shape[1],) or t.device != x.device:
+            raise _lib.CreamflHipError(f'gn_act: {name} must be a [{x.shape[1]}] tensor on {x.device}')
+    if not float(eps) >= 0.0:
+        raise _lib.CreamflHipError(f'gn_act: eps must not be negative, got {eps}')
+    if residual is not None:
+        if tuple(residual.shape) != tuple(x.shape) or residual.device != x.device:
+            raise _lib.CreamflHipError(f'gn_act: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}')
+        residual = _aligned16(residual.to(x.dtype).contiguous(memory_format=torch.channels_last))
+    weight, bias = _f32(weight, 'weight'), _f32(bias, 'bias')
+    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias))
+    y, y2 = _GNActFn.apply(_aligned16(x), residual, weight, bias, groups, float(eps), _GN_ACTS[act], need)
+    return (y, y2) if two else y
+
+
 # --------------------------------------------------------------------------- 1x1 convolution: data gradient (csrc/gemm_bf16.hip)
 GEMM_COUNTERS = {'flops': 0, 'bytes': 0}   # python ints; bench.py turns them into algorithmic work per launch
 
@@ -2250,6 +2350,200 @@ def dropout_keep_mask(seed, p, shape, device):
     keep = torch.empty(n, dtype=torch.uint8, device=device)
     _lib.check(lib.cfl_dropout_mask(int(seed), float(p), n, _ptr(keep), _stream(keep)), 'cfl_dropout_mask')
     return keep.view(*shape).bool()
+
+
+# --------------------------------------------------------------------------- dropout (csrc/dropout.hip)
+_DROP_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, need):
+        y = torch.empty_like(x)
+        used = torch.empty(1, dtype=torch.int32, device=x.device) if need else None
+        with _on_device(x):
+            _lib.check(_lib.load().cfl_dropout(_ptr(x), _DROP_DTYPES[x.dtype], x.numel(), p, seed, None, _ptr(y), _ptr(used), _stream(x)),
+                       'cfl_dropout')
+        if need:
+            ctx.save_for_backward(used)                   # (the seed as the device used it: the tick may move on before the backward)
+            ctx.p = p
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        used, = ctx.saved_tensors
+        dy = dy.contiguous()
+        dx = torch.empty_like(dy)
+        with _on_device(dy):
+            _lib.check(_lib.load().cfl_dropout(_ptr(dy), _DROP_DTYPES[dy.dtype], dy.numel(), ctx.p, 0, _ptr(used), _ptr(dx), None, _stream(dy)),
+                       'cfl_dropout')
+        return dx, None, None, None
+
+
+def dropout(x, p, seed=None):
+    """x / (1 - p) where a counter-based flag of (seed, element's number) says so, 0 elsewhere (csrc/dropout.hip): the mask is never stored,
+    the backward draws it again.  fp32, bf16 or fp16, any shape; elements are numbered in row-major order.  p counts in steps of 2^-16;
+    p = 0 returns x itself, p = 1 zeros.  seed: 32 bits (default: the next one of torch's seed, as the fused dropouts take it);
+    `dropout_keep_mask(seed, p, shape, device)` gives the flags.  Steps replayed from a graph vary with `dropout_tick`."""
+    if not (torch.is_tensor(x) and x.is_cuda):
+        raise _lib.CreamflHipError('dropout: expected a CUDA/HIP tensor (no CPU fallback in creamfl_amd)')
+    if x.dtype not in _DROP_DTYPES:
+        raise _lib.CreamflHipError(f'dropout: expected fp32, bf16 or fp16, got {x.dtype}')
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise _lib.CreamflHipError(f'dropout: p must lie between 0 and 1, got {p}')
+    if p == 0.0 or x.numel() == 0:
+        return x
+    seed = _next_dropout_seed() if seed is None else int(seed) & 0xFFFFFFFF
+    return _DropoutFn.apply(x.contiguous(), p, seed, torch.is_grad_enabled() and x.requires_grad)
+
+
+# --------------------------------------------------------------------------- attention with a relative position bias (csrc/relpos.hip)
+RELPOS_MAX_DISTANCE = 512
+
+
+def relpos_buckets(num_buckets=32, max_distance=128, device=None):
+    """int32 [2 max_distance + 1]: the bucket of the distance d = key - query, clipped to +-max_distance, at place d + max_distance.  Half of
+    the buckets are for keys behind the query; of a half, the first half are single distances, the others grow geometrically up to
+    max_distance (borders in whole numbers: |d| reaches bucket k where (|d| / e)^(n - e) >= (max_distance / e)^(k - e))."""
+    n = int(num_buckets) // 2
+    e = n // 2
+    max_distance = int(max_distance)
+    if int(num_buckets) < 4 or int(num_buckets) % 2 or not e < max_distance <= RELPOS_MAX_DISTANCE:
+        raise _lib.CreamflHipError(f'relpos_buckets: need an even number of at least 4 buckets and num_buckets / 4 < max_distance <= '
+                                   f'{RELPOS_MAX_DISTANCE}; got {num_buckets}, {max_distance}')
+
+    def one(d):
+        a = abs(d)
+        k = min(a, e)
+        if a >= e:
+            while k + 1 < n and a ** (n - e) * e ** (k + 1 - e) >= max_distance ** (k + 1 - e) * e ** (n - e):
+                k += 1
+        return k + (n if d > 0 else 0)
+    return torch.tensor([one(d) for d in range(-max_distance, max_distance + 1)], dtype=torch.int32, device=device)
+
+
+def relpos_attention_supported(head_dim):
+    return head_dim == 64
+
+
+class _RelposFn(torch.autograd.Function):
+    """q [rows, H] and kv [rows, 2 H], or qkv [rows, 3 H] with kv None, as 2-D matrices.  geo = (B, Lq, Lk, T, heads, scale)."""
+
+    @staticmethod
+    def forward(ctx, q, kv, table, buckets, mask, cu, geo, need):
+        lib = _lib.load()
+        B, Lq, Lk, T, heads, scale = geo
+        H = heads * 64
+        o = torch.empty(q.shape[0], H, dtype=torch.bfloat16, device=q.device)
+        lse = torch.empty(heads, q.shape[0], dtype=torch.float32, device=q.device) if need else None
+        kb = q.data_ptr() + 2 * H if kv is None else kv.data_ptr()
+        ldk = 3 * H if kv is None else 2 * H
+        with _on_device(q):
+            _lib.check(lib.cfl_relpos_fwd(_ptr(q), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,
+                                          _ptr(table), int(table.dtype == torch.bfloat16), table.shape[0], _ptr(buckets),
+                                          buckets.numel() // 2, _ptr(o), H, _ptr(lse), _stream(q)), 'cfl_relpos_fwd')
+        if need:
+            ctx.save_for_backward(q, kv, table, buckets, mask, cu, o, lse)
+            ctx.geo = geo
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        lib = _lib.load()
+        q, kv, table, buckets, mask, cu, o, lse = ctx.saved_tensors
+        B, Lq, Lk, T, heads, scale = ctx.geo
+        H, R = heads * 64, buckets.numel() // 2
+        do = _aligned16(_bf16c(do, 'do'))
+        dq = torch.empty_like(q)
+        dkv = None if kv is None else torch.empty_like(kv)
+        dtable = torch.empty_like(table)
+        dsum = torch.empty_like(lse)
+        ws = _ws(lib.cfl_relpos_ws_bytes(B, Lq, Lk, T, heads, R), q.device)
+        kb = q.data_ptr() + 2 * H if kv is None else kv.data_ptr()
+        gb = dq.data_ptr() + 2 * H if kv is None else dkv.data_ptr()
+        ldk = 3 * H if kv is None else 2 * H
+        with _on_device(q):
+            _lib.check(lib.cfl_relpos_bwd(_ptr(q), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,
+                                          _ptr(table), int(table.dtype == torch.bfloat16), table.shape[0], _ptr(buckets), R, _ptr(o),
+                                          _ptr(do), H, _ptr(lse), _ptr(dsum), _ptr(dq), q.shape[1], gb, gb + 2 * H, ldk, _ptr(dtable),
+                                          _ptr(ws), _stream(q)), 'cfl_relpos_bwd')
+        return dq, dkv, dtable, None, None, None, None, None
+
+
+def _relpos_check(name, q, width_of_q, table, buckets, heads, mask, cu, B, L):
+    """The shared argument checks; returns (table, buckets, mask) as the kernels take them."""
+    if heads < 1 or q.shape[-1] != width_of_q * heads * 64:
+        raise _lib.CreamflHipError(f'{name}: a last axis of {q.shape[-1]} is not {width_of_q} x {heads} heads x 64')
+    if not torch.is_tensor(table) or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] != heads or table.device != q.device \
+            or not table.is_floating_point():
+        raise _lib.CreamflHipError(f'{name}: table must be a floating [num_buckets, {heads}] tensor on {q.device}')
+    if not torch.is_tensor(buckets) or buckets.dim() != 1 or buckets.numel() % 2 != 1 or buckets.dtype != torch.int32 \
+            or buckets.device != q.device or buckets.numel() > 2 * RELPOS_MAX_DISTANCE + 1:
+        raise _lib.CreamflHipError(f'{name}: buckets must be an int32 [2 R + 1] tensor on {q.device}, R <= {RELPOS_MAX_DISTANCE} '
+                                   '(relpos_buckets)')
+    if mask is not None:
+        if not torch.is_tensor(mask) or mask.numel() != B * L or mask.shape[0] != B or mask.device != q.device:
+            raise _lib.CreamflHipError(f'{name}: key_mask must hold [{B}, {L}] flags on {q.device}')
+        mask = (mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0).reshape(B, L).contiguous()
+    if cu is not None and (not torch.is_tensor(cu) or cu.dtype != torch.int32 or cu.device != q.device or not cu.is_contiguous()
+                           or cu.dim() != 1 or cu.numel() < 2):
+        raise _lib.CreamflHipError(f'{name}: cu_seqlens must be a contiguous int32 [texts + 1] tensor on the device of the tokens')
+    if table.dtype not in (torch.bfloat16, torch.float32):
+        table = table.float()
+    return table.contiguous(), buckets.contiguous(), mask
+
+
+def _relpos_apply(q, kv, table, buckets, mask, cu, B, Lq, Lk, T, heads, scale):
+    scale = 0.125 if scale is None else float(scale)      # 1 / sqrt(64)
+    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, kv, table))
+    return _RelposFn.apply(q, kv, table, buckets, mask, cu, (B, Lq, Lk, T, heads, scale), need)
+
+
+def relpos_attention(qkv, table, buckets, heads, key_mask=None, scale=None):
+    """softmax_j(scale q_i . k_j + table[bucket of j - i, head]) V per text and head for a fused projection qkv [B, L, 3H] (Q | K | V along
+    the last axis), head dim 64, any length (csrc/relpos.hip).  table: [num_buckets, heads], bf16 or fp32; buckets: `relpos_buckets`, or
+    any int32 [2 R + 1] map of the clipped distance; key_mask [B, L] (True = the key takes part; what stands at a dropped key does not
+    matter), scale 1 / 8 by default.  A text without a key gives zeros.  Differentiable in qkv and table (once).  -> [B, L, H] bf16."""
+    qkv = _aligned16(_bf16c(qkv, 'qkv'))
+    heads = int(heads)
+    if qkv.dim() != 3 or qkv.numel() == 0:
+        raise _lib.CreamflHipError(f'relpos_attention: expected [B, L, 3H], got {tuple(qkv.shape)}')
+    B, L, H3 = qkv.shape
+    table, buckets, mask = _relpos_check('relpos_attention', qkv, 3, table, buckets, heads, key_mask, None, B, L)
+    return _relpos_apply(qkv.view(B * L, H3), None, table, buckets, mask, None, B, L, L, 0, heads, scale).view(B, L, H3 // 3)
+
+
+def relpos_attention_varlen(qkv, cu_seqlens, max_len, table, buckets, heads, scale=None):
+    """`relpos_attention` on PACKED tokens: qkv [T, 3H], text b = rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1] on the device;
+    a text may be empty); max_len: the longest text's length, a hint for the launch.  Rows behind the last text give zeros.  -> [T, H]."""
+    qkv = _aligned16(_bf16c(qkv, 'qkv'))
+    heads, max_len = int(heads), int(max_len)
+    if qkv.dim() != 2 or qkv.numel() == 0 or max_len < 1:
+        raise _lib.CreamflHipError(f'relpos_attention_varlen: expected [T, 3H] and max_len >= 1, got {tuple(qkv.shape)}, {max_len}')
+    table, buckets, _ = _relpos_check('relpos_attention_varlen', qkv, 3, table, buckets, heads, None, cu_seqlens, 0, 0)
+    T = qkv.shape[0]
+    return _relpos_apply(qkv, None, table, buckets, None, cu_seqlens, cu_seqlens.numel() - 1, 0, min(max_len, T), T, heads, scale)
+
+
+def relpos_attention_cls(q, kv, table, buckets, heads, key_mask=None, cu_seqlens=None, max_len=None, scale=None):
+    """The single query at position 0 of every text ([CLS]): q [B, H], kv [B, L, 2H] (K | V; key_mask [B, L]) or, packed, [T, 2H] with
+    cu_seqlens and max_len.  -> [B, H]; differentiable in q, kv and table (once)."""
+    q, kv = _aligned16(_bf16c(q, 'q')), _aligned16(_bf16c(kv, 'kv'))
+    heads = int(heads)
+    packed = cu_seqlens is not None
+    if q.dim() != 2 or kv.dim() != (2 if packed else 3) or q.numel() == 0 or kv.numel() == 0 or kv.device != q.device:
+        raise _lib.CreamflHipError(f'relpos_attention_cls: expected q [B, H] and kv {"[T, 2H]" if packed else "[B, L, 2H]"}; '
+                                   f'got {tuple(q.shape)}, {tuple(kv.shape)}')
+    B, L = q.shape[0], kv.shape[0] if packed else kv.shape[1]
+    if kv.shape[-1] != 2 * q.shape[1] or (not packed and kv.shape[0] != B) or (packed and (key_mask is not None or max_len is None
+                                                                                         or cu_seqlens.numel() != B + 1)):
+        raise _lib.CreamflHipError('relpos_attention_cls: q, kv, key_mask and cu_seqlens do not belong together')
+    table, buckets, mask = _relpos_check('relpos_attention_cls', q, 1, table, buckets, heads, key_mask, cu_seqlens, B, L)
+    Lk = min(max(int(max_len), 1), L) if packed else L
+    return _relpos_apply(q, kv.view(-1, kv.shape[-1]), table, buckets, mask, cu_seqlens, B, 1, Lk, L if packed else 0, heads, scale)
 
 
 # --------------------------------------------------------------------------- A6: retrieval ranks

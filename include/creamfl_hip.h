@@ -190,6 +190,48 @@ int cfl_dropout_mask(unsigned seed, float p, long long n, unsigned char* keep, v
  * seed + *tick * 0x85EBCA6B.  Process-wide; the pointer is read when a launch is issued (or captured). */
 int cfl_set_dropout_tick(const unsigned* tick_dev);
 
+/* ---- dropout of an activation (the embeddings of the BertModel at src/networks/models/pcme.py:36-38) ---------------------
+ * y[e] = keep(e) ? x[e] / (1 - p') : 0 for n elements; keep(e) = the 16 random bits of (seed, e) are >= rint(65536 p), p' = that / 65536:
+ * the flags of cfl_dropout_mask; 0 <= p <= 1 (1: zeros).  dtype: 0 fp32, 1 bf16, 2 fp16.  The seed is *seed_dev where seed_dev is given,
+ * else `seed` (with the tick of cfl_set_dropout_tick, if one is registered); what was used is written to *seed_used (NULL = skip).
+ * The backward is the same call on the gradient with seed_dev = the forward's seed_used.  y may be x. */
+int cfl_dropout(const void* x, int dtype, long long n, double p, unsigned seed, const unsigned* seed_dev, void* y,
+                unsigned* seed_used, void* stream);
+
+/* ---- group normalisation (+ residual) (+ activation), channels last -------------------------------------------------
+ * The normalisation of an image trunk (BatchNorm at src/networks/models/image_encoder.py:27-36, src/networks/resnet_client.py:60-98)
+ * for federations whose clients' batch statistics do not average: x [N][HW][C], G groups of C / G channels, statistics over one
+ * sample's HW C / G values;  z = (x - mu) rstd gamma + beta (+ res), y = act(z), act 0 none, 1 relu, 2 silu.
+ * dtype: 0 fp32, 1 bf16 (x, res, y, dy, dy2, dx, dres); gamma, beta, their gradients, mean / rstd [N][G] fp32 (both NULL = skip).
+ * C % 8 == 0, C <= 2048, N <= 65535, 16-byte aligned activations.  bwd: the gradient is dy + dy2 (dy2 may be NULL); dres = dy act'(z)
+ * where want_dres; `res` as in the forward (NULL = none).  ws: cfl_gn_ws_bytes (forward and backward alike). */
+size_t cfl_gn_ws_bytes(int N, int HW, int C, int G);
+int cfl_gn_fwd(const void* x, const void* res, const float* gamma, const float* beta, int dtype, int N, int HW, int C, int G, float eps,
+               int act, void* y, float* mean, float* rstd, void* ws, void* stream);
+int cfl_gn_bwd(const void* dy, const void* dy2, const void* x, const void* res, const float* gamma, const float* beta, const float* mean,
+               const float* rstd, int dtype, int N, int HW, int C, int G, int act, int want_dres, void* dx, void* dres, float* dgamma,
+               float* dbeta, void* ws, void* stream);
+
+/* ---- self-attention with a learned relative position bias by buckets, head_dim 64 -----------------------------------
+ * s_ij = scale q_i . k_j + table[bucket[clip(j - i, -R, R) + R]][h], softmax over the keys, o_i = sum_j p_ij v_j per (text, head): the
+ * text tower of src/networks/models/pcme.py:36-44 with distances in place of absolute positions.  q, k, v, o and gradients bf16, element
+ * (row, h * 64 + d) at row * ld + h * 64 + d (ldq of q, ldk of k and v, ldo of o and dout, lddq, lddk); table [nb][heads] bf16 or fp32,
+ * bucket [2 R + 1] (values outside [0, nb) are taken as the nearest end), R <= 512.
+ * Padded (cu NULL): text b has query rows b Lq .. and key rows b Lk ..; mask [B][Lk] bytes (0 = key dropped; what stands in its k and v
+ * does not matter) or NULL.  Packed: text b has key rows cu[b] .. cu[b + 1] - 1 of T; Lq = 0: these are its queries too, else Lq
+ * query rows b Lq ..; Lk is the longest text (a hint for the launch: longer ones are handled).  Rows behind cu[B] get zeros.
+ * Query i of a text stands at position i.  A row without a key has o = 0 and no gradient.
+ * lse (fp32 [heads][query rows]) is written by fwd (NULL = skip) and read by bwd; dsum: scratch of the same size; dtable as table.
+ * All ld % 8 == 0, 16-byte aligned bases.  ws: cfl_relpos_ws_bytes (T = 0: padded). */
+size_t cfl_relpos_ws_bytes(int B, int Lq, int Lk, int T, int heads, int R);
+int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
+                   int B, int Lq, int Lk, int T, int heads, int head_dim, float scale, const void* table, int table_bf16, int nb,
+                   const int* bucket, int R, void* o, long long ldo, float* lse, void* stream);
+int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
+                   int B, int Lq, int Lk, int T, int heads, int head_dim, float scale, const void* table, int table_bf16, int nb,
+                   const int* bucket, int R, const void* o, const void* dout, long long ldo, const float* lse, float* dsum, void* dq,
+                   long long lddq, void* dk, void* dv, long long lddk, void* dtable, void* ws, void* stream);
+
 /* ---- BERT self-attention for short sequences (L <= 32 tokens, head_dim 64) -------------------------------------
  * softmax(Q K^T / sqrt(64) + key-padding mask) V per (batch, head): BertSelfAttention of the BertModel built at
  * src/networks/models/pcme.py:36-38 (captions are ~12-30 tokens).  One wavefront per (batch, head), MFMA, nothing
