@@ -145,7 +145,7 @@ class ClientTrainer:
         if self.dset_name in IMAGE_SETS:
             self.model = resnet18_client(pretrained=True, num_class=self.classSize, pool_type=self.pool_type,
                                          is_train=True, scale=self.scale, mlp_local=self.args.mlp_local,
-                                         embed_dim=self.args.feature_dim)
+                                         embed_dim=self.args.feature_dim, norm=flags.get(self.args, 'image_norm'))
         else:
             self.model = EncoderText(embed_dim=self.args.feature_dim, num_class=self.classSize, scale=self.scale,
                                      mlp_local=self.args.mlp_local)

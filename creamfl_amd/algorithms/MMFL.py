@@ -97,6 +97,7 @@ class MMFL(object):
         for k in ('cnn_type', 'bert_name'):               # build-defined encoder overrides (configs 1 and 5)
             if getattr(self.args, k, None):
                 self.config.model[k] = getattr(self.args, k)
+        self.config.model.image_norm = flags.get(self.args, 'image_norm')
         self.config.model.wemb_type = None
 
     # -------------------------------------------------------------------------------------------------- data
@@ -157,6 +158,7 @@ class MMFL(object):
                 config = default_config(embed_dim=args.feature_dim, cnn_type='resnet18', not_bert=True)
                 config.train.use_fp16 = False
             config.model.embed_dim = args.feature_dim
+            config.model.image_norm = flags.get(args, 'image_norm')
             config.model.not_bert = True
             for client_id in range(args.num_mm_clients):
                 loaders = client_loaders.get('mm')

@@ -27,7 +27,6 @@ typedef unsigned int u32;
 typedef unsigned long long u64;
 
 constexpr int TP = 72;                      // LDS row pitch in bf16 (144 bytes: 16-byte rows and both kinds of reads spread over the banks)
-constexpr int KT = 64;                      // rows of a staged tile
 constexpr int BPAD = 64;                    // the bias vector reaches this far beyond +-R: a tile that touches |d| <= R needs no clipping
 constexpr int MAXR = 512;                   // largest R (LDS)
 constexpr float LOG2E = 1.4426950408889634f;
@@ -47,10 +46,12 @@ struct RpArgs {
     const int* bucket;                      // [2 R + 1]
     float* lse;                             // [heads][rows]: log2-sum of a row's scores (+inf: no key)
     float* dsum;                            // [heads][rows]: D
-    float* diag;                            // [heads][slots][2 Rr + 1]
-    int Rr;                                 // min(R, longest distance): distances that occur
+    float* diag;                            // [heads][B nqb][nb]: the bias gradient's parts
     int nqb;                                // query blocks of the longest text
-    long long rows;                         // query rows in all (B Lq or T)
+    int ns;                                 // parts a text's keys (forward, dQ) or queries (dK, dV) are split into
+    float *po, *pm;                         // the parts' results: [ns][heads][rows][64], and of the forward [ns][heads][rows][2] (maximum, sum)
+    float* pv;                              // dV's
+    long long rows, krows;                  // query rows, key rows in all
 };
 
 // rows of text b
@@ -104,32 +105,80 @@ __device__ __forceinline__ void load_rows(const u16* base, long long ld, int row
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) f[kk] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const f32x4*>(p + kk * 16));
 }
-// rows r0 .. r0 + 63 of a [n][64] matrix into a tile; rows >= n and rows whose keep flag is 0 become zeros (whatever stands there,
-// infinities and NaN included, must not reach a product)
-template <int NT>
-__device__ __forceinline__ void stage(const u16* base, long long ld, int r0, int n, const unsigned char* keep, u16* tile) {
+// One tile of `ROWS` rows on its way from memory to LDS through registers: `load` early, `put` late.  Rows whose bit in `bits` is 0 (dropped
+// keys, rows past the end) become zeros: whatever stands there, infinities and NaN included, must not reach a product.
+template <int NT, int ROWS>
+struct Stage {
+    static constexpr int N = ROWS * 8 / NT;
+    f32x4 r[N];
+    __device__ __forceinline__ void load(const u16* base, long long ld, int r0, u64 bits) {
 #pragma unroll
-    for (int it = 0; it < KT * 8 / NT; ++it) {
-        const int c = it * NT + threadIdx.x, row = c >> 3, cc = c & 7;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (r0 + row < n && (!keep || keep[r0 + row])) v = *reinterpret_cast<const f32x4*>(base + (long long)(r0 + row) * ld + cc * 8);
-        *reinterpret_cast<f32x4*>(tile + row * TP + cc * 8) = v;
+        for (int i = 0; i < N; ++i) {
+            const int c = i * NT + threadIdx.x, row = c >> 3;
+            r[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if ((bits >> row) & 1) r[i] = *reinterpret_cast<const f32x4*>(base + (long long)(r0 + row) * ld + (c & 7) * 8);
+        }
     }
+    __device__ __forceinline__ void put(u16* tile) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = i * NT + threadIdx.x;
+            *reinterpret_cast<f32x4*>(tile + (c >> 3) * TP + (c & 7) * 8) = r[i];
+        }
+    }
+};
+__device__ __forceinline__ u64 low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
+// The keys of a text in tiles of KT, 64 tiles at a time: which tiles have a key (bit i of `alive`: tile i from c0), which rows of a tile.
+template <int NW, int KT>
+struct Keys {
+    const unsigned char* mask;
+    int lk, c0;
+    u64* tb;                                                   // [64] in LDS, used with a mask
+    u64 alive;
+    __device__ __forceinline__ void chunk(int c0_) {           // (all waves; a barrier inside where there is a mask)
+        c0 = c0_;
+        const int lane = threadIdx.x & 63, n = min(64, (lk - c0 + KT - 1) / KT);
+        if (!mask) { alive = low_bits(n); return; }
+        __syncthreads();
+        for (int t = threadIdx.x >> 6; t < n; t += NW) {
+            const int j = c0 + t * KT + lane;
+            const u64 bits = __ballot(lane < KT && j < lk && mask[min(j, lk - 1)] != 0);
+            if (lane == 0) tb[t] = bits;
+        }
+        __syncthreads();
+        alive = __ballot(lane < n && tb[lane < n ? lane : 0] != 0);
+    }
+    __device__ __forceinline__ u64 bits(int t) const {
+        if (!mask) return low_bits(min(KT, lk - c0 - t * KT));
+        const u64 v = tb[t];                                   // (the same for every lane)
+        return ((u64)(u32)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)v);
+    }
+    static constexpr u64 FULL = KT == 64 ? ~0ull : 0xffffffffull;
+};
+__device__ __forceinline__ int next_tile(u64& alive) {         // the lowest tile left, taken out; -1: none
+    if (!alive) return -1;
+    const int t = __builtin_ctzll(alive);
+    alive &= alive - 1;
+    return t;
 }
-// the 64 keep flags of keys k0 .. k0 + 63
-__device__ __forceinline__ u64 key_bits(const unsigned char* mask, int k0, int lk, int lane) {
-    const int j = k0 + lane;
-    return __ballot(j < lk && (!mask || mask[j]));
+
+// part `sp` of `ns` of n rows in whole tiles: [from, to)
+struct Part { int from, to; };
+__device__ __forceinline__ Part part_of(int sp, int ns, int n, int tile) {
+    const int per = ((n + tile - 1) / tile + ns - 1) / ns * tile;
+    return Part{min(sp * per, n), min((sp + 1) * per, n)};
 }
-// head h's bias over distances, in units of log2: bl[d + R + BPAD], |d| <= R + BPAD
+
+// head h's bias over the distances lo .. hi, in units of log2: bl[d + R + BPAD]
 template <int NT>
-__device__ __forceinline__ void fill_bias(const RpArgs& a, int h, float* bl) {
-    for (int i = threadIdx.x; i < 2 * (a.R + BPAD) + 1; i += NT) {
-        const int d = min(max(i - BPAD, 0), 2 * a.R);
-        const int b = min(max(a.bucket[d], 0), a.nb - 1);
+__device__ __forceinline__ void fill_bias(const RpArgs& a, int h, float* bl, int lo, int hi) {
+    const int mid = a.R + BPAD, first = max(lo, -mid), last = min(hi, mid);
+    for (int d = first + (int)threadIdx.x; d <= last; d += NT) {
+        const int b = min(max(a.bucket[min(max(d, -a.R), a.R) + a.R], 0), a.nb - 1);
         const float t = a.table_bf16 ? __uint_as_float((u32)((const u16*)a.table)[(long long)b * a.heads + h] << 16)
                                      : ((const float*)a.table)[(long long)b * a.heads + h];
-        bl[i] = t * LOG2E;
+        bl[d + mid] = t * LOG2E;
     }
 }
 // bias of a 32 x 32 block: distances key - query with d0 = (first key) - (first query); near = the block touches |d| < R
@@ -138,24 +187,39 @@ template <bool KEY_LANE>
 __device__ __forceinline__ BlockBias block_bias(const float* bl, int R, int d0, int lane) {
     BlockBias x;
     x.near = d0 - 31 < R && d0 + 31 > -R;
-    x.c = bl[(d0 > 0 ? R : -R) + R + BPAD];
+    x.c = bl[(x.near ? 0 : d0 > 0 ? R : -R) + R + BPAD];
     // lane = query: d = d0 + key - lane, key = acc_r; lane = key: d = d0 + lane - query, query = acc_r
     x.p = bl + R + BPAD + (x.near ? d0 : 0) + (KEY_LANE ? (lane & 31) - 4 * (lane >> 5) : 4 * (lane >> 5) - (lane & 31));
     return x;
 }
+__device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 
-// ---- forward.  A wave owns 32 queries of one (text, head); NW waves share the staged keys.
-template <int NW>
-__global__ __launch_bounds__(NW * 64) void cfl_relpos_fwd_kernel(RpArgs a) {
-    constexpr int NT = NW * 64;
-    __shared__ __attribute__((aligned(16))) u16 Kt[KT * TP], Vt[KT * TP];
+// a lane's 32 values of its row in 32 bits: out [64]
+__device__ __forceinline__ void store_part(const f32x16 (&o)[2], float* out, int lane) {
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 v = {o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+            *reinterpret_cast<f32x4*>(out + 32 * dt + 8 * g + 4 * (lane >> 5)) = v;
+        }
+}
+
+// ---- forward.  A wave owns 32 queries of one (text, head); NW waves share the staged keys, KT at a time in NB buffers.
+template <int NW, int KT, int NB>
+__global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
+    constexpr int NT = NW * 64, U = KT / 32;
+    __shared__ __attribute__((aligned(16))) u16 Kt[NB][KT * TP], Vt[NB][KT * TP];
+    __shared__ u64 tb[64];
     extern __shared__ float bl[];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int qb = id % a.nqb, h = (id / a.nqb) % a.heads, b = id / (a.nqb * a.heads);
+    const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
-    fill_bias<NT>(a, h, bl);
-    const unsigned char* mask = a.mask ? a.mask + (long long)b * a.Lk : nullptr;
+    if (qb * NW * 32 >= t.lq) return;
+    const Part part = part_of(sp, a.ns, t.lk, KT);
+    fill_bias<NT>(a, h, bl, -(t.lq | (NW * 32 - 1)), t.lk | (KT - 1));     // (rows past the end are computed with as well)
+    Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
     for (int blk = qb; blk * NW * 32 < t.lq; blk += a.nqb) {
@@ -165,56 +229,92 @@ __global__ __launch_bounds__(NW * 64) void cfl_relpos_fwd_kernel(RpArgs a) {
         f32x16 o[2];
         zero16(o[0]); zero16(o[1]);
         float m = -INFINITY, l = 0.f;
-        for (int k0 = 0; k0 < t.lk; k0 += KT) {
-            const u64 bits = key_bits(mask, k0, t.lk, lane);
-            if (bits == 0) continue;                           // (the same for every wave of the workgroup)
-            __syncthreads();
-            stage<NT>(kp, a.ldk, k0, t.lk, mask, Kt);
-            stage<NT>(vp, a.ldk, k0, t.lk, mask, Vt);
-            __syncthreads();
-            f32x16 s[2];
-            float top = m;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                zero16(s[u]);
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Kt, 32 * u, kk, lane), qf[kk], s[u], 0, 0, 0);
-                const BlockBias bb = block_bias<false>(bl, a.R, k0 + 32 * u - q0, lane);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float bias = bb.near ? bb.p[(r & 3) + 8 * (r >> 2)] : bb.c;
-                    const float v = fmaf(s[u][r], a.scale2, bias);
-                    s[u][r] = (bits >> (32 * u + acc_r(r, lane))) & 1 ? v : -INFINITY;
-                    top = fmaxf(top, s[u][r]);
+        for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
+            keys.chunk(c0);
+            u64 left = keys.alive;
+            Stage<NT, KT> ks, vs;
+            int cur = next_tile(left);
+            if (cur < 0) continue;
+            u64 bits = keys.bits(cur);
+            ks.load(kp, a.ldk, c0 + cur * KT, bits);
+            vs.load(vp, a.ldk, c0 + cur * KT, bits);
+            int buf = 0;
+            __syncthreads();                                   // (the tiles' last readers, the bias vector)
+            ks.put(Kt[0]);
+            vs.put(Vt[0]);
+            while (true) {
+                const int k0 = c0 + cur * KT, nxt = next_tile(left);
+                u64 nbits = 0;
+                if (nxt >= 0) {
+                    nbits = keys.bits(nxt);
+                    ks.load(kp, a.ldk, c0 + nxt * KT, nbits);
+                    vs.load(vp, a.ldk, c0 + nxt * KT, nbits);
                 }
+                __syncthreads();
+                f32x16 s[U];
+                float top = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    zero16(s[u]);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Kt[buf], 32 * u, kk, lane), qf[kk], s[u], 0, 0, 0);
+                    const BlockBias bb = block_bias<false>(bl, a.R, k0 + 32 * u - q0, lane);
+                    if (bb.near) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, bb.p[(r & 3) + 8 * (r >> 2)]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, bb.c);
+                    }
+                    if (bits != Keys<NW, KT>::FULL) {
+                        const u32 mine = (u32)(bits >> (32 * u)) >> (4 * (lane >> 5));
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[u][r] = (mine >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[u][r] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+                }
+                top = half_max(top);
+                if (__any(top > m)) {                          // a new maximum somewhere in the wave: bring what is summed to it
+                    const float mn = fmaxf(m, top), shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+                    l *= shrink;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) { o[0][r] *= shrink; o[1][r] *= shrink; }
+                    m = mn;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - m);
+                        l += s[u][r];
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) {
+                        const bf16x8 p = pack_acc(s[u], kk);
+#pragma unroll
+                        for (int dt = 0; dt < 2; ++dt)
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Vt[buf], 32 * u + 16 * kk, dt, lane), p, o[dt], 0, 0, 0);
+                    }
+                }
+                if (nxt < 0) break;
+                if (NB == 1) __syncthreads(); else buf ^= 1;
+                ks.put(Kt[buf]);
+                vs.put(Vt[buf]);
+                cur = nxt;
+                bits = nbits;
             }
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float shrink = m == -INFINITY ? 0.f : exp2f(m - top);
-            l *= shrink;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) { o[0][r] *= shrink; o[1][r] *= shrink; }
-            m = top;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[u][r] = exp2f(s[u][r] - m);
-                    l += s[u][r];
-                }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    const bf16x8 p = pack_acc(s[u], kk);
-#pragma unroll
-                    for (int dt = 0; dt < 2; ++dt)
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Vt, 32 * u + 16 * kk, dt, lane), p, o[dt], 0, 0, 0);
-                }
         }
         l += __shfl_xor(l, 32, 64);
         const int row = q0 + (lane & 31);
-        if (row < t.lq) {
+        if (a.ns > 1) {
+            if (row < t.lq) {
+                const long long at = ((long long)sp * a.heads + h) * a.rows + t.q0 + row;
+                store_part(o, a.po + at * 64, lane);
+                if (lane < 32) { a.pm[2 * at] = m; a.pm[2 * at + 1] = l; }
+            }
+        } else if (row < t.lq) {
             const float inv = m == -INFINITY ? 0.f : 1.f / l;
             u16* op = a.out + (t.q0 + row) * a.ldo + h * 64 + 4 * (lane >> 5);
 #pragma unroll
@@ -226,7 +326,7 @@ __global__ __launch_bounds__(NW * 64) void cfl_relpos_fwd_kernel(RpArgs a) {
                     v.y = pack2(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
                     *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
                 }
-            if (a.lse && lane < 32) a.lse[h * a.rows + t.q0 + row] = m == -INFINITY ? INFINITY : m + log2f(l);
+            if (a.lse && lane < 32) a.lse[h * a.rows + t.q0 + row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l);
         }
     }
 }
@@ -244,27 +344,47 @@ __global__ __launch_bounds__(256) void cfl_relpos_tail_kernel(const int* __restr
 // ---- backward, queries: D, dQ and the bias gradient.  Same ownership as the forward.
 // The bias gradient of a distance is the sum of ds along a diagonal.  A lane's 16 values of a near block lie on 16 diagonals: each wave
 // adds them to LDS words of its own, one word per distance and lane half -- the addresses of one instruction are distinct and a wave's
-// LDS operations stay in order, so the sum's order is fixed.  Far blocks are summed in registers.
-template <int NW>
-__global__ __launch_bounds__(NW * 64) void cfl_relpos_dq_kernel(RpArgs a) {
-    constexpr int NT = NW * 64;
-    __shared__ __attribute__((aligned(16))) u16 Kt[KT * TP], Vt[KT * TP];
+// LDS operations stay in order, so the sum's order is fixed.  Far blocks are summed in registers.  At the end the workgroup's sums per
+// distance are gathered by bucket: part [heads][slots][nb], one slot per (text, query block).
+template <int NW, int KT, int NB>
+__global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
+    constexpr int NT = NW * 64, U = KT / 32;
+    __shared__ __attribute__((aligned(16))) u16 Kt[NB][KT * TP], Vt[NB][KT * TP];
+    __shared__ u64 tb[64];
     extern __shared__ float dyn[];
-    const int nd = 2 * (a.R + BPAD) + 1;
+    const int nd = 2 * (a.R + BPAD) + 1, mid = a.R + BPAD;
     float* bl = dyn;
     float* dg = dyn + nd;                                      // [2 NW][nd]
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int qb = id % a.nqb, h = (id / a.nqb) % a.heads, b = id / (a.nqb * a.heads);
+    const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
-    fill_bias<NT>(a, h, bl);
-    for (int i = threadIdx.x; i < 2 * NW * nd; i += NT) dg[i] = 0.f;
+    const Part part = part_of(sp, a.ns, t.lk, KT);
+    float* out = a.diag + ((((long long)h * a.B + b) * a.nqb + qb) * a.ns + sp) * a.nb;
+    if (qb * NW * 32 >= t.lq || t.lk == 0) {
+        for (int i = threadIdx.x; i < a.nb; i += NT) out[i] = 0.f;
+        if (t.lk == 0 && a.Lq)                                 // queries of their own without a key: no gradient
+            for (int i = threadIdx.x; i < t.lq * 8; i += NT) {
+                const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                if (a.ns == 1) {
+                    *reinterpret_cast<f32x4*>(a.dq + (t.q0 + (i >> 3)) * a.lddq + h * 64 + (i & 7) * 8) = z;
+                } else {
+                    float* p = a.po + (((long long)sp * a.heads + h) * a.rows + t.q0 + (i >> 3)) * 64 + (i & 7) * 8;
+                    *reinterpret_cast<f32x4*>(p) = z;
+                    *reinterpret_cast<f32x4*>(p + 4) = z;
+                }
+            }
+        return;
+    }
+    const int dlo = max(-(t.lq | (NW * 32 - 1)), -mid), dhi = min(t.lk | (KT - 1), mid);      // (rows past the end are computed with as well)
+    fill_bias<NT>(a, h, bl, dlo, dhi);
+    for (int c = 0; c < 2 * NW; ++c)
+        for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) dg[c * nd + d + mid] = 0.f;
     float far_lo = 0.f, far_hi = 0.f;
     float* mine = dg + (2 * w + (lane >> 5)) * nd;
-    const unsigned char* mask = a.mask ? a.mask + (long long)b * a.Lk : nullptr;
+    Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
-    __syncthreads();
     for (int blk = qb; blk * NW * 32 < t.lq; blk += a.nqb) {
         const int q0 = blk * NW * 32 + w * 32;
         const int row = q0 + (lane & 31);
@@ -282,56 +402,88 @@ __global__ __launch_bounds__(NW * 64) void cfl_relpos_dq_kernel(RpArgs a) {
                 for (int j = 0; j < 8; ++j) D = fmaf((float)of[kk][j], (float)gf[kk][j], D);
             D += __shfl_xor(D, 32, 64);
         }
-        const float lse = live ? a.lse[h * a.rows + t.q0 + row] : INFINITY;
-        if (live && lane < 32) a.dsum[h * a.rows + t.q0 + row] = D;
+        const float lse = live ? a.lse[h * a.rows + t.q0 + row] : INFINITY;      // (+inf: p = 0 in every row that does not count)
+        if (live && lane < 32 && sp == 0) a.dsum[h * a.rows + t.q0 + row] = D;
         f32x16 dq[2];
         zero16(dq[0]); zero16(dq[1]);
-        for (int k0 = 0; k0 < t.lk; k0 += KT) {
-            const u64 bits = key_bits(mask, k0, t.lk, lane);
-            if (bits == 0) continue;
+        for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
+            keys.chunk(c0);
+            u64 left = keys.alive;
+            Stage<NT, KT> ks, vs;
+            int cur = next_tile(left);
+            if (cur < 0) continue;
+            u64 bits = keys.bits(cur);
+            ks.load(kp, a.ldk, c0 + cur * KT, bits);
+            vs.load(vp, a.ldk, c0 + cur * KT, bits);
+            int buf = 0;
             __syncthreads();
-            stage<NT>(kp, a.ldk, k0, t.lk, mask, Kt);
-            stage<NT>(vp, a.ldk, k0, t.lk, mask, Vt);
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                f32x16 s, dp;
-                zero16(s); zero16(dp);
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Kt, 32 * u, kk, lane), qf[kk], s, 0, 0, 0);
-                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Vt, 32 * u, kk, lane), gf[kk], dp, 0, 0, 0);
+            ks.put(Kt[0]);
+            vs.put(Vt[0]);
+            while (true) {
+                const int k0 = c0 + cur * KT, nxt = next_tile(left);
+                u64 nbits = 0;
+                if (nxt >= 0) {
+                    nbits = keys.bits(nxt);
+                    ks.load(kp, a.ldk, c0 + nxt * KT, nbits);
+                    vs.load(vp, a.ldk, c0 + nxt * KT, nbits);
                 }
-                const int d0 = k0 + 32 * u - q0;
-                const BlockBias bb = block_bias<false>(bl, a.R, d0, lane);
-                float* dst = mine + (bb.p - bl);
+                __syncthreads();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float bias = bb.near ? bb.p[(r & 3) + 8 * (r >> 2)] : bb.c;
-                    const bool ok = live && ((bits >> (32 * u + acc_r(r, lane))) & 1);
-                    const float p = ok ? exp2f(fmaf(s[r], a.scale2, bias) - lse) : 0.f;
-                    s[r] = p == 0.f ? 0.f : p * (dp[r] - D);
+                for (int u = 0; u < U; ++u) {
+                    f32x16 s, dp;
+                    zero16(s); zero16(dp);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Kt[buf], 32 * u, kk, lane), qf[kk], s, 0, 0, 0);
+                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Vt[buf], 32 * u, kk, lane), gf[kk], dp, 0, 0, 0);
+                    }
+                    const int d0 = k0 + 32 * u - q0;
+                    const BlockBias bb = block_bias<false>(bl, a.R, d0, lane);
+                    if (bb.near) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], a.scale2, bb.p[(r & 3) + 8 * (r >> 2)] - lse);
+                    } else {
+                        const float c = bb.c - lse;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], a.scale2, c);
+                    }
+                    if (bits != Keys<NW, KT>::FULL) {
+                        const u32 in = (u32)(bits >> (32 * u)) >> (4 * (lane >> 5));
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[r] = (in >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - D);
+                    if (bb.near) {
+                        float* dst = mine + (bb.p - bl);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            __hip_atomic_fetch_add(dst + (r & 3) + 8 * (r >> 2), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    } else {
+                        float x = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x += s[r];
+                        if (d0 > 0) far_hi += x; else far_lo += x;
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) {
+                        const bf16x8 p = pack_acc(s, kk);
+#pragma unroll
+                        for (int dt = 0; dt < 2; ++dt)
+                            dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Kt[buf], 32 * u + 16 * kk, dt, lane), p, dq[dt], 0, 0, 0);
+                    }
                 }
-                if (bb.near) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        __hip_atomic_fetch_add(dst + (r & 3) + 8 * (r >> 2), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                } else {
-                    float x = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x += s[r];
-                    if (d0 > 0) far_hi += x; else far_lo += x;
-                }
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    const bf16x8 p = pack_acc(s, kk);
-#pragma unroll
-                    for (int dt = 0; dt < 2; ++dt)
-                        dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Kt, 32 * u + 16 * kk, dt, lane), p, dq[dt], 0, 0, 0);
-                }
+                if (nxt < 0) break;
+                if (NB == 1) __syncthreads(); else buf ^= 1;
+                ks.put(Kt[buf]);
+                vs.put(Vt[buf]);
+                cur = nxt;
+                bits = nbits;
             }
         }
-        if (live) {
+        if (a.ns > 1) {
+            if (live) store_part(dq, a.po + (((long long)sp * a.heads + h) * a.rows + t.q0 + row) * 64, lane);
+        } else if (live) {
             u16* op = a.dq + (t.q0 + row) * a.lddq + h * 64 + 4 * (lane >> 5);
 #pragma unroll
             for (int dt = 0; dt < 2; ++dt)
@@ -344,95 +496,134 @@ __global__ __launch_bounds__(NW * 64) void cfl_relpos_dq_kernel(RpArgs a) {
                 }
         }
     }
-    // the workgroup's sums per distance, clipped to +-Rr
+    // the workgroup's sums per distance ...
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
-    if (lane == 0) {                                           // (distances at the vector's ends belong to +-R as well)
-        dg[2 * w * nd] += far_lo;
-        dg[2 * w * nd + nd - 1] += far_hi;
+    if (lane == 0) {                                           // (far blocks exist only where the range reaches beyond +-R)
+        if (dlo <= -a.R) dg[2 * w * nd + mid - a.R] += far_lo;
+        if (dhi >= a.R) dg[2 * w * nd + mid + a.R] += far_hi;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < nd; i += NT) {
+    for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) {
         float x = 0.f;
 #pragma unroll
-        for (int c = 0; c < 2 * NW; ++c) x += dg[c * nd + i];
-        dg[i] = x;                                             // (read above by this thread alone)
+        for (int c = 0; c < 2 * NW; ++c) x += dg[c * nd + d + mid];
+        dg[d + mid] = x;                                       // (read above by this thread alone)
+        bl[d + mid] = __int_as_float(min(max(a.bucket[min(max(d, -a.R), a.R) + a.R], 0), a.nb - 1));      // the bias is not read any more
     }
     __syncthreads();
-    float* out = a.diag + ((long long)h * a.B * a.nqb + (long long)b * a.nqb + qb) * (2 * a.Rr + 1);
-    const int mid = a.R + BPAD;
-    for (int i = threadIdx.x; i < 2 * a.Rr + 1; i += NT) {
-        float x = dg[mid - a.Rr + i];
-        if (i == 0) for (int j = mid - a.Rr - 1; j >= 0; --j) x += dg[j];
-        if (i == 2 * a.Rr) for (int j = mid + a.Rr + 1; j < nd; ++j) x += dg[j];
-        out[i] = x;
+    // ... and per bucket: L lanes each
+    int L = 1;
+    while (L < 64 && 2 * L * a.nb <= NT) L *= 2;
+    for (int b0 = 0; b0 < a.nb; b0 += NT / L) {
+        const int bk = b0 + threadIdx.x / L;
+        float x = 0.f;
+        for (int d = dlo + (int)(threadIdx.x % L); d <= dhi; d += L) x += __float_as_int(bl[d + mid]) == bk ? dg[d + mid] : 0.f;
+        for (int o = L >> 1; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+        if (bk < a.nb && threadIdx.x % L == 0) out[bk] = x;
     }
 }
 
 // ---- backward, keys: dK and dV.  A wave owns 32 keys; the staged rows are queries.
-template <int NW>
-__global__ __launch_bounds__(NW * 64) void cfl_relpos_dkv_kernel(RpArgs a, int nkb) {
-    constexpr int NT = NW * 64;
-    __shared__ __attribute__((aligned(16))) u16 Qt[KT * TP], Gt[KT * TP];
-    __shared__ float ls[KT], ds[KT];
+template <int NW, int KT, int NB>
+__global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, int nkb) {
+    constexpr int NT = NW * 64, U = KT / 32;
+    __shared__ __attribute__((aligned(16))) u16 Qt[NB][KT * TP], Gt[NB][KT * TP];
+    __shared__ __attribute__((aligned(16))) float ls[NB][KT], ds[NB][KT];
     extern __shared__ float bl[];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int kb = id % nkb, h = (id / nkb) % a.heads, b = id / (nkb * a.heads);
+    const int sp = id % a.ns, kb = id / a.ns % nkb, h = id / (a.ns * nkb) % a.heads, b = id / (a.ns * nkb * a.heads);
     const Text t = text_of(a, b);
-    fill_bias<NT>(a, h, bl);
+    if (kb * NW * 32 >= t.lk) return;
+    const Part part = part_of(sp, a.ns, t.lq, KT);
+    fill_bias<NT>(a, h, bl, -(t.lq | (KT - 1)), t.lk | (NW * 32 - 1));
     const unsigned char* mask = a.mask ? a.mask + (long long)b * a.Lk : nullptr;
     const u16* qp = a.q + t.q0 * a.ldq + h * 64;
     const u16* gp = a.dout + t.q0 * a.ldo + h * 64;
+    const float* lp = a.lse + h * a.rows + t.q0;
+    const float* dp_ = a.dsum + h * a.rows + t.q0;
     for (int blk = kb; blk * NW * 32 < t.lk; blk += nkb) {
         const int k0 = blk * NW * 32 + w * 32;
         const int key = k0 + (lane & 31);
         const bool live = key < t.lk && (!mask || mask[key]);
-        bf16x8 kf[4], vf[4];
-        load_rows(a.k + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, kf);
-        load_rows(a.v + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, vf);
         f32x16 dk[2], dv[2];
         zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]);
-        for (int q0 = 0; q0 < t.lq; q0 += KT) {
-            __syncthreads();
-            stage<NT>(qp, a.ldq, q0, t.lq, nullptr, Qt);
-            stage<NT>(gp, a.ldo, q0, t.lq, nullptr, Gt);
-            for (int i = threadIdx.x; i < KT; i += NT) {
-                const bool in = q0 + i < t.lq;
-                ls[i] = in ? a.lse[h * a.rows + t.q0 + q0 + i] : INFINITY;
-                ds[i] = in ? a.dsum[h * a.rows + t.q0 + q0 + i] : 0.f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                f32x16 s, dp;
-                zero16(s); zero16(dp);
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Qt, 32 * u, kk, lane), kf[kk], s, 0, 0, 0);
-                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Gt, 32 * u, kk, lane), vf[kk], dp, 0, 0, 0);
+        if (__syncthreads_or(live) && part.from < part.to) {   // (else no key of the workgroup takes part: zeros)
+            bf16x8 kf[4], vf[4];
+            load_rows(a.k + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, kf);
+            load_rows(a.v + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, vf);
+            Stage<NT, KT> qs, gs;
+            float lr = 0.f, dr = 0.f;
+            const auto fetch = [&](int q0) {
+                const u64 bits = low_bits(part.to - q0);
+                qs.load(qp, a.ldq, q0, bits);
+                gs.load(gp, a.ldo, q0, bits);
+                if (threadIdx.x < KT) {
+                    const bool in = q0 + (int)threadIdx.x < part.to;
+                    lr = in ? lp[q0 + threadIdx.x] : INFINITY;
+                    dr = in ? dp_[q0 + threadIdx.x] : 0.f;
                 }
-                const BlockBias bb = block_bias<true>(bl, a.R, k0 - q0 - 32 * u, lane);
+            };
+            const auto put = [&](int buf) {
+                qs.put(Qt[buf]);
+                gs.put(Gt[buf]);
+                if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
+            };
+            fetch(part.from);
+            int buf = 0;
+            put(0);
+            for (int q0 = part.from; ; ) {
+                const bool more = q0 + KT < part.to;
+                if (more) fetch(q0 + KT);
+                __syncthreads();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = 32 * u + acc_r(r, lane);
-                    const float bias = bb.near ? bb.p[-((r & 3) + 8 * (r >> 2))] : bb.c;
-                    const float p = live ? exp2f(fmaf(s[r], a.scale2, bias) - ls[i]) : 0.f;
-                    s[r] = p;
-                    dp[r] = p == 0.f ? 0.f : p * (dp[r] - ds[i]);
-                }
+                for (int u = 0; u < U; ++u) {
+                    f32x16 s, dp;
+                    zero16(s); zero16(dp);
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    const bf16x8 p = pack_acc(s, kk), g = pack_acc(dp, kk);
+                    for (int kk = 0; kk < 4; ++kk) {
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Qt[buf], 32 * u, kk, lane), kf[kk], s, 0, 0, 0);
+                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Gt[buf], 32 * u, kk, lane), vf[kk], dp, 0, 0, 0);
+                    }
+                    const BlockBias bb = block_bias<true>(bl, a.R, k0 - q0 - 32 * u, lane);
 #pragma unroll
-                    for (int dt = 0; dt < 2; ++dt) {
-                        dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Gt, 32 * u + 16 * kk, dt, lane), p, dv[dt], 0, 0, 0);
-                        dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Qt, 32 * u + 16 * kk, dt, lane), g, dk[dt], 0, 0, 0);
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
+                        const f32x4 D = *reinterpret_cast<const f32x4*>(&ds[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = 4 * g + j;
+                            const float bias = bb.near ? bb.p[-(j + 8 * g)] : bb.c;
+                            const float p = live ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bias - lse[j])) : 0.f;
+                            s[r] = p;
+                            dp[r] = live ? p * (dp[r] - D[j]) : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) {
+                        const bf16x8 p = pack_acc(s, kk), g = pack_acc(dp, kk);
+#pragma unroll
+                        for (int dt = 0; dt < 2; ++dt) {
+                            dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Gt[buf], 32 * u + 16 * kk, dt, lane), p, dv[dt], 0, 0, 0);
+                            dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Qt[buf], 32 * u + 16 * kk, dt, lane), g, dk[dt], 0, 0, 0);
+                        }
                     }
                 }
+                if (!more) break;
+                if (NB == 1) __syncthreads(); else buf ^= 1;
+                put(buf);
+                q0 += KT;
             }
         }
-        if (key < t.lk) {
+        if (a.ns > 1) {
+            if (key < t.lk) {
+                if (!live) { zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]); }
+                const long long at = (((long long)sp * a.heads + h) * a.krows + t.k0 + key) * 64;
+                store_part(dk, a.po + at, lane);
+                store_part(dv, a.pv + at, lane);
+            }
+        } else if (key < t.lk) {
             u16* kq = a.dk + (t.k0 + key) * a.lddk + h * 64 + 4 * (lane >> 5);
             u16* vq = a.dv + (t.k0 + key) * a.lddk + h * 64 + 4 * (lane >> 5);
 #pragma unroll
@@ -451,54 +642,124 @@ __global__ __launch_bounds__(NW * 64) void cfl_relpos_dkv_kernel(RpArgs a, int n
     }
 }
 
-// ---- dtable[bucket][h]: the sums of the bucket's distances over all workgroups of the dQ kernel, in a fixed order.  grid = (nb, heads)
-__global__ __launch_bounds__(256) void cfl_relpos_dtable_kernel(const float* __restrict__ diag, const int* __restrict__ bucket, int R, int Rr,
-                                                                int nb, int heads, long long slots, void* dtable, int bf16) {
-    __shared__ float red[4];
-    const int b = blockIdx.x, h = blockIdx.y, nd = 2 * Rr + 1;
-    float x = 0.f;
-    for (int i = 0; i < nd; ++i) {
-        if (min(max(bucket[R - Rr + i], 0), nb - 1) != b) continue;
-        for (long long s = threadIdx.x; s < slots; s += 256) x += diag[(h * slots + s) * nd + i];
+// ---- joins of the parts: a wave per (row, head), a lane per d
+__global__ __launch_bounds__(256) void cfl_relpos_join_kernel(const float* __restrict__ po, const float* __restrict__ pm, int ns, int heads,
+                                                              long long rows, long long last, const int* __restrict__ end, u16* o, long long ldo,
+                                                              float* __restrict__ lse) {
+    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const long long row = i / heads, h = i % heads;
+    if (row >= min(rows, end ? (long long)max(*end, 0) : last)) return;
+    float m = -INFINITY;
+    for (int s = 0; s < ns; ++s) m = fmaxf(m, pm[2 * ((s * heads + h) * rows + row)]);
+    float l = 0.f, x = 0.f;
+    for (int s = 0; s < ns; ++s) {
+        const long long at = (s * heads + h) * rows + row;
+        const float ms = pm[2 * at], c = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+        l = fmaf(pm[2 * at + 1], c, l);
+        if (c != 0.f) x = fmaf(po[at * 64 + lane], c, x);
     }
-    x = block_sum_256(x, red);
-    if (threadIdx.x == 0) {
+    reinterpret_cast<__bf16*>(o)[row * ldo + h * 64 + lane] = (__bf16)(m == -INFINITY ? 0.f : x / l);
+    if (lse && lane == 0) lse[h * rows + row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+__global__ __launch_bounds__(256) void cfl_relpos_join_sum_kernel(const float* __restrict__ po, int ns, int heads, long long rows, long long last,
+                                                                  const int* __restrict__ end, float scale, u16* o, long long ldo) {
+    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const long long row = i / heads, h = i % heads;
+    if (row >= min(rows, end ? (long long)max(*end, 0) : last)) return;
+    float x = 0.f;
+    for (int s = 0; s < ns; ++s) x += po[((s * heads + h) * rows + row) * 64 + lane];
+    reinterpret_cast<__bf16*>(o)[row * ldo + h * 64 + lane] = (__bf16)(x * scale);
+}
+
+// ---- dtable[bucket][h]: the slots' sums, in a fixed order.  grid = (ceil(nb / 32), heads): 32 buckets x 8 strands of slots
+__global__ __launch_bounds__(256) void cfl_relpos_dtable_kernel(const float* __restrict__ part, int nb, int heads, long long slots, void* dtable,
+                                                                int bf16) {
+    __shared__ float red[8][32];
+    const int h = blockIdx.y, b = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
+    float x = 0.f;
+    if (b < nb) {
+        const float* p = part + (long long)h * slots * nb + b;
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        long long s = strand;
+        for (; s + 24 < slots; s += 32)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] += p[(s + 8 * k) * nb];
+        for (; s < slots; s += 8) y[0] += p[s * nb];
+        x = (y[0] + y[1]) + (y[2] + y[3]);
+    }
+    red[strand][threadIdx.x & 31] = x;
+    __syncthreads();
+    if (strand == 0 && b < nb) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) x += red[k][threadIdx.x];
         if (bf16) ((__bf16*)dtable)[b * heads + h] = (__bf16)x;
         else ((float*)dtable)[b * heads + h] = x;
     }
 }
 
-// waves per workgroup: texts of at most one wave's rows get workgroups of one wave
-inline int rp_waves(int L) { return L <= 32 ? 1 : 4; }
-inline int rp_blocks(int L) { return cfl_cdiv(L, 32 * rp_waves(L)); }
-
-// distances that can occur, at most R (packed texts: whatever their lengths are)
-inline int rp_reach(int Lq, int Lk, int T, int R) {
-    const int far = (T > 0 ? (T > Lq ? T : Lq) : (Lq > Lk ? Lq : Lk)) - 1;
-    return R < far ? R : far;
+// Launch shape for `L` rows that waves own (32 each) against `K` rows that are passed over, for every (text, head).
+struct Shape { int nw, kt, blocks, ns; };
+inline Shape rp_shape(long long BH, int L, int K) {
+    Shape p;
+    p.kt = K <= 32 ? 32 : 64;
+    const long long waves = BH * cfl_cdiv(L, 32);
+    // few waves against a long axis: split it, into parts of four tiles at least, until every SIMD has a wave
+    long long ns = 1024 / waves;
+    const int most = K / 256 < 16 ? K / 256 : 16;
+    p.ns = (int)(ns > most ? most : ns);
+    if (p.ns < 1) p.ns = 1;
+    // four waves share what is staged, where that leaves a workgroup for every CU
+    p.nw = L > 32 && BH * cfl_cdiv(L, 128) * p.ns >= 256 ? 4 : 1;
+    p.blocks = cfl_cdiv(L, 32 * p.nw);
+    return p;
 }
 
 inline int rp_check(const RpArgs& a, int head_dim) {
     if (!a.q || !a.k || !a.v || !a.table || !a.bucket || a.B < 1 || a.Lq < 0 || a.Lk < 1 || a.heads < 1 || a.nb < 1 || a.R < 0 ||
         (a.cu ? a.T < 1 || a.mask != nullptr : a.Lq < 1)) return CFL_EINVAL;
     if (a.ldq % 8 || a.ldk % 8 || a.ldo % 8 || (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15)) return CFL_EALIGN;
+    const int L = a.Lq > a.Lk ? a.Lq : a.Lk;
     if (head_dim != 64 || a.R > MAXR || a.heads > 65535 || a.nb > 65535 ||
-        (long long)a.B * a.heads * rp_blocks(a.Lq > a.Lk ? a.Lq : a.Lk) > 0x7fffffffll) return CFL_ELIMIT;
+        (long long)a.B * a.heads * (cfl_cdiv(L, 32) + 16) > 0x7fffffffll) return CFL_ELIMIT;
     return 0;
+}
+
+#define RP_LAUNCH(ID, KERN, P, LDS1, ...)                                                                                              \
+    do {                                                                                                                               \
+        const dim3 grid_((unsigned)((long long)a.B * a.heads * (P).blocks * (P).ns));                                                  \
+        if ((P).nw == 4 && (P).kt == 64) { CFL_LAUNCH(ID, (KERN<4, 64, 2>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }         \
+        else if ((P).nw == 4) { CFL_LAUNCH(ID, (KERN<4, 32, 1>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }                    \
+        else if ((P).kt == 64) { CFL_LAUNCH(ID, (KERN<1, 64, 1>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                    \
+        else { CFL_LAUNCH(ID, (KERN<1, 32, 1>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                                      \
+    } while (0)
+
+inline size_t rp_part_bytes(const Shape& p, int heads, long long rows) {
+    return p.ns > 1 ? cfl_align256((size_t)p.ns * heads * rows * 64 * 4) : 0;
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t cfl_relpos_ws_bytes(int B, int Lq, int Lk, int T, int heads, int R) {
-    if (B < 1 || Lq < 0 || Lk < 1 || T < 0 || (Lq == 0 && T == 0) || heads < 1 || R < 0 || R > MAXR) return 0;
-    return (size_t)B * heads * rp_blocks(Lq ? Lq : Lk) * (2 * rp_reach(Lq, Lk, T, R) + 1) * 4;
+size_t cfl_relpos_fwd_ws_bytes(int B, int Lq, int Lk, int T, int heads) {
+    if (B < 1 || Lq < 0 || Lk < 1 || T < 0 || heads < 1 || (Lq == 0 && T == 0)) return 0;
+    const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk);
+    const long long rows = Lq ? (long long)B * Lq : T;
+    return p.ns > 1 ? rp_part_bytes(p, heads, rows) + (size_t)p.ns * heads * rows * 2 * 4 : 0;
+}
+
+size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb) {
+    if (B < 1 || Lq < 0 || Lk < 1 || T < 0 || heads < 1 || nb < 1 || (Lq == 0 && T == 0)) return 0;
+    const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk), k = rp_shape((long long)B * heads, Lk, Lq ? Lq : Lk);
+    const long long rows = Lq ? (long long)B * Lq : T, krows = T ? T : (long long)B * Lk;
+    return cfl_align256((size_t)B * heads * p.blocks * p.ns * nb * 4) + rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
 }
 
 int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
                    int B, int Lq, int Lk, int T, int heads, int head_dim, float scale, const void* table, int table_bf16, int nb,
-                   const int* bucket, int R, void* o, long long ldo, float* lse, void* stream_) {
+                   const int* bucket, int R, void* o, long long ldo, float* lse, void* ws, void* stream_) {
     RpArgs a{};
     a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.ldq = ldq; a.ldk = ldk; a.ldo = ldo; a.out = (u16*)o;
     a.mask = mask; a.cu = cu; a.B = B; a.Lq = Lq; a.Lk = Lk; a.T = T; a.heads = heads; a.scale = scale; a.scale2 = scale * LOG2E;
@@ -506,15 +767,20 @@ int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, l
     a.rows = Lq ? (long long)B * Lq : T;
     const int rc = rp_check(a, head_dim);
     if (rc) return rc;
-    if (!o) return CFL_EINVAL;
+    const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk);
+    if (!o || (p.ns > 1 && !ws)) return CFL_EINVAL;
     if ((uintptr_t)o & 15) return CFL_EALIGN;
     hipStream_t stream = (hipStream_t)stream_;
-    const int L = Lq ? Lq : Lk;
-    a.nqb = rp_blocks(L);
-    const dim3 grid((unsigned)(B * heads * a.nqb));
+    a.nqb = p.blocks; a.ns = p.ns;
+    a.po = (float*)ws;
+    a.pm = (float*)((char*)ws + rp_part_bytes(p, heads, a.rows));
     const size_t lds = (2 * (R + BPAD) + 1) * 4;
-    if (rp_waves(L) == 1) { CFL_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel<1>, grid, dim3(64), lds, stream, a); }
-    else { CFL_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel<4>, grid, dim3(256), lds, stream, a); }
+#define RP_LDS(NW) lds
+    RP_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel, p, RP_LDS, a);
+#undef RP_LDS
+    if (p.ns > 1)
+        CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_kernel, dim3((unsigned)((a.rows * heads + 3) / 4)), dim3(256), 0, stream, a.po, a.pm, p.ns, heads,
+                   a.rows, a.rows, cu && !Lq ? cu + B : (const int*)nullptr, (u16*)o, ldo, lse);
     if (cu && !Lq) CFL_LAUNCH(K_RELPOS_TAIL, cfl_relpos_tail_kernel, dim3(64), dim3(256), 0, stream, cu, B, T, (u16*)o, ldo, heads * 64);
     return 0;
 }
@@ -529,23 +795,44 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     a.mask = mask; a.cu = cu; a.B = B; a.Lq = Lq; a.Lk = Lk; a.T = T; a.heads = heads; a.scale = scale; a.scale2 = scale * LOG2E;
     a.table = table; a.table_bf16 = table_bf16; a.nb = nb; a.R = R; a.bucket = bucket; a.lse = const_cast<float*>(lse); a.dsum = dsum;
     a.rows = Lq ? (long long)B * Lq : T;
+    a.krows = cu ? T : (long long)B * Lk;
     const int rc = rp_check(a, head_dim);
     if (rc) return rc;
     if (!o || !dout || !lse || !dsum || !dq || !dk || !dv || !dtable || !ws) return CFL_EINVAL;
     if (lddq % 8 || lddk % 8 || (((uintptr_t)o | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15)) return CFL_EALIGN;
     hipStream_t stream = (hipStream_t)stream_;
     const int L = Lq ? Lq : Lk;
-    a.Rr = rp_reach(Lq, Lk, cu ? T : 0, R);
-    a.diag = (float*)ws;
-    a.nqb = rp_blocks(L);
-    const int nkb = rp_blocks(Lk), nd = 2 * (R + BPAD) + 1;
-    const dim3 gq((unsigned)(B * heads * a.nqb)), gk((unsigned)(B * heads * nkb));
-    if (rp_waves(L) == 1) { CFL_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel<1>, gq, dim3(64), (size_t)nd * 3 * 4, stream, a); }
-    else { CFL_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel<4>, gq, dim3(256), (size_t)nd * 9 * 4, stream, a); }
-    if (rp_waves(Lk) == 1) { CFL_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel<1>, gk, dim3(64), (size_t)nd * 4, stream, a, nkb); }
-    else { CFL_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel<4>, gk, dim3(256), (size_t)nd * 4, stream, a, nkb); }
-    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(nb, heads), dim3(256), 0, stream, a.diag, bucket, R, a.Rr, nb, heads,
-               (long long)B * a.nqb, dtable, table_bf16);
+    const Shape p = rp_shape((long long)B * heads, L, Lk), kp = rp_shape((long long)B * heads, Lk, L);
+    const size_t bl = (2 * (R + BPAD) + 1) * 4;
+    char* at = (char*)ws;
+    a.diag = (float*)at;
+    at += cfl_align256((size_t)B * heads * p.blocks * p.ns * nb * 4);
+    a.po = (float*)at;
+    at += rp_part_bytes(p, heads, a.rows);
+    a.nqb = p.blocks; a.ns = p.ns;
+#define RP_LDS(NW) bl * (1 + 2 * (NW))
+    RP_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel, p, RP_LDS, a);
+#undef RP_LDS
+    const int* qend = cu && !Lq ? cu + B : nullptr;
+    if (p.ns > 1)
+        CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, dim3((unsigned)((a.rows * heads + 3) / 4)), dim3(256), 0, stream, a.po, p.ns, heads,
+                   a.rows, a.rows, qend, scale, (u16*)dq, lddq);
+    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(cfl_cdiv(nb, 32), heads), dim3(256), 0, stream, a.diag, nb, heads,
+               (long long)B * p.blocks * p.ns, dtable, table_bf16);
+    a.po = (float*)at;
+    a.pv = (float*)(at + rp_part_bytes(kp, heads, a.krows));
+    a.ns = kp.ns;
+#define RP_LDS(NW) bl
+    RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, RP_LDS, a, kp.blocks);
+#undef RP_LDS
+    if (kp.ns > 1) {
+        const dim3 g((unsigned)((a.krows * heads + 3) / 4));
+        const int* kend = cu ? cu + B : nullptr;
+        CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, g, dim3(256), 0, stream, a.po, kp.ns, heads, a.krows, a.krows, kend, scale, (u16*)dk,
+                   lddk);
+        CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, g, dim3(256), 0, stream, a.pv, kp.ns, heads, a.krows, a.krows, kend, 1.f, (u16*)dv,
+                   lddk);
+    }
     if (cu) {
         if (!Lq) CFL_LAUNCH(K_RELPOS_TAIL, cfl_relpos_tail_kernel, dim3(64), dim3(256), 0, stream, cu, B, T, (u16*)dq, lddq, heads * 64);
         CFL_LAUNCH(K_RELPOS_TAIL, cfl_relpos_tail_kernel, dim3(64), dim3(256), 0, stream, cu, B, T, (u16*)dk, lddk, heads * 64);

@@ -24,9 +24,9 @@ static const char* const g_kernel_names[K_NUM] = {
     "cfl_conv3x3_wgrad_kernel", "cfl_conv3x3_wgrad_reduce_kernel", "cfl_conv1x1_wgrad_kernel", "cfl_conv1x1_wgrad_reduce_kernel",
     "cfl_conv3x3_x3_kernel", "cfl_conv3x3_x3_wgrad_kernel", "cfl_conv3x3_x3_wgrad_reduce_kernel", "cfl_conv3x3_wimage_kernel",
     "cfl_pair_bwd_reduce_kernel",
-    "cfl_dropout_kernel", "cfl_gn_stats_kernel", "cfl_gn_apply_kernel", "cfl_gn_bwd_reduce_kernel", "cfl_gn_bwd_apply_kernel",
+    "cfl_dropout_kernel", "cfl_gn_res_kernel", "cfl_gn_stats_kernel", "cfl_gn_apply_kernel", "cfl_gn_bwd_reduce_kernel", "cfl_gn_bwd_apply_kernel",
     "cfl_gn_bwd_final_kernel",
-    "cfl_relpos_fwd_kernel", "cfl_relpos_tail_kernel", "cfl_relpos_dq_kernel", "cfl_relpos_dkv_kernel", "cfl_relpos_dtable_kernel",
+    "cfl_relpos_fwd_kernel", "cfl_relpos_join_kernel", "cfl_relpos_tail_kernel", "cfl_relpos_dq_kernel", "cfl_relpos_dkv_kernel", "cfl_relpos_dtable_kernel",
 };
 
 namespace {

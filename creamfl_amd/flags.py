@@ -26,7 +26,11 @@ BUILD_FLAGS = {
     'bucket_mb': (dict(type=int, default=32),
                   'multi-GPU: size of a gradient all-reduce bucket in MB (overlap granularity of the encoder-gradient all-reduce)'),
     'cnn_type': (dict(type=str, default=None), 'override the server image trunk (resnet18 / resnet50 / resnet101 / vit_b16)'),
-    'bert_name': (dict(type=str, default=None), 'override the server text trunk (bert-mini / bert-base / bert-large)'),
+    'bert_name': (dict(type=str, default=None), 'override the server text trunk (bert-mini / bert-base / bert-large; bert-mini-relative / '
+                  'bert-base-relative: a learned bias of the distance on the attention scores instead of absolute positions)'),
+    'image_norm': (dict(type=str, default='batch', choices=['batch', 'group']),
+                   'normalisation of the ResNet image encoders, server and clients: batch = the reference\'s; group = GroupNorm(32), whose '
+                   'statistics are per sample (batch statistics do not average over clients with different label distributions)'),
     'image_size': (dict(type=int, default=224), 'side of the synthetic images when no loaders are passed'),
     'test_pairs': (dict(type=int, default=5000), 'captions of the synthetic test set when no loaders are passed'),
     'quiet': (dict(action='store_true'), 'no console logging'),

@@ -71,6 +71,47 @@ class BNAct(nn.BatchNorm2d):
         return (y, y) if two else y
 
 
+class GNAct(nn.GroupNorm):
+    """GroupNorm(groups, channels) with BNAct's calling surface -- `gn(x, residual, relu, two)` -- for trunks whose normalisation must not
+    depend on the batch (clients with different label distributions: batch statistics do not average, group statistics are per sample).
+    Same parameters / state_dict as nn.GroupNorm.  channels_last bf16 / fp32 activations on the GPU run on csrc/gnorm.hip, training and
+    evaluation alike; any other input takes the library path."""
+
+    def __init__(self, num_channels, num_groups=32):
+        super().__init__(num_groups, num_channels)
+
+    def forward(self, x, residual=None, relu=False, two=False):
+        from .. import ops
+        if ops.gn_act_supported(x, self.num_channels, self.num_groups):
+            return ops.gn_act(x, self.weight, self.bias, self.num_groups, self.eps, 'relu' if relu else 'none', residual, two)
+        y = super().forward(x)
+        if residual is not None:
+            y = y + residual
+        y = F.relu(y) if relu else y
+        return (y, y) if two else y
+
+
+NORMS = {'batch': BNAct, 'group': GNAct}
+
+
+def norm_layer(kind):
+    """The trunks' normalisation by name: 'batch' (what the reference uses) or 'group'."""
+    if kind not in NORMS:
+        raise ValueError(f"unknown normalisation {kind!r}: 'batch' or 'group'")
+    return NORMS[kind]
+
+
+class CounterDropout(nn.Dropout):
+    """nn.Dropout on the counter-based generator (ops.dropout: no stored mask, replays of a captured step vary with ops.dropout_tick); any
+    other input takes the library path."""
+
+    def forward(self, x):
+        if self.training and x.is_cuda and x.dtype in (torch.float32, torch.bfloat16, torch.float16):
+            from .. import ops
+            return ops.dropout(x, self.p)
+        return super().forward(x)
+
+
 class TrunkConv(nn.Conv2d):
     """nn.Conv2d(cin, cout, k, stride, padding, bias=False) of the ResNet trunks.  On the channels_last GPU training
     path the backward is split (ops.conv_split): data gradient on the critical path -- for 1x1 / stride-1 kernels on the
@@ -139,6 +180,8 @@ def stem_tail(bn, pool, x):
     """maxpool(relu(bn(x))) of a ResNet stem: BatchNorm + ReLU + max pooling in one pass per direction where the fused kernels apply
     (training mode, channels_last bf16 / fp32 on the GPU), the two modules otherwise."""
     from .. import ops
+    if isinstance(bn, GNAct):
+        return pool(bn(x, relu=True))
     if (bn.training and bn.track_running_stats and bn.momentum is not None and bn.affine
             and isinstance(pool, MaxPool3s2) and ops.bn_relu_maxpool_supported(x, bn.num_features)):
         if torch.cuda.is_current_stream_capturing():          # (as BNAct.forward: inside a HIP-graph capture the count lives on the device)
@@ -158,13 +201,14 @@ def first_of(x):
 class BasicBlock(nn.Module):
     expansion = 1
 
-    def __init__(self, inplanes, planes, stride=1, downsample=None):
+    def __init__(self, inplanes, planes, stride=1, downsample=None, norm='batch'):
         super().__init__()
+        norm = norm_layer(norm)
         self.conv1 = TrunkConv(inplanes, planes, 3, stride, 1)
-        self.bn1 = BNAct(planes)
+        self.bn1 = norm(planes)
         self.relu = nn.ReLU(inplace=True)
         self.conv2 = TrunkConv(planes, planes, 3, 1, 1)
-        self.bn2 = BNAct(planes)
+        self.bn2 = norm(planes)
         self.downsample = downsample
         self.stride = stride
 
@@ -178,15 +222,16 @@ class BasicBlock(nn.Module):
 class Bottleneck(nn.Module):
     expansion = 4
 
-    def __init__(self, inplanes, planes, stride=1, downsample=None):
+    def __init__(self, inplanes, planes, stride=1, downsample=None, norm='batch'):
         super().__init__()
+        norm = norm_layer(norm)
         self.conv1 = Conv1x1(inplanes, planes)
-        self.bn1 = BNAct(planes)
+        self.bn1 = norm(planes)
         self.conv2 = TrunkConv(planes, planes, 3, stride, 1)                 # stride on the 3x3 (torchvision v1.5)
-        self.bn2 = BNAct(planes)
+        self.bn2 = norm(planes)
         self.conv3 = Conv1x1(planes, planes * 4)
-        self.conv3.bn_follows = True
-        self.bn3 = BNAct(planes * 4)
+        self.conv3.bn_follows = norm is BNAct
+        self.bn3 = norm(planes * 4)
         self.relu = nn.ReLU(inplace=True)
         self.downsample = downsample
         if isinstance(downsample, nn.Sequential) and len(downsample) == 2 and isinstance(downsample[0], TrunkConv) \
@@ -205,11 +250,12 @@ class Bottleneck(nn.Module):
 class ResNetTrunk(nn.Module):
     """conv1 .. layer4 of a torchvision-style ResNet; `features(x)` returns the last feature map."""
 
-    def __init__(self, block, layers, relu_inplace=True):
+    def __init__(self, block, layers, relu_inplace=True, norm='batch'):
         super().__init__()
         self.inplanes = 64
+        self.norm = norm
         self.conv1 = TrunkConv(3, 64, 7, 2, 3)
-        self.bn1 = BNAct(64)
+        self.bn1 = norm_layer(norm)(64)
         self.relu = nn.ReLU(inplace=relu_inplace)
         self.maxpool = MaxPool3s2()
         self.layer1 = self._make_layer(block, 64, layers[0])
@@ -229,10 +275,10 @@ class ResNetTrunk(nn.Module):
         if stride != 1 or self.inplanes != planes * block.expansion:
             downsample = nn.Sequential(
                 TrunkConv(self.inplanes, planes * block.expansion, 1, stride),
-                BNAct(planes * block.expansion))
-        layers = [block(self.inplanes, planes, stride, downsample)]
+                norm_layer(self.norm)(planes * block.expansion))
+        layers = [block(self.inplanes, planes, stride, downsample, norm=self.norm)]
         self.inplanes = planes * block.expansion
-        layers += [block(self.inplanes, planes) for _ in range(1, blocks)]
+        layers += [block(self.inplanes, planes, norm=self.norm) for _ in range(1, blocks)]
         return nn.Sequential(*layers)
 
     def features(self, x):
@@ -354,21 +400,23 @@ class ViTTrunk(nn.Module):
 _VITS = {'vit_b_16': dict(dim=768, depth=12, heads=12, mlp_dim=3072), 'vit_tiny_16': dict(dim=192, depth=2, heads=3, mlp_dim=384)}
 
 
-def resnet_trunk(name):
-    """Image trunk by name: torchvision-style ResNets (what the reference uses) or the build-defined ViTs."""
+def resnet_trunk(name, norm='batch'):
+    """Image trunk by name: torchvision-style ResNets (what the reference uses; norm 'batch' or 'group') or the build-defined ViTs."""
     if name in _VITS:
         return ViTTrunk(**_VITS[name])
     if name not in _RESNETS:
         raise ValueError(f'unknown cnn_type {name}')
     block, layers = _RESNETS[name]
-    return ResNetTrunk(block, layers)
+    return ResNetTrunk(block, layers, norm=norm)
 
 
 # ----------------------------------------------------------------------------------------- BERT
 class BertConfig:
     def __init__(self, vocab_size=30522, hidden_size=768, num_hidden_layers=12, num_attention_heads=12,
                  intermediate_size=3072, max_position_embeddings=512, type_vocab_size=2, layer_norm_eps=1e-12,
-                 hidden_dropout_prob=0.1):
+                 hidden_dropout_prob=0.1, position_embedding_type='absolute', relative_num_buckets=32, relative_max_distance=128):
+        if position_embedding_type not in ('absolute', 'relative_bucket'):
+            raise ValueError(f"position_embedding_type must be 'absolute' or 'relative_bucket', got {position_embedding_type!r}")
         self.__dict__.update(locals())
         del self.__dict__['self']
 
@@ -377,6 +425,10 @@ BERT_CONFIGS = {
     'bert-base-uncased': dict(),
     'bert-large-uncased': dict(hidden_size=1024, num_hidden_layers=24, num_attention_heads=16, intermediate_size=4096),
     'bert-mini': dict(hidden_size=256, num_hidden_layers=4, num_attention_heads=4, intermediate_size=1024),
+    # positions as a learned bias on the attention scores by the bucket of the distance, one table for all layers: texts of any length
+    'bert-base-relative': dict(position_embedding_type='relative_bucket'),
+    'bert-mini-relative': dict(hidden_size=256, num_hidden_layers=4, num_attention_heads=4, intermediate_size=1024,
+                               position_embedding_type='relative_bucket'),
 }
 
 
@@ -412,12 +464,18 @@ class _BertEmbeddings(nn.Module):
     def __init__(self, c):
         super().__init__()
         self.word_embeddings = nn.Embedding(c.vocab_size, c.hidden_size, padding_idx=0)
-        self.position_embeddings = nn.Embedding(c.max_position_embeddings, c.hidden_size)
+        self.relative = c.position_embedding_type == 'relative_bucket'      # positions enter the attention scores instead
+        if not self.relative:
+            self.position_embeddings = nn.Embedding(c.max_position_embeddings, c.hidden_size)
         self.token_type_embeddings = nn.Embedding(c.type_vocab_size, c.hidden_size)
         self.LayerNorm = nn.LayerNorm(c.hidden_size, eps=c.layer_norm_eps)
-        self.dropout = nn.Dropout(c.hidden_dropout_prob)
+        self.dropout = (CounterDropout if self.relative else nn.Dropout)(c.hidden_dropout_prob)
 
     def forward(self, input_ids, token_type_ids=None, pack=None):
+        if self.relative:
+            x = self.word_embeddings(input_ids if pack is None else input_ids.reshape(-1).index_select(0, pack.tok_idx))
+            tt = self.token_type_embeddings.weight[0] if token_type_ids is None else self.token_type_embeddings(token_type_ids)
+            return self.dropout(self.LayerNorm(x + tt))
         if pack is not None:            # packed tokens [T]: the real tokens of the batch only, each with its own position
             x = self.word_embeddings(input_ids.reshape(-1).index_select(0, pack.tok_idx)) + self.position_embeddings(pack.pos_ids)
             return self.dropout(self.LayerNorm(x + self.token_type_embeddings.weight[0]))
@@ -436,7 +494,9 @@ class _SelfAttention(nn.Module):
         self.key = nn.Linear(c.hidden_size, c.hidden_size)
         self.value = nn.Linear(c.hidden_size, c.hidden_size)
 
-    def forward(self, x, mask, cls_only=False, pack=None):
+    def forward(self, x, mask, cls_only=False, pack=None, rel=None):
+        if rel is not None:
+            return self._forward_relative(x, mask, cls_only, pack, rel)
         if pack is not None:
             return self._forward_packed(x, mask, cls_only, pack)
         B, L, H = x.shape
@@ -482,6 +542,45 @@ class _SelfAttention(nn.Module):
         return o.transpose(1, 2).reshape(B, H)
 
 
+    def _forward_relative(self, x, mask, cls_only, pack, rel):
+        """Scores with the learned bias of the distance's bucket; rel = (table [buckets, heads], bucket map).  bf16 on the GPU: csrc/relpos.hip
+        on the fused projection, padded, packed or for the [CLS] row alone; else the library's attention with the bias as its mask."""
+        from .. import ops
+        table, buckets = rel
+        H = x.shape[-1]
+        if _bert_fusable(x, self.query.weight) and ops.relpos_attention_supported(H // self.h):
+            if not cls_only:
+                w = torch.cat([self.query.weight, self.key.weight, self.value.weight], 0)
+                b = torch.cat([self.query.bias, self.key.bias, self.value.bias], 0)
+                qkv = F.linear(x, w, b)
+                if pack is not None:
+                    return ops.relpos_attention_varlen(qkv, pack.cu, pack.L, table, buckets, self.h)
+                return ops.relpos_attention(qkv, table, buckets, self.h, None if mask is None else mask.reshape(x.shape[:2]))
+            w, b = torch.cat([self.key.weight, self.value.weight], 0), torch.cat([self.key.bias, self.value.bias], 0)
+            kv = F.linear(x, w, b)
+            if pack is not None:
+                return ops.relpos_attention_cls(self.query(x.index_select(0, pack.cls_rows)), kv, table, buckets, self.h,
+                                                cu_seqlens=pack.cu, max_len=pack.L)
+            return ops.relpos_attention_cls(self.query(x[:, 0]), kv, table, buckets, self.h,
+                                            None if mask is None else mask.reshape(x.shape[:2]))[:, None]
+        if pack is not None:
+            raise RuntimeError('packed BERT run outside the bf16 path')
+        B, L, _ = x.shape
+        xq = x[:, :1] if cls_only else x
+
+        def split(t):
+            return t.view(B, t.shape[1], self.h, H // self.h).transpose(1, 2)
+        R = buckets.numel() // 2
+        d = torch.arange(L, device=x.device)[None, :] - torch.arange(xq.shape[1], device=x.device)[:, None]
+        bias = table[buckets.long()[d.clamp(-R, R) + R]].permute(2, 0, 1)[None]
+        q, k, v = split(self.query(xq)), split(self.key(x)), split(self.value(x))
+        bias = bias.to(q.dtype)
+        if mask is not None:
+            bias = bias.masked_fill(~mask, float('-inf'))
+        o = F.scaled_dot_product_attention(q, k, v, attn_mask=bias)
+        return o.transpose(1, 2).reshape(B, xq.shape[1], H)
+
+
 class _SelfOutput(nn.Module):
     def __init__(self, c, d_in):
         super().__init__()
@@ -507,10 +606,10 @@ class _Attention(nn.Module):
         self.self = _SelfAttention(c)
         self.output = _SelfOutput(c, c.hidden_size)
 
-    def forward(self, x, res, mask, cls_only=False, pack=None):
+    def forward(self, x, res, mask, cls_only=False, pack=None, rel=None):
         if pack is not None:
-            return self.output(self.self(x, mask, cls_only, pack), res.index_select(0, pack.cls_rows) if cls_only else res)
-        return self.output(self.self(x, mask, cls_only), res[:, :1] if cls_only else res)
+            return self.output(self.self(x, mask, cls_only, pack, rel), res.index_select(0, pack.cls_rows) if cls_only else res)
+        return self.output(self.self(x, mask, cls_only, None, rel), res[:, :1] if cls_only else res)
 
 
 class _Intermediate(nn.Module):
@@ -532,8 +631,8 @@ class _BertLayer(nn.Module):
         self.intermediate = _Intermediate(c)
         self.output = _SelfOutput(c, c.intermediate_size)
 
-    def forward(self, x, res, mask, cls_only=False, pack=None):
-        x, res = self.attention(x, res, mask, cls_only, pack)
+    def forward(self, x, res, mask, cls_only=False, pack=None, rel=None):
+        x, res = self.attention(x, res, mask, cls_only, pack, rel)
         return self.output(self.intermediate(x), res)
 
 
@@ -541,12 +640,17 @@ class _BertEncoder(nn.Module):
     def __init__(self, c):
         super().__init__()
         self.layer = nn.ModuleList([_BertLayer(c) for _ in range(c.num_hidden_layers)])
+        if c.position_embedding_type == 'relative_bucket':
+            from .. import ops
+            self.relative_attention_bias = nn.Embedding(c.relative_num_buckets, c.num_attention_heads)     # shared by the layers
+            self.register_buffer('relative_buckets', ops.relpos_buckets(c.relative_num_buckets, c.relative_max_distance), persistent=False)
 
     def forward(self, x, mask, cls_only=False, pack=None):
         last = len(self.layer) - 1
         res = x
+        rel = (self.relative_attention_bias.weight, self.relative_buckets) if hasattr(self, 'relative_attention_bias') else None
         for i, l in enumerate(self.layer):
-            x, res = l(x, res, mask, cls_only and i == last, pack)
+            x, res = l(x, res, mask, cls_only and i == last, pack, rel)
         return x
 
 
@@ -576,13 +680,19 @@ class BertModel(nn.Module):
     def from_pretrained(cls, name):
         return cls(name)
 
+    @property
+    def pack_longest(self):
+        """The longest sequence of a packed run: 32 tokens, any length with relative positions."""
+        return 1 << 30 if self.config.position_embedding_type == 'relative_bucket' else 32
+
     @staticmethod
-    def pack_plan(host_lengths, L, device):
+    def pack_plan(host_lengths, L, device, longest=32):
         """The index tensors of a PACKED run from the captions' lengths as HOST integers (no device synchronisation: the loaders
         know the lengths on the host, src/datasets/_dataloader.py:49-64 builds `cap_lengths` from python lists).  None when a
-        sequence does not fit the varlen attention kernel (> 32 tokens) or the lengths do not fit the padded frame."""
+        sequence does not fit the varlen attention kernel (`longest`: 32 tokens, or what `pack_longest` says of a model) or the lengths do
+        not fit the padded frame."""
         lens = [int(v) for v in host_lengths]
-        if not lens or min(lens) < 1 or max(lens) > min(L, 32):
+        if not lens or min(lens) < 1 or max(lens) > min(L, longest):
             return None
         B = len(lens)
         cu = [0]

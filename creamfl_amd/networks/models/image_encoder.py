@@ -18,7 +18,7 @@ class EncoderImage(nn.Module):
     def __init__(self, config, mlp_local):
         super().__init__()
         embed_dim = config.embed_dim
-        self.cnn = resnet_trunk(config.cnn_type)          # random init: no ImageNet weights offline
+        self.cnn = resnet_trunk(config.cnn_type, config.get('image_norm', 'batch'))          # random init: no ImageNet weights offline
         cnn_dim = self.cnn_dim = self.cnn.out_dim
         self.avgpool = nn.AdaptiveAvgPool2d((1, 1))       # kept for state_dict / API parity; fused in forward
         self.fc = nn.Linear(cnn_dim, embed_dim)

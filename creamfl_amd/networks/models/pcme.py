@@ -78,7 +78,7 @@ class PCME(nn.Module):
         c = getattr(self, '_pack_cache', None)
         if c is not None and (c[0] is host or c[0] == host) and c[1] == L and c[2] == device:
             return c[3]
-        plan = BertModel.pack_plan(host, L, device)
+        plan = BertModel.pack_plan(host, L, device, self.txt_enc.pack_longest)
         self._pack_cache = (host, L, device, plan)
         return plan
 

@@ -8,7 +8,7 @@ import math
 import torch.nn as nn
 
 from .. import ops
-from .backbones import BasicBlock, BNAct, Bottleneck, MaxPool3s2, TrunkConv, first_of, stem_tail
+from .backbones import BasicBlock, Bottleneck, MaxPool3s2, TrunkConv, first_of, norm_layer, stem_tail
 from .language_model import clamped_head, local_projection_head
 
 STAGE_WIDTHS = (64, 128, 256, 512)
@@ -22,9 +22,10 @@ class ResNet(nn.Module):
         self.scale = int(kwargs['scale'])
         self.phase = str(kwargs.get('phase', 'none'))
         self.mlp_local = kwargs.get('mlp_local', False)
+        self.norm = kwargs.get('norm', 'batch')                      # 'group': statistics per sample instead of per batch
         # stem
         self.conv1 = TrunkConv(3, 64, 7, stride=2, padding=3)        # (an nn.Conv2d: same parameter name, same state_dict)
-        self.bn1 = BNAct(64)                                         # (an nn.BatchNorm2d: same state_dict; ReLU fused where the fused kernels apply)
+        self.bn1 = norm_layer(self.norm)(64)                         # (an nn.BatchNorm2d: same state_dict; ReLU fused where the fused kernels apply)
         self.relu = nn.ReLU(inplace=False)
         self.maxpool = MaxPool3s2()
         # four stages; only the first keeps the resolution
@@ -55,8 +56,9 @@ class ResNet(nn.Module):
         shortcut = None
         if stride != 1 or self.inplanes != out_planes:
             shortcut = nn.Sequential(TrunkConv(self.inplanes, out_planes, 1, stride=stride),
-                                     BNAct(out_planes))
-        stage = [block(self.inplanes, planes, stride, shortcut)] + [block(out_planes, planes) for _ in range(blocks - 1)]
+                                     norm_layer(self.norm)(out_planes))
+        stage = [block(self.inplanes, planes, stride, shortcut, norm=self.norm)]
+        stage += [block(out_planes, planes, norm=self.norm) for _ in range(blocks - 1)]
         self.inplanes = out_planes
         return nn.Sequential(*stage)
 

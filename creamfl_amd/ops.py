@@ -2440,10 +2440,12 @@ class _RelposFn(torch.autograd.Function):
         lse = torch.empty(heads, q.shape[0], dtype=torch.float32, device=q.device) if need else None
         kb = q.data_ptr() + 2 * H if kv is None else kv.data_ptr()
         ldk = 3 * H if kv is None else 2 * H
+        n = lib.cfl_relpos_fwd_ws_bytes(B, Lq, Lk, T, heads)
+        ws = _ws(n, q.device) if n else None
         with _on_device(q):
             _lib.check(lib.cfl_relpos_fwd(_ptr(q), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,
                                           _ptr(table), int(table.dtype == torch.bfloat16), table.shape[0], _ptr(buckets),
-                                          buckets.numel() // 2, _ptr(o), H, _ptr(lse), _stream(q)), 'cfl_relpos_fwd')
+                                          buckets.numel() // 2, _ptr(o), H, _ptr(lse), _ptr(ws), _stream(q)), 'cfl_relpos_fwd')
         if need:
             ctx.save_for_backward(q, kv, table, buckets, mask, cu, o, lse)
             ctx.geo = geo
@@ -2461,7 +2463,7 @@ class _RelposFn(torch.autograd.Function):
         dkv = None if kv is None else torch.empty_like(kv)
         dtable = torch.empty_like(table)
         dsum = torch.empty_like(lse)
-        ws = _ws(lib.cfl_relpos_ws_bytes(B, Lq, Lk, T, heads, R), q.device)
+        ws = _ws(lib.cfl_relpos_bwd_ws_bytes(B, Lq, Lk, T, heads, table.shape[0]), q.device)
         kb = q.data_ptr() + 2 * H if kv is None else kv.data_ptr()
         gb = dq.data_ptr() + 2 * H if kv is None else dkv.data_ptr()
         ldk = 3 * H if kv is None else 2 * H

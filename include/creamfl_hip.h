@@ -194,7 +194,7 @@ int cfl_set_dropout_tick(const unsigned* tick_dev);
  * y[e] = keep(e) ? x[e] / (1 - p') : 0 for n elements; keep(e) = the 16 random bits of (seed, e) are >= rint(65536 p), p' = that / 65536:
  * the flags of cfl_dropout_mask; 0 <= p <= 1 (1: zeros).  dtype: 0 fp32, 1 bf16, 2 fp16.  The seed is *seed_dev where seed_dev is given,
  * else `seed` (with the tick of cfl_set_dropout_tick, if one is registered); what was used is written to *seed_used (NULL = skip).
- * The backward is the same call on the gradient with seed_dev = the forward's seed_used.  y may be x. */
+ * The backward is the same call on the gradient with seed_dev = the forward's seed_used. */
 int cfl_dropout(const void* x, int dtype, long long n, double p, unsigned seed, const unsigned* seed_dev, void* y,
                 unsigned* seed_used, void* stream);
 
@@ -222,11 +222,13 @@ int cfl_gn_bwd(const void* dy, const void* dy2, const void* x, const void* res, 
  * query rows b Lq ..; Lk is the longest text (a hint for the launch: longer ones are handled).  Rows behind cu[B] get zeros.
  * Query i of a text stands at position i.  A row without a key has o = 0 and no gradient.
  * lse (fp32 [heads][query rows]) is written by fwd (NULL = skip) and read by bwd; dsum: scratch of the same size; dtable as table.
- * All ld % 8 == 0, 16-byte aligned bases.  ws: cfl_relpos_ws_bytes (T = 0: padded). */
-size_t cfl_relpos_ws_bytes(int B, int Lq, int Lk, int T, int heads, int R);
+ * All ld % 8 == 0, 16-byte aligned bases.
+ * ws: cfl_relpos_fwd_ws_bytes (0: may be NULL) / cfl_relpos_bwd_ws_bytes (T = 0: padded). */
+size_t cfl_relpos_fwd_ws_bytes(int B, int Lq, int Lk, int T, int heads);
+size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb);
 int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
                    int B, int Lq, int Lk, int T, int heads, int head_dim, float scale, const void* table, int table_bf16, int nb,
-                   const int* bucket, int R, void* o, long long ldo, float* lse, void* stream);
+                   const int* bucket, int R, void* o, long long ldo, float* lse, void* ws, void* stream);
 int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
                    int B, int Lq, int Lk, int T, int heads, int head_dim, float scale, const void* table, int table_bf16, int nb,
                    const int* bucket, int R, const void* o, const void* dout, long long ldo, const float* lse, float* dsum, void* dq,

@@ -220,7 +220,7 @@ def check_padded(dev, t, mask, scale=None, heads=None):
 
 
 @pytest.mark.parametrize('B,L,heads', [(1, 1, 1), (3, 2, 2), (2, 17, 3), (2, 31, 4), (3, 32, 12), (2, 33, 2), (2, 63, 1), (2, 64, 2), (1, 65, 3), (2, 96, 2),
-                                       (1, 127, 1), (2, 128, 2), (2, 129, 2), (2, 197, 3), (1, 300, 2), (1, 513, 1), (9, 24, 12), (1, 1025, 1)])
+                                       (1, 127, 1), (2, 128, 2), (2, 129, 2), (2, 197, 3), (1, 300, 2), (1, 513, 1), (9, 24, 12), (1, 1025, 1), (40, 160, 8)])
 def test_relpos_attention_matches_oracle(dev, B, L, heads):
     check_padded(dev, attn_inputs(B * 1000 + L, B, L, heads), None)
 
@@ -266,7 +266,8 @@ def test_relpos_attention_scale_and_maps(dev):
 
 
 @pytest.mark.parametrize('lens,max_len,tail', [([1], 1, 0), ([5, 0, 32, 1, 17], 32, 0), ([5, 0, 32, 1, 17], 32, 3), ([40, 0, 7, 129, 64], 129, 0),
-                                               ([0, 70, 0], 70, 9), ([300, 20], 20, 0), ([33, 90, 128], 17, 1)])
+                                               ([0, 70, 0], 70, 9), ([300, 20], 20, 0), ([33, 90, 128], 17, 1),
+                                               ([700, 0, 1300], 1300, 5)])
 def test_relpos_attention_varlen(dev, lens, max_len, tail):
     """Packed texts, empty ones among them, rows behind the last one, texts longer than the hint."""
     from creamfl_amd import ops
@@ -296,7 +297,7 @@ def test_relpos_attention_varlen(dev, lens, max_len, tail):
 
 
 @pytest.mark.parametrize('lens,packed', [([1], False), ([24, 7, 0, 31], False), ([24, 7, 0, 31], True), ([200, 0, 65, 129], False), ([200, 0, 65, 129], True),
-                                         ([1000], False), ([3, 1], True)])
+                                         ([1000], False), ([3, 1], True), ([2100, 0, 5], True), ([600, 0, 37, 1500], False)])
 def test_relpos_attention_cls(dev, lens, packed):
     from creamfl_amd import ops
     heads, H, B, L = 3, 192, len(lens), max(max(lens), 1)

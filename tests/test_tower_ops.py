@@ -118,7 +118,7 @@ def test_entries_refuse_bad_arguments():
     assert lib.cfl_gn_ws_bytes(2, 9, 16, 3) == 0 and lib.cfl_gn_ws_bytes(2, 9, 16, 4) > 0
 
     def fwd(q=P, ldq=192, mask=None, cu=None, b=2, lq=4, lk=4, t=0, heads=1, hd=64, table=P, nb=4, bucket=P, r=2, o=P, ldo=64):
-        return lib.cfl_relpos_fwd(q, ldq, P, P, 192, mask, cu, b, lq, lk, t, heads, hd, 0.125, table, 1, nb, bucket, r, o, ldo, None, None)
+        return lib.cfl_relpos_fwd(q, ldq, P, P, 192, mask, cu, b, lq, lk, t, heads, hd, 0.125, table, 1, nb, bucket, r, o, ldo, None, None, None)
     for kw in (dict(q=None), dict(b=0), dict(lq=0), dict(lk=0), dict(heads=0), dict(table=None), dict(nb=0), dict(bucket=None), dict(r=-1),
                dict(o=None), dict(cu=P, t=0), dict(cu=P, t=8, mask=P)):
         assert fwd(**kw) == EINVAL, kw
@@ -126,4 +126,61 @@ def test_entries_refuse_bad_arguments():
     assert fwd(hd=32) == ELIMIT and fwd(r=513) == ELIMIT and fwd(b=1 << 30, heads=64) == ELIMIT
     assert lib.cfl_relpos_bwd(P, 192, P, P, 192, None, None, 2, 4, 4, 0, 1, 64, 0.125, P, 1, 4, P, 2, P, P, 64, P, None, P, 192, P, P, 192, P, P,
                               None) == EINVAL
-    assert lib.cfl_relpos_ws_bytes(2, 4, 4, 0, 1, 513) == 0 and lib.cfl_relpos_ws_bytes(2, 0, 4, 0, 1, 2) == 0
+    assert lib.cfl_relpos_bwd_ws_bytes(0, 4, 4, 0, 1, 4) == 0 and lib.cfl_relpos_bwd_ws_bytes(2, 0, 4, 8, 1, 4) > 0
+    assert lib.cfl_relpos_fwd_ws_bytes(1, 1, 4096, 0, 1) > 0 and lib.cfl_relpos_fwd_ws_bytes(64, 64, 64, 0, 12) == 0
+    assert fwd(b=1, lq=1, lk=4096) == EINVAL               # (a split forward without its workspace)
+
+
+# ------------------------------------------------------------------------------------------------ the towers that call them
+def test_group_normed_trunk_on_the_library_path():
+    from creamfl_amd.networks import backbones
+    from creamfl_amd.networks.resnet_client import resnet18_client
+    torch.manual_seed(0)
+    m = backbones.resnet_trunk('resnet18', 'group')
+    assert not any(isinstance(x, torch.nn.BatchNorm2d) for x in m.modules())
+    y = m(torch.randn(2, 3, 64, 64))
+    assert y.shape == (2, 512, 2, 2) and torch.isfinite(y).all()
+    one = m(torch.randn(1, 3, 64, 64))
+    assert one.shape == (1, 512, 2, 2)                     # (statistics per sample: a batch of one is a batch)
+    y.sum().backward()
+    assert all(p.grad is not None for p in m.parameters())
+    assert backbones.resnet_trunk('resnet50', 'group').layer1[0].conv3.bn_follows is False
+    assert backbones.resnet_trunk('resnet50').layer1[0].conv3.bn_follows is True
+    c = resnet18_client(num_class=10, is_train=True, scale=128, embed_dim=512, norm='group')
+    assert not any(isinstance(x, torch.nn.BatchNorm2d) for x in c.modules())
+    with pytest.raises(ValueError):
+        backbones.resnet_trunk('resnet18', 'layer')
+
+
+def test_relative_bert_on_the_library_path():
+    from creamfl_amd.networks.backbones import BertConfig, BertModel
+    torch.manual_seed(1)
+    m = BertModel('bert-mini-relative').eval()
+    assert not any('position_embeddings' in n for n, _ in m.named_parameters())
+    ids = torch.randint(1, 1000, (3, 40))
+    mask = torch.arange(40)[None] < torch.tensor([40, 9, 23])[:, None]
+    out = m(ids, attention_mask=mask)['last_hidden_state']
+    cls = m(ids, attention_mask=mask, cls_only=True)['last_hidden_state']
+    np.testing.assert_allclose(cls[:, 0].detach().numpy(), out[:, 0].detach().numpy(), rtol=1e-4, atol=1e-5)
+    shorter = m(ids[1:2, :9])['last_hidden_state']         # padding changes nothing for the real tokens
+    np.testing.assert_allclose(shorter[0].detach().numpy(), out[1, :9].detach().numpy(), rtol=1e-4, atol=1e-5)
+    out.square().sum().backward()
+    assert float(m.encoder.relative_attention_bias.weight.grad.abs().max()) > 0
+    assert m(torch.randint(1, 1000, (1, 700)))['last_hidden_state'].shape == (1, 700, 256)         # longer than any position table
+    assert BertModel('bert-mini').pack_longest == 32 and m.pack_longest > 700
+    with pytest.raises(ValueError):
+        BertConfig(position_embedding_type='rotary')
+
+
+def test_flags_reach_the_models():
+    import argparse
+    from creamfl_amd import flags
+    from creamfl_amd.networks.models import get_model
+    from creamfl_amd.utils.config import default_config
+    ns = flags.add_build_flags(argparse.ArgumentParser()).parse_args(['--image_norm', 'group', '--bert_name', 'bert-mini-relative'])
+    assert flags.get(ns, 'image_norm') == 'group' and flags.get(argparse.Namespace(), 'image_norm') == 'batch'
+    cfg = default_config(embed_dim=64, cnn_type='resnet18')
+    cfg.model.image_norm, cfg.model.bert_name = ns.image_norm, ns.bert_name
+    m = get_model({'<pad>': 0}, cfg.model, False)
+    assert not any(isinstance(x, torch.nn.BatchNorm2d) for x in m.img_enc.modules())
+    assert m.txt_enc.config.position_embedding_type == 'relative_bucket'
