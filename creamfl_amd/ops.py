@@ -1222,10 +1222,17 @@ def bn_act_eval(x, weight, bias, running_mean, running_var, eps, relu=False, res
 _GN_ACTS = {'none': 0, None: 0, 'relu': 1, 'silu': 2}
 
 
-def _on_device(t):
-    """Context in which a launch for `t` may be issued: its device is the current one (launches go to the current device)."""
+def _launch(name, t, *args):
+    """Entry `name` of the library with `args` and t's current stream, t's device being the current one (launches go to the current device)."""
+    fn = getattr(_lib.load(), name)
     idx = t.device.index
-    return contextlib.nullcontext() if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(idx)
+    if idx is None or idx == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(t.device))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, _raw_stream(t.device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _aligned16(t):
@@ -1242,32 +1249,31 @@ def gn_act_supported(x, num_channels, groups):
 
 class _GNActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, weight, bias, groups, eps, act, need):
-        lib = _lib.load()
+    def forward(ctx, x, residual, weight, bias, groups, eps, act, need, two):
         N, C, H, W = x.shape
         y = torch.empty_like(x)                           # keeps channels_last
-        stats = torch.empty(2, N, groups, dtype=torch.float32, device=x.device) if need else None
-        ws = _ws(lib.cfl_gn_ws_bytes(N, H * W, C, groups), x.device)
-        with _on_device(x):
-            _lib.check(lib.cfl_gn_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), int(x.dtype == torch.bfloat16), N, H * W, C, groups,
-                                      eps, act, _ptr(y), _ptr(stats), _ptr(stats[1]) if need else None, _ptr(ws), _stream(x)), 'cfl_gn_fwd')
+        n = _lib.load().cfl_gn_ws_bytes(N, H * W, C, groups)
+        # one buffer: the statistics [2][N][groups] that the backward reads, then the launch's scratch
+        buf = torch.empty(n + 8 * N * groups, dtype=torch.uint8, device=x.device)
+        at = buf.data_ptr()
+        _launch('cfl_gn_fwd', x, x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(), int(x.dtype == torch.bfloat16), N, H * W, C,
+                groups, eps, act, y.data_ptr(), at if need else None, at + 4 * N * groups if need else None, at + 8 * N * groups)
         if need:
             # (without an activation dz = dy: the residual is not read again)
-            ctx.save_for_backward(x, residual if act else None, weight, bias, stats)
+            ctx.save_for_backward(x, residual if act else None, weight, bias, buf[:8 * N * groups].clone() if n > 8 * N * groups + 65536 else buf)
             ctx.hyper = (groups, act, residual is not None)
         ctx.set_materialize_grads(False)                  # an unused alias must arrive as None, not as a zero tensor
-        return y, _alias(y)
+        return (y, _alias(y)) if two else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dy2):
-        lib = _lib.load()
+    def backward(ctx, dy, dy2=None):
         x, residual, weight, bias, stats = ctx.saved_tensors
         groups, act, has_res = ctx.hyper
         if dy is None:
             dy, dy2 = dy2, None
         if dy is None:
-            return (None,) * 8
+            return (None,) * 9
         N, C, H, W = x.shape
         from . import streams
         streams.flush(x.device)                           # a long HBM-bound phase: let the queued weight gradients run beside it
@@ -1281,13 +1287,13 @@ class _GNActFn(torch.autograd.Function):
         # without an activation the residual's gradient is dy itself, unless two gradients have to be added
         own = want and (act != 0 or dy2 is not None)
         dres = torch.empty_like(x) if own else dy if want else None
-        dgb = torch.empty(2, C, dtype=torch.float32, device=x.device)
-        ws = _ws(lib.cfl_gn_ws_bytes(N, H * W, C, groups), x.device)
-        with _on_device(x):
-            _lib.check(lib.cfl_gn_bwd(_ptr(dy), _ptr(dy2), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(stats), _ptr(stats[1]),
-                                      int(x.dtype == torch.bfloat16), N, H * W, C, groups, act, int(own), _ptr(dx),
-                                      _ptr(dres) if own else None, _ptr(dgb), _ptr(dgb[1]), _ptr(ws), _stream(x)), 'cfl_gn_bwd')
-        return dx, dres, dgb[0], dgb[1], None, None, None, None
+        dgamma, dbeta = torch.empty_like(weight), torch.empty_like(bias)
+        ws = _ws(_lib.load().cfl_gn_ws_bytes(N, H * W, C, groups), x.device)
+        at = stats.data_ptr()
+        _launch('cfl_gn_bwd', x, dy.data_ptr(), _ptr(dy2), x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(), at,
+                at + 4 * N * groups, int(x.dtype == torch.bfloat16), N, H * W, C, groups, act, int(own), dx.data_ptr(),
+                dres.data_ptr() if own else None, dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr())
+        return dx, dres, dgamma, dbeta, None, None, None, None, None
 
 
 def gn_act(x, weight, bias, groups, eps=1e-5, act='none', residual=None, two=False):
@@ -1314,8 +1320,7 @@ def gn_act(x, weight, bias, groups, eps=1e-5, act='none', residual=None, two=Fal
         residual = _aligned16(residual.to(x.dtype).contiguous(memory_format=torch.channels_last))
     weight, bias = _f32(weight, 'weight'), _f32(bias, 'bias')
     need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias))
-    y, y2 = _GNActFn.apply(_aligned16(x), residual, weight, bias, groups, float(eps), _GN_ACTS[act], need)
-    return (y, y2) if two else y
+    return _GNActFn.apply(_aligned16(x), residual, weight, bias, groups, float(eps), _GN_ACTS[act], need, bool(two))
 
 
 # --------------------------------------------------------------------------- 1x1 convolution: data gradient (csrc/gemm_bf16.hip)
@@ -2361,9 +2366,7 @@ class _DropoutFn(torch.autograd.Function):
     def forward(ctx, x, p, seed, need):
         y = torch.empty_like(x)
         used = torch.empty(1, dtype=torch.int32, device=x.device) if need else None
-        with _on_device(x):
-            _lib.check(_lib.load().cfl_dropout(_ptr(x), _DROP_DTYPES[x.dtype], x.numel(), p, seed, None, _ptr(y), _ptr(used), _stream(x)),
-                       'cfl_dropout')
+        _launch('cfl_dropout', x, x.data_ptr(), _DROP_DTYPES[x.dtype], x.numel(), p, seed, None, y.data_ptr(), _ptr(used))
         if need:
             ctx.save_for_backward(used)                   # (the seed as the device used it: the tick may move on before the backward)
             ctx.p = p
@@ -2375,9 +2378,7 @@ class _DropoutFn(torch.autograd.Function):
         used, = ctx.saved_tensors
         dy = dy.contiguous()
         dx = torch.empty_like(dy)
-        with _on_device(dy):
-            _lib.check(_lib.load().cfl_dropout(_ptr(dy), _DROP_DTYPES[dy.dtype], dy.numel(), ctx.p, 0, _ptr(used), _ptr(dx), None, _stream(dy)),
-                       'cfl_dropout')
+        _launch('cfl_dropout', dy, dy.data_ptr(), _DROP_DTYPES[dy.dtype], dy.numel(), ctx.p, 0, used.data_ptr(), dx.data_ptr(), None)
         return dx, None, None, None
 
 
@@ -2433,19 +2434,16 @@ class _RelposFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, kv, table, buckets, mask, cu, geo, need):
-        lib = _lib.load()
         B, Lq, Lk, T, heads, scale = geo
-        H = heads * 64
-        o = torch.empty(q.shape[0], H, dtype=torch.bfloat16, device=q.device)
-        lse = torch.empty(heads, q.shape[0], dtype=torch.float32, device=q.device) if need else None
-        kb = q.data_ptr() + 2 * H if kv is None else kv.data_ptr()
-        ldk = 3 * H if kv is None else 2 * H
-        n = lib.cfl_relpos_fwd_ws_bytes(B, Lq, Lk, T, heads)
+        H, rows = heads * 64, q.shape[0]
+        o = torch.empty(rows, H, dtype=torch.bfloat16, device=q.device)
+        lse = torch.empty(2, heads, rows, dtype=torch.float32, device=q.device) if need else None      # [1]: the backward's row sums
+        n = _lib.load().cfl_relpos_fwd_ws_bytes(B, Lq, Lk, T, heads)
         ws = _ws(n, q.device) if n else None
-        with _on_device(q):
-            _lib.check(lib.cfl_relpos_fwd(_ptr(q), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,
-                                          _ptr(table), int(table.dtype == torch.bfloat16), table.shape[0], _ptr(buckets),
-                                          buckets.numel() // 2, _ptr(o), H, _ptr(lse), _ptr(ws), _stream(q)), 'cfl_relpos_fwd')
+        kb, ldk = (q.data_ptr() + 2 * H, 3 * H) if kv is None else (kv.data_ptr(), 2 * H)
+        _launch('cfl_relpos_fwd', q, q.data_ptr(), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,
+                table.data_ptr(), int(table.dtype == torch.bfloat16), table.shape[0], buckets.data_ptr(), buckets.numel() // 2, o.data_ptr(), H,
+                _ptr(lse), _ptr(ws))
         if need:
             ctx.save_for_backward(q, kv, table, buckets, mask, cu, o, lse)
             ctx.geo = geo
@@ -2454,24 +2452,20 @@ class _RelposFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        lib = _lib.load()
         q, kv, table, buckets, mask, cu, o, lse = ctx.saved_tensors
         B, Lq, Lk, T, heads, scale = ctx.geo
-        H, R = heads * 64, buckets.numel() // 2
+        H, nb = heads * 64, table.shape[0]
         do = _aligned16(_bf16c(do, 'do'))
         dq = torch.empty_like(q)
         dkv = None if kv is None else torch.empty_like(kv)
         dtable = torch.empty_like(table)
-        dsum = torch.empty_like(lse)
-        ws = _ws(lib.cfl_relpos_bwd_ws_bytes(B, Lq, Lk, T, heads, table.shape[0]), q.device)
-        kb = q.data_ptr() + 2 * H if kv is None else kv.data_ptr()
+        ws = _ws(_lib.load().cfl_relpos_bwd_ws_bytes(B, Lq, Lk, T, heads, nb), q.device)
+        kb, ldk = (q.data_ptr() + 2 * H, 3 * H) if kv is None else (kv.data_ptr(), 2 * H)
         gb = dq.data_ptr() + 2 * H if kv is None else dkv.data_ptr()
-        ldk = 3 * H if kv is None else 2 * H
-        with _on_device(q):
-            _lib.check(lib.cfl_relpos_bwd(_ptr(q), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,
-                                          _ptr(table), int(table.dtype == torch.bfloat16), table.shape[0], _ptr(buckets), R, _ptr(o),
-                                          _ptr(do), H, _ptr(lse), _ptr(dsum), _ptr(dq), q.shape[1], gb, gb + 2 * H, ldk, _ptr(dtable),
-                                          _ptr(ws), _stream(q)), 'cfl_relpos_bwd')
+        _launch('cfl_relpos_bwd', q, q.data_ptr(), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,
+                table.data_ptr(), int(table.dtype == torch.bfloat16), nb, buckets.data_ptr(), buckets.numel() // 2, o.data_ptr(), do.data_ptr(), H,
+                lse.data_ptr(), lse.data_ptr() + lse.numel() * 2, dq.data_ptr(), q.shape[1], gb, gb + 2 * H, ldk, dtable.data_ptr(),
+                ws.data_ptr())
         return dq, dkv, dtable, None, None, None, None, None
 
 
