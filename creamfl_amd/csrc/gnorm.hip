@@ -34,15 +34,40 @@ __device__ __forceinline__ GMap gn_map(int C) {
     return m;
 }
 
-template <int ACT> __device__ __forceinline__ float gn_act(float z) {
-    if (ACT == GN_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-    if (ACT == GN_SILU) return z / (1.f + __expf(-z));
+// 1 / (1 + e^-z) on the hardware's exp2 and reciprocal (one unit in the last place each; an IEEE division would cost more than all the rest
+// of the pass: the forward has 28 vector operations per element at the memory's pace, and a division takes ten)
+__device__ __forceinline__ float gn_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+}
+__device__ __forceinline__ float gn_act(int act, float z) {
+    if (act == GN_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+    if (act == GN_SILU) return z * gn_sigmoid(z);
     return z;
 }
-template <int ACT> __device__ __forceinline__ float gn_act_grad(float z) {
-    if (ACT == GN_RELU) return z > 0.f ? 1.f : 0.f;
-    if (ACT == GN_SILU) { const float s = 1.f / (1.f + __expf(-z)); return s * (1.f + z * (1.f - s)); }
+__device__ __forceinline__ float gn_act_grad(int act, float z) {
+    if (act == GN_RELU) return z > 0.f ? 1.f : 0.f;
+    if (act == GN_SILU) { const float s = gn_sigmoid(z); return s * fmaf(z, 1.f - s, 1.f); }
     return 1.f;
+}
+// 8 channels rounded once (hardware conversion, two values an instruction)
+__device__ __forceinline__ void gn_store(U4* p, const float (&f)[8]) {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    v8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (__bf16)f[j];
+    *reinterpret_cast<v8*>(p) = o;
+}
+__device__ __forceinline__ void gn_store(F8* p, const float (&f)[8]) { *p = pack8g<F8>(f); }
+// group (from the slice's first) of each of a thread's 8 channels cl .. cl + 7
+__device__ __forceinline__ void gn_groups(int cl, int cpg, int (&g)[8]) {
+    g[0] = cl / cpg;
+    int r = cl - g[0] * cpg;
+#pragma unroll
+    for (int j = 1; j < 8; ++j) {
+        const bool next = ++r == cpg;
+        g[j] = g[j - 1] + (next ? 1 : 0);
+        r = next ? 0 : r;
+    }
 }
 
 // ---- forward, pass 1: (mean, M2) of every group over a chunk of rows.  grid = (chunks, N); part: [N][chunks][G][2]
@@ -131,9 +156,11 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_apply_kernel(const E* __restrict_
     if (blockIdx.x == 0 && mean) for (int g = threadIdx.x; g < G; g += GN_T) { mean[(long long)n * G + g] = mu[g]; rstd[(long long)n * G + g] = rs[g]; }
     if (!m.active) return;
     float sc[8], sh[8], mv[8];
+    int gi[8];
+    gn_groups(m.c0, cpg, gi);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int g = (m.c0 + j) / cpg;
+        const int g = gi[j];
         sc[j] = rs[g] * gamma[m.c0 + j]; sh[j] = beta[m.c0 + j]; mv[j] = mu[g];
     }
     const int r0 = blockIdx.x * rows, r1 = min(HW, r0 + rows), C8 = C >> 3;
@@ -146,9 +173,9 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_apply_kernel(const E* __restrict_
         for (int j = 0; j < 8; ++j) {
             float z = fmaf(f[j] - mv[j], sc[j], sh[j]);
             if (RES) z += h[j];
-            f[j] = gn_act<ACT>(z);
+            f[j] = gn_act(ACT, z);
         }
-        y[at] = pack8g<E>(f);
+        gn_store(y + at, f);
     }
 }
 
@@ -175,7 +202,7 @@ __device__ __forceinline__ void gn_dz(const E& xv, const E& rv, const float (&mv
         if (ACT != GN_NONE) {
             float z = fmaf(xh[j], ga[j], be[j]);
             if (RES) z += h[j];
-            dz[j] *= gn_act_grad<ACT>(z);
+            dz[j] *= gn_act_grad(ACT, z);
         }
     }
 }
@@ -194,9 +221,11 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_bwd_reduce_kernel(const E* __rest
     const int r0 = blockIdx.x * rows, r1 = min(HW, r0 + rows);
     if (m.active) {
         float mv[8], rv[8], ga[8], be[8], a[8], b[8];
+        int gi[8];
+        gn_groups(m.c0, cpg, gi);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int g = (m.c0 + j) / cpg;
+            const int g = gi[j];
             mv[j] = mean[(long long)n * G + g]; rv[j] = rstd[(long long)n * G + g];
             ga[j] = gamma[m.c0 + j]; be[j] = beta[m.c0 + j];
             a[j] = 0.f; b[j] = 0.f;
@@ -252,9 +281,11 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_bwd_apply_kernel(const E* __restr
     __syncthreads();
     if (!m.active) return;
     float mv[8], rv[8], ga[8], be[8], c1[8], c2[8];
+    int gi[8];
+    gn_groups(m.c0, cpg, gi);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int g = (m.c0 + j) / cpg;
+        const int g = gi[j];
         mv[j] = mean[(long long)n * G + g]; rv[j] = rstd[(long long)n * G + g];
         ga[j] = gamma[m.c0 + j]; be[j] = beta[m.c0 + j];
         c1[j] = s1[g]; c2[j] = s2[g];
@@ -267,10 +298,10 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_bwd_apply_kernel(const E* __restr
         if (RES && ACT != GN_NONE) rr = res[at];
         gn_dy(dy, dy2, at, dz);
         gn_dz<E, ACT, RES>(x[at], rr, mv, rv, ga, be, xh, dz);
-        if (dres) dres[at] = pack8g<E>(dz);
+        if (dres) gn_store(dres + at, dz);
 #pragma unroll
         for (int j = 0; j < 8; ++j) dz[j] = rv[j] * (fmaf(dz[j], ga[j], -c1[j]) - xh[j] * c2[j]);
-        dx[at] = pack8g<E>(dz);
+        gn_store(dx + at, dz);
     }
 }
 
@@ -287,29 +318,31 @@ __global__ __launch_bounds__(1024) void cfl_gn_bwd_final_kernel(const float* __r
 // ---- one pass: a workgroup holds all H W rows of a slice of S channels (whole groups) of one sample in registers, so the activation is
 // read once.  Record: 8 channels of one row; a thread holds up to V of them, rows rsub, rsub + rpp, ...  NG = 1: a thread's 8 channels
 // lie in one group; NG = 8: each is treated by itself.
-struct ResPlan { int S, T; };                                  // channels of a slice (0: does not fit), threads
 constexpr int RES_V16 = 14, RES_V32 = 8;                       // records a thread holds in the forward: bf16 / fp32
 constexpr int RES_B16 = 13, RES_B32 = 9;                       // ... in the backward: x and the 32-bit gradient
-constexpr int RES_TF = 1024, RES_TB = 512;                     // most threads: 128 registers each / 256
+constexpr int RES_F16 = 4, RES_F32 = 3;                        // ... in the variants for few records
+constexpr int STR_T = 1024;                                    // threads of the two-pass kernels
+constexpr int RES_T = 512;                                     // most threads of the one-pass kernels
 
 // (count, mean, M2) of the workgroup's groups from per-thread pairs in LDS: lds[rsub * slots + slot] = (mean, M2) over cnt(rsub) rows of the
 // slot's `w` channels.  Two levels, both exact merges; results in mu[], rs[] (GS groups, `spg` slots each).
-__device__ __forceinline__ void gn_block_stats(float2* lds, int T, int slots, int spg, int GS, int rpp, int HW, float w, float eps, float* mu,
-                                               float* rs) {
+__device__ __forceinline__ void gn_block_stats(float2* lds, float* cn, int T, int slots, int spg, int GS, int rpp, int HW, float w, float eps,
+                                               float* mu, float* rs) {
     const int t = threadIdx.x;
-    // level 1: part `part` of P merges rows part, part + P, ... of its slot; its pair takes the place of row `part`
-    const int P = min(min(T / slots, 16), rpp), slot = t % slots, part = t / slots;
+    // level 1: part `part` of P merges rows part, part + P, ... of its slot; its pair takes the place of row `part`, its count cn[part]
+    const int q = T / slots, P = min(min(q, 16), rpp), part = t / slots, slot = t - part * slots, rows = min(rpp, HW);
+    const int full = HW / rpp, more = HW - full * rpp;         // a row phase r has full + (r < more) rows
     float n1 = 0.f, mean = 0.f, m2 = 0.f;
     if (part < P) {
         float sum = 0.f;
-        for (int r = part; r < rpp && r < HW; r += P) {
-            const float c = (float)((HW - r + rpp - 1) / rpp) * w;
+        for (int r = part; r < rows; r += P) {
+            const float c = (float)(full + (r < more)) * w;
             sum = fmaf(c, lds[r * slots + slot].x, sum);
             n1 += c;
         }
         mean = n1 > 0.f ? sum / n1 : 0.f;
-        for (int r = part; r < rpp && r < HW; r += P) {
-            const float c = (float)((HW - r + rpp - 1) / rpp) * w;
+        for (int r = part; r < rows; r += P) {
+            const float c = (float)(full + (r < more)) * w;
             const float2 v = lds[r * slots + slot];
             const float d = v.x - mean;
             m2 += fmaf(c * d, d, v.y);
@@ -318,41 +351,33 @@ __device__ __forceinline__ void gn_block_stats(float2* lds, int T, int slots, in
     __syncthreads();
     if (part < P) {
         lds[part * slots + slot] = make_float2(mean, m2);
-        if (slot == 0) rs[part] = n1;                          // (counts: the same for every slot; rs is free until the end)
+        if (slot == 0) cn[part] = n1;
     }
     __syncthreads();
     // level 2: L lanes of one wave per group
     int L = 1;
-    while (L < 64 && 2 * L * GS <= T) L *= 2;
-    float cnt[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) cnt[k] = k < P ? rs[k] : 0.f;
-    __syncthreads();
+    while (L < 64 && 2 * L * GS <= T && L < P * spg) L *= 2;
     for (int g0 = 0; g0 < GS; g0 += T / L) {
-        const int g = g0 + t / L, l = t % L;
+        const int g = g0 + t / L, l = t & (L - 1);
         const bool on = g < GS;
-        const int E = on ? P * spg : 0;
         float n = 0.f, sum = 0.f;
-        for (int e = l; e < E; e += L) {
-            const int k = e / spg;
-            float c = 0.f;
-#pragma unroll
-            for (int q = 0; q < 16; ++q) c = q == k ? cnt[q] : c;
-            n += c;
-            sum = fmaf(c, lds[k * slots + g * spg + e % spg].x, sum);
-        }
+        if (on)
+            for (int k = l / spg, s = l - k * spg; k < P; ) {
+                const float c = cn[k];
+                n += c;
+                sum = fmaf(c, lds[k * slots + g * spg + s].x, sum);
+                for (s += L; s >= spg && k < P; s -= spg) ++k;
+            }
         for (int o = L >> 1; o > 0; o >>= 1) { n += __shfl_xor(n, o, 64); sum += __shfl_xor(sum, o, 64); }
         const float gm = n > 0.f ? sum / n : 0.f;
         float q2 = 0.f;
-        for (int e = l; e < E; e += L) {
-            const int k = e / spg;
-            float c = 0.f;
-#pragma unroll
-            for (int q = 0; q < 16; ++q) c = q == k ? cnt[q] : c;
-            const float2 v = lds[k * slots + g * spg + e % spg];
-            const float d = v.x - gm;
-            q2 += fmaf(c * d, d, v.y);
-        }
+        if (on)
+            for (int k = l / spg, s = l - k * spg; k < P; ) {
+                const float2 v = lds[k * slots + g * spg + s];
+                const float d = v.x - gm;
+                q2 += fmaf(cn[k] * d, d, v.y);
+                for (s += L; s >= spg && k < P; s -= spg) ++k;
+            }
         for (int o = L >> 1; o > 0; o >>= 1) q2 += __shfl_xor(q2, o, 64);
         if (on && l == 0) { mu[g] = gm; rs[g] = 1.f / sqrtf(q2 / n + eps); }
     }
@@ -360,17 +385,18 @@ __device__ __forceinline__ void gn_block_stats(float2* lds, int T, int slots, in
 }
 
 template <class E, int NG, int V>
-__global__ __launch_bounds__(RES_TF) void cfl_gn_res_fwd_kernel(const E* __restrict__ x, const E* __restrict__ res, const float* __restrict__ gamma,
+__global__ __launch_bounds__(V <= 4 ? 256 : RES_T) void cfl_gn_res_fwd_kernel(const E* __restrict__ x, const E* __restrict__ res, const float* __restrict__ gamma,
                                                               const float* __restrict__ beta, int HW, int C, int G, int S, float eps, int act,
                                                               E* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
     extern __shared__ __attribute__((aligned(16))) float gl[];
     const int T = blockDim.x, t = threadIdx.x, cpg = C / G, GS = S / cpg, tpr = S >> 3, rpp = T / tpr, C8 = C >> 3, nsl = C / S;
-    const int slots = NG == 1 ? tpr : S, nrs = max(GS, 16);
-    float* mu = gl;
-    float* rs = gl + nrs;
-    float2* lds = reinterpret_cast<float2*>(gl + 2 * nrs);
+    const int slots = NG == 1 ? tpr : S;
+    float* cn = gl;                                            // [16]
+    float2* lds = reinterpret_cast<float2*>(gl + 16);          // [T NG]
+    float* mu = gl + 16 + 2 * T * NG;
+    float* rs = mu + GS;
     const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / nsl, s0 = (id % nsl) * S;
-    const int rsub = t / tpr, cl = (t % tpr) * 8, c0 = s0 + cl;
+    const int rsub = t / tpr, cl = (t - rsub * tpr) * 8, c0 = s0 + cl;
     const bool active = rsub < rpp;
     const long long at0 = ((long long)n * HW + rsub) * C8 + (c0 >> 3), step = (long long)rpp * C8;
     E v[V];
@@ -418,13 +444,15 @@ __global__ __launch_bounds__(RES_TF) void cfl_gn_res_fwd_kernel(const E* __restr
         }
     }
     __syncthreads();
-    gn_block_stats(lds, T, slots, NG == 1 ? cpg >> 3 : cpg, GS, rpp, HW, NG == 1 ? 8.f : 1.f, eps, mu, rs);
-    if (mean && t < GS) { mean[(long long)n * G + s0 / cpg + t] = mu[t]; rstd[(long long)n * G + s0 / cpg + t] = rs[t]; }
+    gn_block_stats(lds, cn, T, slots, NG == 1 ? cpg >> 3 : cpg, GS, rpp, HW, NG == 1 ? 8.f : 1.f, eps, mu, rs);
+    if (mean) for (int g = t; g < GS; g += T) { mean[(long long)n * G + s0 / cpg + g] = mu[g]; rstd[(long long)n * G + s0 / cpg + g] = rs[g]; }
     if (!active) return;
     float sc[8], sh[8], mv[8];
+    int gi[8];
+    gn_groups(cl, cpg, gi);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int g = (cl + j) / cpg;
+        const int g = gi[j];
         sc[j] = rs[g] * gamma[c0 + j]; sh[j] = beta[c0 + j]; mv[j] = mu[g];
     }
 #pragma unroll
@@ -437,15 +465,46 @@ __global__ __launch_bounds__(RES_TF) void cfl_gn_res_fwd_kernel(const E* __restr
             for (int j = 0; j < 8; ++j) {
                 float z = fmaf(f[j] - mv[j], sc[j], sh[j]);
                 if (res) z += h[j];
-                f[j] = act == GN_RELU ? gn_act<GN_RELU>(z) : act == GN_SILU ? gn_act<GN_SILU>(z) : z;
+                f[j] = gn_act(act, z);
             }
-            y[at0 + k * step] = pack8g<E>(f);
+            gn_store(y + at0 + k * step, f);
         }
+}
+
+// the workgroup's channel sums from its row phases' (la, lb: [rpp][S]): to pc[0 .. S), pc[C .. C + S), and, weighted with gamma, their groups'
+// means s1, s2.  Two levels over the row phases, then L lanes of a wave per group; S <= T.
+__device__ __forceinline__ void gn_block_sums(float* la, float* lb, float* ta, float* tb, float* s1, float* s2, int T, int S, int GS, int cpg,
+                                              int rpp, int HW, const float* __restrict__ gamma, float* __restrict__ pc, int C) {
+    const int t = threadIdx.x, part = t / S, c = t - part * S, P = min(min(T / S, 16), rpp);
+    float a = 0.f, b = 0.f;
+    if (part < P) for (int r = part; r < rpp; r += P) { a += la[r * S + c]; b += lb[r * S + c]; }
+    __syncthreads();
+    if (part < P) { la[part * S + c] = a; lb[part * S + c] = b; }
+    __syncthreads();
+    if (t < S) {
+        float ca = 0.f, cb = 0.f;
+        for (int r = 0; r < P; ++r) { ca += la[r * S + t]; cb += lb[r * S + t]; }
+        pc[t] = ca;
+        pc[C + t] = cb;
+        ta[t] = ca * gamma[t]; tb[t] = cb * gamma[t];
+    }
+    __syncthreads();
+    int L = 1;
+    while (L < 64 && 2 * L * GS <= T && L < cpg) L *= 2;
+    const float inv = 1.f / ((float)HW * (float)cpg);
+    for (int g0 = 0; g0 < GS; g0 += T / L) {
+        const int g = g0 + t / L, l = t & (L - 1);
+        float x = 0.f, y = 0.f;
+        if (g < GS) for (int k = l; k < cpg; k += L) { x += ta[g * cpg + k]; y += tb[g * cpg + k]; }
+        for (int o = L >> 1; o > 0; o >>= 1) { x += __shfl_xor(x, o, 64); y += __shfl_xor(y, o, 64); }
+        if (g < GS && l == 0) { s1[g] = x * inv; s2[g] = y * inv; }
+    }
+    __syncthreads();
 }
 
 // backward in one pass over x, dy (dy2, res): x stays packed, dz in 32 bits.  pc [N][2][C]: the sample's sums of dz and dz xh.
 template <class E, int V>
-__global__ __launch_bounds__(RES_TB) void cfl_gn_res_bwd_kernel(const E* __restrict__ x, const E* __restrict__ dy, const E* __restrict__ dy2,
+__global__ __launch_bounds__(V <= 4 ? 256 : RES_T) void cfl_gn_res_bwd_kernel(const E* __restrict__ x, const E* __restrict__ dy, const E* __restrict__ dy2,
                                                               const E* __restrict__ res, const float* __restrict__ gamma,
                                                               const float* __restrict__ beta, const float* __restrict__ mean,
                                                               const float* __restrict__ rstd, int HW, int C, int G, int S, int act,
@@ -459,21 +518,28 @@ __global__ __launch_bounds__(RES_TB) void cfl_gn_res_bwd_kernel(const E* __restr
     float* la = tb + S;                                        // [rpp][S]
     float* lb = la + rpp * S;
     const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / nsl, s0 = (id % nsl) * S;
-    const int rsub = t / tpr, cl = (t % tpr) * 8, c0 = s0 + cl;
+    const int rsub = t / tpr, cl = (t - rsub * tpr) * 8, c0 = s0 + cl, g0 = s0 / cpg;
     const bool active = rsub < rpp;
     const long long at0 = ((long long)n * HW + rsub) * C8 + (c0 >> 3), step = (long long)rpp * C8;
     E v[V];
     float dz[V][8], mv[8], rv[8], ga[8];
-    int cnt = 0;
+    int cnt = 0, gi[8];
+    gn_groups(cl, cpg, gi);
     if (active) {
         float be[8], a8[8], b8[8];
-        E d[V];
+        E d[V], w[V];                                          // (everything is requested before anything is used)
 #pragma unroll
         for (int k = 0; k < V; ++k)
             if (rsub + k * rpp < HW) { v[k] = x[at0 + k * step]; d[k] = dy[at0 + k * step]; ++cnt; }
+        constexpr bool AHEAD = sizeof(E) == 16 || V <= 3;      // (the 32-byte records of fp32 leave no registers for it)
+        if (AHEAD && res) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (k < cnt) w[k] = res[at0 + k * step];
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int g = s0 / cpg + (cl + j) / cpg;
+            const int g = g0 + gi[j];
             mv[j] = mean[(long long)n * G + g]; rv[j] = rstd[(long long)n * G + g];
             ga[j] = gamma[c0 + j]; be[j] = beta[c0 + j];
             a8[j] = 0.f; b8[j] = 0.f;
@@ -489,14 +555,14 @@ __global__ __launch_bounds__(RES_TB) void cfl_gn_res_bwd_kernel(const E* __restr
 #pragma unroll
                     for (int j = 0; j < 8; ++j) dz[k][j] += h[j];
                 }
-                if (res) unpack8(res[at0 + k * step], h);
+                if (res) unpack8(AHEAD ? w[k] : res[at0 + k * step], h);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     xh[j] = (xh[j] - mv[j]) * rv[j];
                     if (act != GN_NONE) {
                         float z = fmaf(xh[j], ga[j], be[j]);
                         if (res) z += h[j];
-                        dz[k][j] *= act == GN_RELU ? gn_act_grad<GN_RELU>(z) : gn_act_grad<GN_SILU>(z);
+                        dz[k][j] *= gn_act_grad(act, z);
                     }
                     a8[j] += dz[k][j];
                     b8[j] = fmaf(dz[k][j], xh[j], b8[j]);
@@ -506,75 +572,256 @@ __global__ __launch_bounds__(RES_TB) void cfl_gn_res_bwd_kernel(const E* __restr
         for (int j = 0; j < 8; ++j) { la[rsub * S + cl + j] = a8[j]; lb[rsub * S + cl + j] = b8[j]; }
     }
     __syncthreads();
-    // level 1: part of the row phases of one channel; level 2: the parts of a channel, then the channels of a group
-    const int P = min(min(T / S, 32), rpp), c = t % S, part = t / S;
-    float a = 0.f, b = 0.f;
-    if (part < P) for (int r = part; r < rpp; r += P) { a += la[r * S + c]; b += lb[r * S + c]; }
-    __syncthreads();
-    if (part < P) { la[part * S + c] = a; lb[part * S + c] = b; }
-    __syncthreads();
-    if (t < S) {
-        float ca = 0.f, cb = 0.f;
-        for (int r = 0; r < P; ++r) { ca += la[r * S + t]; cb += lb[r * S + t]; }
-        pc[(long long)n * 2 * C + s0 + t] = ca;
-        pc[(long long)n * 2 * C + C + s0 + t] = cb;
-        ta[t] = ca * gamma[s0 + t]; tb[t] = cb * gamma[s0 + t];
-    }
-    __syncthreads();
-    if (t < GS) {
-        const float inv = 1.f / ((float)HW * (float)cpg);
-        float ga_ = 0.f, gb_ = 0.f;
-        for (int k = 0; k < cpg; ++k) { ga_ += ta[t * cpg + k]; gb_ += tb[t * cpg + k]; }
-        s1[t] = ga_ * inv; s2[t] = gb_ * inv;
-    }
-    __syncthreads();
+    gn_block_sums(la, lb, ta, tb, s1, s2, T, S, GS, cpg, rpp, HW, gamma + s0, pc + (long long)n * 2 * C + s0, C);
     if (!active) return;
     float c1[8], c2[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { const int g = (cl + j) / cpg; c1[j] = s1[g]; c2[j] = s2[g]; }
+    for (int j = 0; j < 8; ++j) { c1[j] = s1[gi[j]]; c2[j] = s2[gi[j]]; }
 #pragma unroll
     for (int k = 0; k < V; ++k)
         if (k < cnt) {
             float xh[8];
             unpack8(v[k], xh);
-            if (dres) dres[at0 + k * step] = pack8g<E>(dz[k]);
+            if (dres) gn_store(dres + at0 + k * step, dz[k]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 xh[j] = (xh[j] - mv[j]) * rv[j];
                 xh[j] = rv[j] * (fmaf(dz[k][j], ga[j], -c1[j]) - xh[j] * c2[j]);
             }
-            dx[at0 + k * step] = pack8g<E>(xh);
+            gn_store(dx + at0 + k * step, xh);
         }
+}
+
+// ---- the same in two passes of one workgroup over its slice, for slices that do not fit the registers: the second pass finds most of the
+// slice in the caches (L2 and the 256 MB behind it), and runs from the last row to the first, the most recently read ones.
+// Deviations are summed from the thread's first value of a channel: what that costs in digits is at most the row count times 2^-24 of
+// the squared deviation of that one value, which is itself part of the sum.
+template <class E, int NG, int U>
+__global__ __launch_bounds__(STR_T) void cfl_gn_str_fwd_kernel(const E* __restrict__ x, const E* __restrict__ res, const float* __restrict__ gamma,
+                                                               const float* __restrict__ beta, int HW, int C, int G, int S, float eps, int act,
+                                                               E* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+    extern __shared__ __attribute__((aligned(16))) float gl[];
+    const int T = blockDim.x, t = threadIdx.x, cpg = C / G, GS = S / cpg, tpr = S >> 3, rpp = T / tpr, C8 = C >> 3, nsl = C / S;
+    const int slots = NG == 1 ? tpr : S;
+    float* cn = gl;
+    float2* lds = reinterpret_cast<float2*>(gl + 16);
+    float* mu = gl + 16 + 2 * T * NG;
+    float* rs = mu + GS;
+    const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / nsl, s0 = (id % nsl) * S;
+    const int rsub = t / tpr, cl = (t - rsub * tpr) * 8, c0 = s0 + cl;
+    const bool active = rsub < rpp;
+    const long long step = (long long)rpp * C8;
+    const E* px = x + ((long long)n * HW + rsub) * C8 + (c0 >> 3);
+    const int cnt = active && rsub < HW ? (HW - rsub + rpp - 1) / rpp : 0;
+    if (active) {
+        float K[8], s[8], q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s[j] = 0.f; q[j] = 0.f; K[j] = 0.f; }
+        if (cnt) unpack8(px[0], K);
+        for (int k0 = 0; k0 < cnt; k0 += U) {
+            E v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = px[min(k0 + u, cnt - 1) * step];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float f[8];
+                unpack8(v[u], f);
+                const bool in = k0 + u < cnt;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { const float d = in ? f[j] - K[j] : 0.f; s[j] += d; q[j] = fmaf(d, d, q[j]); }
+            }
+        }
+        const float inv = cnt ? 1.f / (float)cnt : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            q[j] = fmaxf(fmaf(-s[j] * inv, s[j], q[j]), 0.f);
+            s[j] = fmaf(s[j], inv, K[j]);
+        }
+        if (NG == 1) {
+            float m = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m += s[j];
+            m *= 0.125f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { const float d = s[j] - m; m2 += fmaf((float)cnt * d, d, q[j]); }
+            lds[rsub * slots + (cl >> 3)] = make_float2(m, m2);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) lds[rsub * slots + cl + j] = make_float2(s[j], q[j]);
+        }
+    }
+    __syncthreads();
+    gn_block_stats(lds, cn, T, slots, NG == 1 ? cpg >> 3 : cpg, GS, rpp, HW, NG == 1 ? 8.f : 1.f, eps, mu, rs);
+    if (mean) for (int g = t; g < GS; g += T) { mean[(long long)n * G + s0 / cpg + g] = mu[g]; rstd[(long long)n * G + s0 / cpg + g] = rs[g]; }
+    if (!cnt) return;
+    float sc[8], sh[8], mv[8];
+    int gi[8];
+    gn_groups(cl, cpg, gi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { sc[j] = rs[gi[j]] * gamma[c0 + j]; sh[j] = beta[c0 + j]; mv[j] = mu[gi[j]]; }
+    const E* pr = res ? res + (px - x) : nullptr;
+    E* py = y + (px - x);
+    for (int k0 = cnt - 1; k0 >= 0; k0 -= U) {
+        E v[U], w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = px[max(k0 - u, 0) * step];
+        if (res) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = pr[max(k0 - u, 0) * step];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 - u < 0) break;
+            float f[8], h[8];
+            unpack8(v[u], f);
+            if (res) unpack8(w[u], h);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float z = fmaf(f[j] - mv[j], sc[j], sh[j]);
+                if (res) z += h[j];
+                f[j] = gn_act(act, z);
+            }
+            gn_store(py + (k0 - u) * step, f);
+        }
+    }
+}
+
+template <class E, int U>
+__global__ __launch_bounds__(STR_T) void cfl_gn_str_bwd_kernel(const E* __restrict__ x, const E* __restrict__ dy, const E* __restrict__ dy2,
+                                                               const E* __restrict__ res, const float* __restrict__ gamma,
+                                                               const float* __restrict__ beta, const float* __restrict__ mean,
+                                                               const float* __restrict__ rstd, int HW, int C, int G, int S, int act,
+                                                               E* __restrict__ dx, E* __restrict__ dres, float* __restrict__ pc) {
+    extern __shared__ __attribute__((aligned(16))) float gl[];
+    const int T = blockDim.x, t = threadIdx.x, cpg = C / G, GS = S / cpg, tpr = S >> 3, rpp = T / tpr, C8 = C >> 3, nsl = C / S;
+    float* s1 = gl;
+    float* s2 = gl + GS;
+    float* ta = gl + 2 * GS;
+    float* tb = ta + S;
+    float* la = tb + S;
+    float* lb = la + rpp * S;
+    const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / nsl, s0 = (id % nsl) * S;
+    const int rsub = t / tpr, cl = (t - rsub * tpr) * 8, c0 = s0 + cl, g0 = s0 / cpg;
+    const bool active = rsub < rpp;
+    const long long at0 = ((long long)n * HW + rsub) * C8 + (c0 >> 3), step = (long long)rpp * C8;
+    const int cnt = active && rsub < HW ? (HW - rsub + rpp - 1) / rpp : 0;
+    float mv[8], rv[8], ga[8], be[8];
+    int gi[8];
+    gn_groups(cl, cpg, gi);
+    const auto load = [&](int k, E& xv, float (&dz)[8], E& hv) {
+        const long long at = at0 + k * step;
+        xv = x[at];
+        gn_dy(dy, dy2, at, dz);
+        if (res) hv = res[at];
+    };
+    const auto form = [&](const E& xv, const E& hv, float (&xh)[8], float (&dz)[8]) {
+        float h[8];
+        unpack8(xv, xh);
+        if (res) unpack8(hv, h);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            xh[j] = (xh[j] - mv[j]) * rv[j];
+            if (act != GN_NONE) {
+                float z = fmaf(xh[j], ga[j], be[j]);
+                if (res) z += h[j];
+                dz[j] *= gn_act_grad(act, z);
+            }
+        }
+    };
+    if (active) {
+        float a8[8], b8[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            mv[j] = mean[(long long)n * G + g0 + gi[j]]; rv[j] = rstd[(long long)n * G + g0 + gi[j]];
+            ga[j] = gamma[c0 + j]; be[j] = beta[c0 + j];
+            a8[j] = 0.f; b8[j] = 0.f;
+        }
+        for (int k0 = 0; k0 < cnt; k0 += U) {
+            E xv[U], hv[U];
+            float dz[U][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(min(k0 + u, cnt - 1), xv[u], dz[u], hv[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 + u >= cnt) break;
+                float xh[8];
+                form(xv[u], hv[u], xh, dz[u]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { a8[j] += dz[u][j]; b8[j] = fmaf(dz[u][j], xh[j], b8[j]); }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { la[rsub * S + cl + j] = a8[j]; lb[rsub * S + cl + j] = b8[j]; }
+    }
+    __syncthreads();
+    gn_block_sums(la, lb, ta, tb, s1, s2, T, S, GS, cpg, rpp, HW, gamma + s0, pc + (long long)n * 2 * C + s0, C);
+    if (!cnt) return;
+    float c1[8], c2[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { c1[j] = s1[gi[j]]; c2[j] = s2[gi[j]]; }
+    for (int k0 = cnt - 1; k0 >= 0; k0 -= U) {
+        E xv[U], hv[U];
+        float dz[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(max(k0 - u, 0), xv[u], dz[u], hv[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 - u < 0) break;
+            const long long at = at0 + (k0 - u) * step;
+            float xh[8];
+            form(xv[u], hv[u], xh, dz[u]);
+            if (dres) gn_store(dres + at, dz[u]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) xh[j] = rv[j] * (fmaf(dz[u][j], ga[j], -c1[j]) - xh[j] * c2[j]);
+            gn_store(dx + at, xh);
+        }
+    }
 }
 
 inline int gn_gcd(int a, int b) { while (b) { const int r = a % b; a = b; b = r; } return a; }
 
-// Slice width and threads of the one-pass kernels for records of `size` bytes an element and at most V records a thread, or S = 0.
-// Slices are whole groups and whole records; the widest one up to 128 bytes a row that fits (a row's neighbours then share no cache
-// line), else the narrowest possible.  `words`: 32-bit words of LDS per channel and row phase.
-inline ResPlan gn_plan(int HW, int C, int G, int size, int V, bool bwd) {
+// How a call is run: slices of S channels (whole groups, whole records) by workgroups of T threads, in one pass over registers (kind 1) or
+// two passes (2), or all channels in chunks of rows by several launches (0).
+struct Plan { int kind, S, T; bool few; };
+// One pass where a slice of 64 or 128 bytes a row (a narrower one shares its cache lines with its neighbours) fits half a CU's threads at
+// V records each, so that one workgroup's loads run beside another's stores; else two passes where there is a slice for every CU; else
+// (few samples, large maps) chunks.  Measured, forward / forward with residual / backward with residual, microseconds:
+//   bf16 256 x 56 x 56 x 256: one pass 242 / 307 / 684 (32-byte slices), two passes 225 / 288 / 609
+//   bf16 128 x 28 x 28 x 512: one pass 47 / 67 / 139, two passes 64 / 81 / 155;  fp32 128 x 28 x 28 x 128: 23 / 28 / 52, 27 / 34 / 66
+//   bf16 64 x 112 x 112 x 64 (128 slices): two passes 67 / 116 / 247, chunks 86 / 160 / 222
+inline Plan gn_plan(int N, int HW, int C, int G, int size, bool bwd) {
     const int cpg = C / G, unit = cpg / gn_gcd(cpg, 8) * 8;     // lcm(cpg, 8)
-    ResPlan best{0, 0};
+    const int V = bwd ? (size == 2 ? RES_B16 : RES_B32) : (size == 2 ? RES_V16 : RES_V32);
+    const int few = size == 2 ? RES_F16 : RES_F32;
+    Plan best{0, 0, 0, false};
+    int wide = 0;                                              // the widest slice up to 128 bytes (or the narrowest possible)
     for (int S = unit; S <= C; S += unit) {
         if (C % S) continue;
-        if (best.S && S * size > 128) break;
-        const int tpr = S >> 3;
-        const int most = bwd ? RES_TB : RES_TF;
-        if (tpr > most || (bwd || cpg % 8 ? S : tpr) > most) break;
-        if ((long long)(most / tpr) * V < HW) break;
-        const long long rec = (long long)HW * tpr;
-        int T = 128;
-        while (T < most && (T * 4 < rec || (long long)(T / tpr) * V < HW || (bwd || cpg % 8 ? S : tpr) > T)) T *= 2;
-        best.S = S; best.T = T;
+        if (wide && S * size > 128) break;
+        // (a wider slice than 64 bytes only where workgroups are plenty: fp32 128 x 28 x 28 x 128 backward 40 against 44)
+        if (wide * size >= 64 && (long long)N * (C / S) < (best.kind ? 1024 : 256)) break;
+        wide = S;
+        const int tpr = S >> 3, slots = bwd || cpg % 8 ? S : tpr;
+        if (slots > 512 || (long long)(512 / tpr) * V < HW || (S * size < 64 && S < C && HW > 64)) continue;
+        int T = 64;
+        while ((long long)(T / tpr) * V < HW || slots > T) T *= 2;
+        best.kind = 1; best.S = S; best.T = T;
+        // rows of a few records a thread: leaner registers, more workgroups at a time
+        while (T < 512 && (long long)(T / tpr) * few < HW && (long long)T * few < (long long)HW * tpr * 2) T *= 2;
+        best.few = (long long)(T / tpr) * few >= HW && T <= 256;
+        if (best.few) best.T = T;
     }
+    if (best.kind == 0 && wide && (bwd || cpg % 8 ? wide : wide >> 3) <= STR_T && (long long)N * (C / wide) >= (bwd ? 256 : 128)) {
+        best.kind = 2; best.S = wide; best.T = STR_T;
+        while (best.T > 256 && (long long)(best.T >> 1) * 8 >= (long long)HW * (wide >> 3) && (bwd || cpg % 8 ? wide : wide >> 3) <= best.T >> 1)
+            best.T >>= 1;                                      // (eight records a thread are enough)
+    }
+    if (best.kind && (long long)N * (C / best.S) > 0x7fffffffll) best.kind = 0;
     return best;
 }
 
 // rows per chunk: one register load per thread (RPT rows), the chunk count bounded so that its merge stays short
-inline int gn_rows(int HW, int C) {
-    const int rpp = GN_T / (C >> 3);
-    return rpp * GN_RPT;
-}
+inline int gn_rows(int HW, int C) { return GN_T / (C >> 3) * GN_RPT; }
 inline bool gn_bad(const void* x, int N, int HW, int C, int G) { return !x || N < 1 || HW < 1 || C < 1 || G < 1 || C % G != 0; }
 inline bool gn_limit(int N, int HW, int C) { return C % 8 != 0 || C > GN_MAXC || N > 65535; }
 
@@ -584,7 +831,7 @@ extern "C" {
 
 size_t cfl_gn_ws_bytes(int N, int HW, int C, int G) {
     if (N < 1 || HW < 1 || C < 8 || G < 1 || C % G || gn_limit(N, HW, C)) return 0;
-    const size_t chunks = cfl_cdiv(HW, gn_rows(HW, C));
+    const size_t chunks = cfl_cdiv(HW, gn_rows(HW, C));        // (also enough for the one-workgroup kernels: [N][2][C])
     return cfl_align256((size_t)N * chunks * G * 2 * 4) + cfl_align256((size_t)N * chunks * C * 2 * 4);
 }
 
@@ -605,20 +852,32 @@ int cfl_gn_fwd(const void* x, const void* res, const float* gamma, const float* 
     if (((uintptr_t)x | (uintptr_t)res | (uintptr_t)y) & 15) return CFL_EALIGN;
     if (gn_limit(N, HW, C)) return CFL_ELIMIT;
     hipStream_t stream = (hipStream_t)stream_;
-    const ResPlan rp = gn_plan(HW, C, G, dtype ? 2 : 4, dtype ? RES_V16 : RES_V32, false);
-    if (rp.S && (long long)N * (C / rp.S) <= 0x7fffffffll) {
-        const int ng = (C / G) % 8 ? 8 : 1, gs = rp.S / (C / G), nrs = gs < 16 ? 16 : gs;
-        const size_t lds = (size_t)2 * nrs * 4 + (size_t)rp.T * ng * 8;
-        const dim3 rg((unsigned)(N * (C / rp.S)));
-#define GN_RES(E, NG, V)                                                                                                                   \
-    do {                                                                                                                                   \
-        CFL_SET_LDS((cfl_gn_res_fwd_kernel<E, NG, V>), 96 * 1024);                                                                         \
-        CFL_LAUNCH(K_GN_RES, (cfl_gn_res_fwd_kernel<E, NG, V>), rg, dim3(rp.T), lds, stream, (const E*)x, (const E*)res, gamma, beta, HW, C, \
-                   G, rp.S, eps, act, (E*)y, mean, rstd);                                                                                  \
+    const Plan p = gn_plan(N, HW, C, G, dtype ? 2 : 4, false);
+    if (p.kind) {
+        const int ng = (C / G) % 8 ? 8 : 1, gs = p.S / (C / G);
+        const size_t lds = (size_t)(16 + 2 * gs) * 4 + (size_t)p.T * ng * 8;
+        const dim3 rg((unsigned)(N * (C / p.S)));
+#define GN_ONE(KERN)                                                                                                                     \
+    do {                                                                                                                                 \
+        CFL_SET_LDS(KERN, 96 * 1024);                                                                                                    \
+        CFL_LAUNCH(K_GN_RES, KERN, rg, dim3(p.T), lds, stream, (const GE*)x, (const GE*)res, gamma, beta, HW, C, G, p.S, eps, act, (GE*)y, \
+                   mean, rstd);                                                                                                          \
     } while (0)
-        if (dtype == 0 && ng == 1) { GN_RES(F8, 1, RES_V32); } else if (dtype == 0) { GN_RES(F8, 8, RES_V32); }
-        else if (ng == 1) { GN_RES(U4, 1, RES_V16); } else { GN_RES(U4, 8, RES_V16); }
-#undef GN_RES
+#define GN_KIND(NG, VF, V)                                                                \
+    do {                                                                                  \
+        if (p.kind == 2) { GN_ONE((cfl_gn_str_fwd_kernel<GE, NG, 4>)); }                  \
+        else if (p.few) { GN_ONE((cfl_gn_res_fwd_kernel<GE, NG, VF>)); }                  \
+        else { GN_ONE((cfl_gn_res_fwd_kernel<GE, NG, V>)); }                              \
+    } while (0)
+        if (dtype == 0) {
+            typedef F8 GE;
+            if (ng == 1) { GN_KIND(1, RES_F32, RES_V32); } else { GN_KIND(8, RES_F32, RES_V32); }
+        } else {
+            typedef U4 GE;
+            if (ng == 1) { GN_KIND(1, RES_F16, RES_V16); } else { GN_KIND(8, RES_F16, RES_V16); }
+        }
+#undef GN_ONE
+#undef GN_KIND
         return 0;
     }
     const int rows = gn_rows(HW, C);
@@ -646,20 +905,27 @@ int cfl_gn_bwd(const void* dy, const void* dy2, const void* x, const void* res, 
     if (((uintptr_t)x | (uintptr_t)res | (uintptr_t)dy | (uintptr_t)dy2 | (uintptr_t)dx | (uintptr_t)dres) & 15) return CFL_EALIGN;
     if (gn_limit(N, HW, C)) return CFL_ELIMIT;
     hipStream_t stream = (hipStream_t)stream_;
-    const ResPlan rp = gn_plan(HW, C, G, dtype ? 2 : 4, dtype ? RES_B16 : RES_B32, true);
-    if (rp.S && (long long)N * (C / rp.S) <= 0x7fffffffll) {
-        const int rpp = rp.T / (rp.S >> 3);
-        const size_t lds = (size_t)2 * (rp.S / (C / G) + rp.S + rpp * rp.S) * 4;
-        const dim3 rg((unsigned)(N * (C / rp.S)));
+    const Plan p = gn_plan(N, HW, C, G, dtype ? 2 : 4, true);
+    if (p.kind) {
+        const int rpp = p.T / (p.S >> 3);
+        const size_t lds = (size_t)2 * (p.S / (C / G) + p.S + rpp * p.S) * 4;
+        const dim3 rg((unsigned)(N * (C / p.S)));
         float* pcr = (float*)ws;
-#define GN_RES(E, V)                                                                                                                        \
-    do {                                                                                                                                    \
-        CFL_SET_LDS((cfl_gn_res_bwd_kernel<E, V>), 96 * 1024);                                                                              \
-        CFL_LAUNCH(K_GN_RES, (cfl_gn_res_bwd_kernel<E, V>), rg, dim3(rp.T), lds, stream, (const E*)x, (const E*)dy, (const E*)dy2,          \
-                   (const E*)res, gamma, beta, mean, rstd, HW, C, G, rp.S, act, (E*)dx, want_dres ? (E*)dres : (E*)nullptr, pcr);           \
+#define GN_ONE(KERN)                                                                                                                    \
+    do {                                                                                                                                \
+        CFL_SET_LDS(KERN, 96 * 1024);                                                                                                   \
+        CFL_LAUNCH(K_GN_RES, KERN, rg, dim3(p.T), lds, stream, (const GE*)x, (const GE*)dy, (const GE*)dy2, (const GE*)res, gamma, beta, \
+                   mean, rstd, HW, C, G, p.S, act, (GE*)dx, want_dres ? (GE*)dres : (GE*)nullptr, pcr);                                 \
     } while (0)
-        if (dtype == 0) { GN_RES(F8, RES_B32); } else { GN_RES(U4, RES_B16); }
-#undef GN_RES
+#define GN_KIND(VF, V)                                                                    \
+    do {                                                                                  \
+        if (p.kind == 2) { GN_ONE((cfl_gn_str_bwd_kernel<GE, 2>)); }                      \
+        else if (p.few) { GN_ONE((cfl_gn_res_bwd_kernel<GE, VF>)); }                      \
+        else { GN_ONE((cfl_gn_res_bwd_kernel<GE, V>)); }                                  \
+    } while (0)
+        if (dtype == 0) { typedef F8 GE; GN_KIND(RES_F32, RES_B32); } else { typedef U4 GE; GN_KIND(RES_F16, RES_B16); }
+#undef GN_ONE
+#undef GN_KIND
         CFL_LAUNCH(K_GN_BWD_FINAL, cfl_gn_bwd_final_kernel, dim3(cfl_cdiv(C, 16)), dim3(1024), 0, stream, pcr, N, C, dgamma, dbeta);
         return 0;
     }
