@@ -221,14 +221,15 @@ def _gn_plain(s):
 
 
 def _gn_own(s):
-    from creamfl_amd import ops
+    from creamfl_amd import ops, runtime
     c = s['case']
     if not c['train']:
         with torch.no_grad():
             return [ops.gn_act(s['x'], s['gamma'], s['beta'], c['groups'], act=c['act'], residual=s['res'])]
     leaves = [s[k].detach().requires_grad_(True) for k in ('x', 'gamma', 'beta', 'res') if s[k] is not None]
     y = ops.gn_act(leaves[0], leaves[1], leaves[2], c['groups'], act=c['act'], residual=leaves[3] if s['res'] is not None else None)
-    return [y.detach(), *torch.autograd.grad(y, leaves, s['dy'])]
+    with runtime.backward_here():                              # (the framework's steps run their backward on the calling thread)
+        return [y.detach(), *torch.autograd.grad(y, leaves, s['dy'])]
 
 
 def _gn_exact(s):
@@ -286,14 +287,15 @@ def _dropout_plain(s):
 
 
 def _dropout_own(s):
-    from creamfl_amd import ops
+    from creamfl_amd import ops, runtime
     c = s['case']
     if not c['train']:
         with torch.no_grad():
             return [ops.dropout(s['x'], c['p'], seed=s['seed'])]
     x = s['x'].detach().requires_grad_(True)
     y = ops.dropout(x, c['p'], seed=s['seed'])
-    return [y.detach(), *torch.autograd.grad(y, [x], s['dy'])]
+    with runtime.backward_here():
+        return [y.detach(), *torch.autograd.grad(y, [x], s['dy'])]
 
 
 def _dropout_exact(s):
@@ -379,7 +381,7 @@ def _attn_plain(s):
 
 
 def _attn_own(s):
-    from creamfl_amd import ops
+    from creamfl_amd import ops, runtime
     c = s['case']
     names = ('q', 'kv', 'table') if c['form'] == 'cls' else ('qkv', 'table')
     leaves = [s[k].detach().requires_grad_(c['train']) for k in names]
@@ -389,7 +391,10 @@ def _attn_own(s):
         o = ops.relpos_attention_varlen(leaves[0], s['cu'], c['l'], leaves[1], s['buckets'], c['heads'])
     else:
         o = ops.relpos_attention(leaves[0], leaves[1], s['buckets'], c['heads'], key_mask=s['mask'])
-    return [o.detach(), *torch.autograd.grad(o, leaves, s['do'])] if c['train'] else [o]
+    if not c['train']:
+        return [o]
+    with runtime.backward_here():
+        return [o.detach(), *torch.autograd.grad(o, leaves, s['do'])]
 
 
 def _attn_exact(s):
