@@ -16,6 +16,7 @@
 // one query and its keys sit in the lane's registers; registers 8 kk .. 8 kk + 7 are then, packed to bf16, the second operand of the
 // following product (o^T = V^T P^T) whose first operand is read transposed out of LDS in the same key order (ds_read_b64_tr_b16).
 // P and ds are rounded to bf16 there (2^-9 relative, the precision of v and k themselves); sums stay in 32 bits.
+#include <limits.h>
 #include "common.h"
 
 namespace {
@@ -38,7 +39,7 @@ struct RpArgs {
     long long lddq, lddk;
     const unsigned char* mask;              // [B][Lk] key mask (non-zero = takes part) or NULL
     const int* cu;                          // packed form: text b = rows cu[b] .. cu[b + 1] - 1 of [T] rows; NULL = padded
-    int B, Lq, Lk, T, heads;                // Lq = 0: the queries are the packed rows themselves; Lk: (about) the longest text
+    int B, Lq, Lk, T, heads;                // Lq = 0: the queries are the packed rows themselves; Lk: the longest text
     float scale2;                           // scale * log2(e)
     float scale;
     const void* table;                      // [nb][heads]
@@ -54,18 +55,45 @@ struct RpArgs {
     long long rows, krows;                  // query rows, key rows in all
 };
 
-// rows of text b
-struct Text { long long q0, k0; int lq, lk; };
+// rows of text b; a packed text longer than Lk is cut to its first Lk rows (`to`: where its rows end)
+struct Text { long long q0, k0, to; int lq, lk; };
 __device__ __forceinline__ Text text_of(const RpArgs& a, int b) {
     Text t;
     if (a.cu) {
         const int r0 = min(max(a.cu[b], 0), a.T), r1 = min(max(a.cu[b + 1], r0), a.T);
-        t.k0 = r0; t.lk = r1 - r0;
+        t.k0 = r0; t.to = r1; t.lk = min(r1 - r0, a.Lk);
         t.q0 = a.Lq ? (long long)b * a.Lq : r0; t.lq = a.Lq ? a.Lq : t.lk;
     } else {
-        t.q0 = (long long)b * a.Lq; t.k0 = (long long)b * a.Lk; t.lq = a.Lq; t.lk = a.Lk;
+        t.q0 = (long long)b * a.Lq; t.k0 = (long long)b * a.Lk; t.lq = a.Lq; t.lk = a.Lk; t.to = t.k0 + a.Lk;
     }
     return t;
+}
+// head h's 64 columns of rows from .. to - 1: zeros
+template <int NT>
+__device__ __forceinline__ void zero_rows(u16* p, long long ld, int h, long long from, long long to) {
+    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    for (long long i = threadIdx.x; i < (to - from) * 8; i += NT) *reinterpret_cast<f32x4*>(p + (from + (i >> 3)) * ld + h * 64 + (i & 7) * 8) = z;
+}
+// The packed rows that belong to no text, or to a text's cut part: zeros, written by the workgroups of the text before (the first text's:
+// also what stands before it).  Split: the join writes the rows before cu[B], from parts that are empty there (zeros; maximum -inf).
+template <int NT>
+__device__ __forceinline__ void clear_rest(const RpArgs& a, const Text& t, int b, int h, int sp, u16* p, u16* p2, long long ld) {
+    const long long ends[3][2] = {{b == 0 ? 0 : t.k0, t.k0}, {t.k0 + t.lk, t.to}, {t.to, b == a.B - 1 ? a.T : t.to}};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const long long from = ends[i][0], to = ends[i][1];
+        if (a.ns == 1 || (i == 2 && sp == 0)) {
+            zero_rows<NT>(p, ld, h, from, to);
+            if (p2) zero_rows<NT>(p2, ld, h, from, to);
+        } else if (i < 2) {
+            const long long at = ((long long)sp * a.heads + h) * a.T;
+            for (long long r = (at + from) * 64 + threadIdx.x; r < (at + to) * 64; r += NT) {
+                a.po[r] = 0.f;
+                if (p2) a.pv[r] = 0.f;
+            }
+            if (a.pm) for (long long r = at + from + threadIdx.x; r < at + to; r += NT) { a.pm[2 * r] = -INFINITY; a.pm[2 * r + 1] = 0.f; }
+        }
+    }
 }
 
 __device__ __forceinline__ int acc_r(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
@@ -192,6 +220,7 @@ __device__ __forceinline__ BlockBias block_bias(const float* bl, int R, int d0, 
     x.p = bl + R + BPAD + (x.near ? d0 : 0) + (KEY_LANE ? (lane & 31) - 4 * (lane >> 5) : 4 * (lane >> 5) - (lane & 31));
     return x;
 }
+__device__ __forceinline__ void lds_add(float* p, float v) { __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 __device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 
 // a lane's 32 values of its row in 32 bits: out [64]
@@ -216,14 +245,15 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
+    if (a.cu && !a.Lq && qb == 0) clear_rest<NT>(a, t, b, h, sp, a.out, nullptr, a.ldo);
     if (qb * NW * 32 >= t.lq) return;
     const Part part = part_of(sp, a.ns, t.lk, KT);
     fill_bias<NT>(a, h, bl, -(t.lq | (NW * 32 - 1)), t.lk | (KT - 1));     // (rows past the end are computed with as well)
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
-    for (int blk = qb; blk * NW * 32 < t.lq; blk += a.nqb) {
-        const int q0 = blk * NW * 32 + w * 32;
+    {
+        const int q0 = qb * NW * 32 + w * 32;
         bf16x8 qf[4];
         load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, q0, t.lq, lane, qf);
         f32x16 o[2];
@@ -331,21 +361,32 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     }
 }
 
-// rows behind the last text of a packed batch: zeros (grid-stride over 16-byte pieces of `width` bf16 per row)
-__global__ __launch_bounds__(256) void cfl_relpos_tail_kernel(const int* __restrict__ cu, int B, int T, u16* p, long long ld, int width) {
-    const int r0 = min(max(cu[B], 0), T), per = width / 8;
-    const long long n = (long long)(T - r0) * per;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        *reinterpret_cast<f32x4*>(p + (r0 + i / per) * ld + (i % per) * 8) = z;
+// Sums of a 32 x 32 block along its diagonals.  Register r of lane (x, half) holds query x and key kr = (r & 3) + 8 (r >> 2) + 4 half; read
+// from lane (x + kr) mod 32 it is the value of distance d0 - x, or d0 - x + 32 where that wrapped.  `here` + the block before's `next` are
+// the sums of the distances d0 - x.
+struct Diag {
+    float here, next;
+    __device__ __forceinline__ void add(const f32x16& v, int lane) {
+        const int at = 4 * ((lane & 31) + 4 * (lane >> 5)), half = 4 * (lane & 32);
+        here = next;
+        next = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int to = at + 4 * ((r & 3) + 8 * (r >> 2));
+            const float f = __int_as_float(__builtin_amdgcn_ds_bpermute((to & 124) | half, __float_as_int(v[r])));
+            const bool over = to >= 128;
+            here += over ? 0.f : f;
+            next += over ? f : 0.f;
+        }
     }
-}
+};
 
 // ---- backward, queries: D, dQ and the bias gradient.  Same ownership as the forward.
-// The bias gradient of a distance is the sum of ds along a diagonal.  A lane's 16 values of a near block lie on 16 diagonals: each wave
-// adds them to LDS words of its own, one word per distance and lane half -- the addresses of one instruction are distinct and a wave's
-// LDS operations stay in order, so the sum's order is fixed.  Far blocks are summed in registers.  At the end the workgroup's sums per
-// distance are gathered by bucket: part [heads][slots][nb], one slot per (text, query block).
+// The bias gradient of a distance is the sum of ds along a diagonal.  A lane's 16 values of a near block lie on 16 diagonals: each is moved
+// to the lane of its diagonal (key - query mod 32; `Diag`) and summed in registers, with one LDS addition per block into words of the
+// wave's own (the addresses of one instruction are distinct and a wave's LDS operations stay in order, so the sum's order is fixed;
+// adding all 16 in LDS took 340 us instead of @DQ@ at 32 texts of 512 tokens, 12 heads).  Far blocks are summed in registers.  At the end the
+// workgroup's sums per distance are gathered by bucket: part [heads][slots][nb], one slot per (text, query block, part).
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     constexpr int NT = NW * 64, U = KT / 32;
@@ -361,6 +402,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     const Text t = text_of(a, b);
     const Part part = part_of(sp, a.ns, t.lk, KT);
     float* out = a.diag + ((((long long)h * a.B + b) * a.nqb + qb) * a.ns + sp) * a.nb;
+    if (a.cu && !a.Lq && qb == 0) clear_rest<NT>(a, t, b, h, sp, a.dq, nullptr, a.lddq);
     if (qb * NW * 32 >= t.lq || t.lk == 0) {
         for (int i = threadIdx.x; i < a.nb; i += NT) out[i] = 0.f;
         if (t.lk == 0 && a.Lq)                                 // queries of their own without a key: no gradient
@@ -382,11 +424,17 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
         for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) dg[c * nd + d + mid] = 0.f;
     float far_lo = 0.f, far_hi = 0.f;
     float* mine = dg + (2 * w + (lane >> 5)) * nd;
+    Diag dg_{0.f, 0.f};
+    int dn = INT_MIN;                                          // the distance (first key - first query) that dg_.next belongs to
+    const auto flush = [&]() {
+        if (dn != INT_MIN) lds_add(mine + mid + dn - (lane & 31), dg_.next);
+        dg_.next = 0.f;
+    };
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
-    for (int blk = qb; blk * NW * 32 < t.lq; blk += a.nqb) {
-        const int q0 = blk * NW * 32 + w * 32;
+    {
+        const int q0 = qb * NW * 32 + w * 32;
         const int row = q0 + (lane & 31);
         const bool live = row < t.lq;
         bf16x8 qf[4], gf[4];
@@ -455,10 +503,10 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - D);
                     if (bb.near) {
-                        float* dst = mine + (bb.p - bl);
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            __hip_atomic_fetch_add(dst + (r & 3) + 8 * (r >> 2), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                        if (d0 != dn) flush();                 // (not the block after the last near one)
+                        dg_.add(s, lane);
+                        lds_add(mine + mid + d0 - (lane & 31), dg_.here);
+                        dn = d0 + 32;
                     } else {
                         float x = 0.f;
 #pragma unroll
@@ -496,6 +544,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
                 }
         }
     }
+    flush();
     // the workgroup's sums per distance ...
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
@@ -535,6 +584,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, kb = id / a.ns % nkb, h = id / (a.ns * nkb) % a.heads, b = id / (a.ns * nkb * a.heads);
     const Text t = text_of(a, b);
+    if (a.cu && kb == 0) clear_rest<NT>(a, t, b, h, sp, a.dk, a.dv, a.lddk);
     if (kb * NW * 32 >= t.lk) return;
     const Part part = part_of(sp, a.ns, t.lq, KT);
     fill_bias<NT>(a, h, bl, -(t.lq | (KT - 1)), t.lk | (NW * 32 - 1));
@@ -543,8 +593,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     const u16* gp = a.dout + t.q0 * a.ldo + h * 64;
     const float* lp = a.lse + h * a.rows + t.q0;
     const float* dp_ = a.dsum + h * a.rows + t.q0;
-    for (int blk = kb; blk * NW * 32 < t.lk; blk += nkb) {
-        const int k0 = blk * NW * 32 + w * 32;
+    {
+        const int k0 = kb * NW * 32 + w * 32;
         const int key = k0 + (lane & 31);
         const bool live = key < t.lk && (!mask || mask[key]);
         f32x16 dk[2], dv[2];
@@ -642,6 +692,148 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     }
 }
 
+// ---- backward of texts of at most 32 tokens: everything in one kernel, a wave per (text, head).  The rows come straight from memory as
+// operands; K, Q and dO pass through LDS for the products that contract over rows.  D is summed from p and dp themselves, so the
+// rounding of o plays no part.  The bias gradient's diagonals go to memory as they are: part [heads][B][64], place d + 32.
+// 256 packed captions of 8 to 32 tokens, 12 heads: @B32@ us, against @B32OLD@ with the kernels for long texts.
+__global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
+    __shared__ __attribute__((aligned(16))) u16 Kt[32 * TP], Qt[32 * TP], Gt[32 * TP];
+    __shared__ float bl[64];
+    __shared__ __attribute__((aligned(16))) float ls[32], Ds[32];
+    const int lane = threadIdx.x, x = lane & 31, half = lane >> 5;
+    const int id = xcd_remap(blockIdx.x, gridDim.x), h = id % a.heads, b = id / a.heads;
+    const Text t = text_of(a, b);
+    float* part = a.diag + ((long long)h * a.B + b) * 64;
+    if (a.cu) {
+        if (!a.Lq) clear_rest<64>(a, t, b, h, 0, a.dq, nullptr, a.lddq);
+        clear_rest<64>(a, t, b, h, 0, a.dk, a.dv, a.lddk);
+    }
+    if (t.lq == 0 || t.lk == 0) {
+        part[lane] = 0.f;
+        zero_rows<64>(a.dq, a.lddq, h, t.q0, t.q0 + t.lq);
+        return;
+    }
+    const u32 bits = (u32)__ballot(lane < t.lk && (!a.mask || a.mask[(long long)b * a.Lk + min(lane, t.lk - 1)] != 0));
+    const bool keep = (bits >> x) & 1;
+    bf16x8 kf[4], vf[4], qf[4], gf[4];
+    load_rows(a.k + t.k0 * a.ldk + h * 64, a.ldk, 0, t.lk, lane, kf);
+    load_rows(a.v + t.k0 * a.ldk + h * 64, a.ldk, 0, t.lk, lane, vf);
+    load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, 0, t.lq, lane, qf);
+    load_rows(a.dout + t.q0 * a.ldo + h * 64, a.ldo, 0, t.lq, lane, gf);
+    const float lse = x < t.lq ? a.lse[h * a.rows + t.q0 + x] : INFINITY;
+    {
+        const int d = min(max(lane - 31, -a.R), a.R);
+        const int bk = min(max(a.bucket[d + a.R], 0), a.nb - 1);
+        bl[lane] = LOG2E * (a.table_bf16 ? __uint_as_float((u32)((const u16*)a.table)[(long long)bk * a.heads + h] << 16)
+                                         : ((const float*)a.table)[(long long)bk * a.heads + h]);
+    }
+    const f32x4 z4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        const int at = x * TP + kk * 16 + half * 8;
+        if (!keep) { kf[kk] = __builtin_bit_cast(bf16x8, z4); vf[kk] = __builtin_bit_cast(bf16x8, z4); }
+        *reinterpret_cast<bf16x8*>(Kt + at) = kf[kk];
+        *reinterpret_cast<bf16x8*>(Qt + at) = qf[kk];
+        *reinterpret_cast<bf16x8*>(Gt + at) = gf[kk];
+    }
+    __syncthreads();
+    f32x16 s, dp;
+    // lane = query
+    zero16(s); zero16(dp);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf[kk], s, 0, 0, 0);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[kk], gf[kk], dp, 0, 0, 0);
+    }
+    float D = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int kr = (r & 3) + 8 * (r >> 2);
+        const bool ok = (bits >> (kr + 4 * half)) & 1;
+        const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bl[31 + 4 * half - x + kr] - lse)) : 0.f;
+        s[r] = p;
+        D = fmaf(p, dp[r], D);
+    }
+    D += __shfl_xor(D, 32, 64);
+    if (lane < 32) { ls[x] = lse; Ds[x] = D; }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= dp[r] - D;
+    Diag dg{0.f, 0.f};
+    dg.add(s, lane);
+    dg.here += __shfl_xor(dg.here, 32, 64);
+    dg.next += __shfl_xor(dg.next, 32, 64);
+    part[half && x ? 64 - x : half ? 0 : 32 - x] = half ? dg.next : dg.here;      // (distance 32 does not occur: next of x = 0 is zero)
+    f32x16 out[2];
+    const auto store = [&](u16* p, long long ld, bool on, bool live, float c) {
+        if (!on) return;
+        u16* op = p + x * ld + 4 * half;
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint2 v;
+                v.x = live ? pack2(out[dt][4 * g] * c, out[dt][4 * g + 1] * c) : 0u;
+                v.y = live ? pack2(out[dt][4 * g + 2] * c, out[dt][4 * g + 3] * c) : 0u;
+                *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
+            }
+    };
+    const auto apply = [&](const u16* tile, const f32x16& w) {
+        zero16(out[0]); zero16(out[1]);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const bf16x8 f = pack_acc(w, kk);
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt) out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(tile, 16 * kk, dt, lane), f, out[dt], 0, 0, 0);
+        }
+    };
+    apply(Kt, s);
+    store(a.dq + t.q0 * a.lddq + h * 64, a.lddq, x < t.lq, true, a.scale);
+    __syncthreads();
+    // lane = key
+    zero16(s); zero16(dp);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[kk], kf[kk], s, 0, 0, 0);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gf[kk], vf[kk], dp, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int i = acc_r(r, lane);
+        const float p = keep ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bl[31 + x - i] - ls[i])) : 0.f;
+        s[r] = p;
+        dp[r] = keep ? p * (dp[r] - Ds[i]) : 0.f;
+    }
+    apply(Gt, s);
+    store(a.dv + t.k0 * a.lddk + h * 64, a.lddk, x < t.lk, keep, 1.f);
+    apply(Qt, dp);
+    store(a.dk + t.k0 * a.lddk + h * 64, a.lddk, x < t.lk, keep, a.scale);
+}
+// ... and its bias gradient: the texts' sums per distance, then the buckets.  grid = heads
+__global__ __launch_bounds__(1024) void cfl_relpos_dtable32_kernel(const float* __restrict__ part, const int* __restrict__ bucket, int R, int nb,
+                                                                   int heads, int B, void* dtable, int bf16) {
+    __shared__ float red[16][64];
+    __shared__ int bk[64];
+    const int h = blockIdx.x, d = threadIdx.x & 63, strand = threadIdx.x >> 6;
+    const float* p = part + (long long)h * B * 64 + d;
+    float x = 0.f;
+    for (int b = strand; b < B; b += 16) x += p[(long long)b * 64];
+    red[strand][d] = x;
+    if (strand == 0) bk[d] = min(max(bucket[min(max(d - 32, -R), R) + R], 0), nb - 1);
+    __syncthreads();
+    if (strand == 0) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) x += red[k][d];
+        red[0][d] = x;                                         // (its own place)
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += 1024) {
+        float y = 0.f;
+        for (int i = 0; i < 64; ++i) y += bk[i] == b ? red[0][i] : 0.f;
+        if (bf16) ((__bf16*)dtable)[(long long)b * heads + h] = (__bf16)y;
+        else ((float*)dtable)[(long long)b * heads + h] = y;
+    }
+}
+
 // ---- joins of the parts: a wave per (row, head), a lane per d
 __global__ __launch_bounds__(256) void cfl_relpos_join_kernel(const float* __restrict__ po, const float* __restrict__ pm, int ns, int heads,
                                                               long long rows, long long last, const int* __restrict__ end, u16* o, long long ldo,
@@ -700,10 +892,11 @@ __global__ __launch_bounds__(256) void cfl_relpos_dtable_kernel(const float* __r
 }
 
 // Launch shape for `L` rows that waves own (32 each) against `K` rows that are passed over, for every (text, head).
-struct Shape { int nw, kt, blocks, ns; };
+struct Shape { int nw, kt, blocks, ns; bool small; };
 inline Shape rp_shape(long long BH, int L, int K) {
     Shape p;
     p.kt = K <= 32 ? 32 : 64;
+    p.small = L <= 32 && K <= 32;
     const long long waves = BH * cfl_cdiv(L, 32);
     // few waves against a long axis: split it, into parts of four tiles at least, until every SIMD has a wave
     long long ns = 1024 / waves;
@@ -754,6 +947,7 @@ size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb) 
     if (B < 1 || Lq < 0 || Lk < 1 || T < 0 || heads < 1 || nb < 1 || (Lq == 0 && T == 0)) return 0;
     const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk), k = rp_shape((long long)B * heads, Lk, Lq ? Lq : Lk);
     const long long rows = Lq ? (long long)B * Lq : T, krows = T ? T : (long long)B * Lk;
+    if (p.small) return (size_t)B * heads * 64 * 4;
     return cfl_align256((size_t)B * heads * p.blocks * p.ns * nb * 4) + rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
 }
 
@@ -773,7 +967,7 @@ int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, l
     hipStream_t stream = (hipStream_t)stream_;
     a.nqb = p.blocks; a.ns = p.ns;
     a.po = (float*)ws;
-    a.pm = (float*)((char*)ws + rp_part_bytes(p, heads, a.rows));
+    a.pm = p.ns > 1 ? (float*)((char*)ws + rp_part_bytes(p, heads, a.rows)) : nullptr;
     const size_t lds = (2 * (R + BPAD) + 1) * 4;
 #define RP_LDS(NW) lds
     RP_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel, p, RP_LDS, a);
@@ -781,7 +975,6 @@ int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, l
     if (p.ns > 1)
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_kernel, dim3((unsigned)((a.rows * heads + 3) / 4)), dim3(256), 0, stream, a.po, a.pm, p.ns, heads,
                    a.rows, a.rows, cu && !Lq ? cu + B : (const int*)nullptr, (u16*)o, ldo, lse);
-    if (cu && !Lq) CFL_LAUNCH(K_RELPOS_TAIL, cfl_relpos_tail_kernel, dim3(64), dim3(256), 0, stream, cu, B, T, (u16*)o, ldo, heads * 64);
     return 0;
 }
 
@@ -806,6 +999,13 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     const size_t bl = (2 * (R + BPAD) + 1) * 4;
     char* at = (char*)ws;
     a.diag = (float*)at;
+    if (p.small) {
+        a.ns = 1;
+        CFL_LAUNCH(K_RELPOS_BWD32, cfl_relpos_bwd32_kernel, dim3((unsigned)(B * heads)), dim3(64), 0, stream, a);
+        CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable32_kernel, dim3(heads), dim3(1024), 0, stream, a.diag, bucket, R, nb, heads, B, dtable,
+                   table_bf16);
+        return 0;
+    }
     at += cfl_align256((size_t)B * heads * p.blocks * p.ns * nb * 4);
     a.po = (float*)at;
     at += rp_part_bytes(p, heads, a.rows);
@@ -832,11 +1032,6 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
                    lddk);
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, g, dim3(256), 0, stream, a.pv, kp.ns, heads, a.krows, a.krows, kend, 1.f, (u16*)dv,
                    lddk);
-    }
-    if (cu) {
-        if (!Lq) CFL_LAUNCH(K_RELPOS_TAIL, cfl_relpos_tail_kernel, dim3(64), dim3(256), 0, stream, cu, B, T, (u16*)dq, lddq, heads * 64);
-        CFL_LAUNCH(K_RELPOS_TAIL, cfl_relpos_tail_kernel, dim3(64), dim3(256), 0, stream, cu, B, T, (u16*)dk, lddk, heads * 64);
-        CFL_LAUNCH(K_RELPOS_TAIL, cfl_relpos_tail_kernel, dim3(64), dim3(256), 0, stream, cu, B, T, (u16*)dv, lddk, heads * 64);
     }
     return 0;
 }

@@ -2514,7 +2514,8 @@ def relpos_attention(qkv, table, buckets, heads, key_mask=None, scale=None):
 
 def relpos_attention_varlen(qkv, cu_seqlens, max_len, table, buckets, heads, scale=None):
     """`relpos_attention` on PACKED tokens: qkv [T, 3H], text b = rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1] on the device;
-    a text may be empty); max_len: the longest text's length, a hint for the launch.  Rows behind the last text give zeros.  -> [T, H]."""
+    a text may be empty); max_len: the longest text's length -- a longer one is cut to its first max_len tokens.  Rows that belong to no
+    text, or to a cut one's rest, give zeros.  -> [T, H]."""
     qkv = _aligned16(_bf16c(qkv, 'qkv'))
     heads, max_len = int(heads), int(max_len)
     if qkv.dim() != 2 or qkv.numel() == 0 or max_len < 1:

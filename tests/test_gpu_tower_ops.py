@@ -266,34 +266,37 @@ def test_relpos_attention_scale_and_maps(dev):
 
 
 @pytest.mark.parametrize('lens,max_len,tail', [([1], 1, 0), ([5, 0, 32, 1, 17], 32, 0), ([5, 0, 32, 1, 17], 32, 3), ([40, 0, 7, 129, 64], 129, 0),
-                                               ([0, 70, 0], 70, 9), ([300, 20], 20, 0), ([33, 90, 128], 17, 1),
-                                               ([700, 0, 1300], 1300, 5)])
-def test_relpos_attention_varlen(dev, lens, max_len, tail):
-    """Packed texts, empty ones among them, rows behind the last one, texts longer than the hint."""
+                                               ([0, 70, 0], 70, 9), ([300, 20], 20, 0), ([33, 90, 128], 17, 1), ([9, 40, 3], 32, 2),
+                                               ([700, 0, 1300], 1300, 5), ([700, 0, 1300], 900, 5)])
+@pytest.mark.parametrize('lead', [0, 4])
+def test_relpos_attention_varlen(dev, lens, max_len, tail, lead):
+    """Packed texts, empty ones among them, rows before the first and behind the last one, texts longer than max_len (cut)."""
     from creamfl_amd import ops
     heads, H = 2, 128
-    T = sum(lens) + tail
+    T = lead + sum(lens) + tail
     t = attn_inputs(T, 1, T, heads)
-    cu = torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32)
+    cu = torch.tensor([lead] + [lead + int(v) for v in np.cumsum(lens)], dtype=torch.int32)
     qkv, table = t['qkv'][0].to(dev).requires_grad_(True), t['table'].to(dev).requires_grad_(True)
-    if tail:
-        with torch.no_grad():
-            qkv[-tail:] = float('nan')
+    idle = torch.ones(T, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        idle[int(cu[b]):int(cu[b]) + min(n, max_len)] = False
+    with torch.no_grad():
+        qkv[idle.to(dev)] = float('nan')
     o = ops.relpos_attention_varlen(qkv, cu.to(dev), max_len, table, t['buckets'].to(dev), heads)
     dqkv, dtable = torch.autograd.grad(o, [qkv, table], t['do'][0].to(dev))
     dt, et = torch.zeros(32, heads, dtype=torch.float64), torch.zeros(32, heads, dtype=torch.float64)
     for b, n in enumerate(lens):
+        n = min(n, max_len)
         if n == 0:
             continue
-        at = slice(int(cu[b]), int(cu[b + 1]))
+        at = slice(int(cu[b]), int(cu[b]) + n)
         w = text_oracle(t['qkv'][0, at], t['table'], t['buckets'], None, t['do'][0, at])
         within(o[at].view(n, heads, 64), w['o'], 'o')
         for i, name in enumerate(('dq', 'dk', 'dv')):
             within(dqkv[at, i * H:(i + 1) * H].reshape(n, heads, 64), w[name], name)
         dt, et = dt + w['dtable'][0], et + w['dtable'][1]
     within(dtable, (dt, et + 2.0 ** -8 * (dt.abs() + et) + 1e-30), 'dtable')
-    if tail:
-        assert bool((o[-tail:] == 0).all()) and bool((dqkv[-tail:] == 0).all())
+    assert bool((o.cpu()[idle] == 0).all()) and bool((dqkv.cpu()[idle] == 0).all())
 
 
 @pytest.mark.parametrize('lens,packed', [([1], False), ([24, 7, 0, 31], False), ([24, 7, 0, 31], True), ([200, 0, 65, 129], False), ([200, 0, 65, 129], True),
