@@ -28,7 +28,7 @@ typedef unsigned int u32;
 typedef unsigned long long u64;
 
 constexpr int TP = 72;                      // LDS row pitch in bf16 (144 bytes: 16-byte rows and both kinds of reads spread over the banks)
-constexpr int BPAD = 64;                    // the bias vector reaches this far beyond +-R: a tile that touches |d| <= R needs no clipping
+constexpr int BPAD = 96;                    // the bias vector reaches this far beyond +-R: a tile of 32 x 64 that touches |d| < R needs no clipping
 constexpr int MAXR = 512;                   // largest R (LDS)
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -133,26 +133,30 @@ __device__ __forceinline__ void load_rows(const u16* base, long long ld, int row
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) f[kk] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const f32x4*>(p + kk * 16));
 }
-// One tile of `ROWS` rows on its way from memory to LDS through registers: `load` early, `put` late.  Rows whose bit in `bits` is 0 (dropped
+// One tile of ROWS rows on its way from memory to LDS through registers: `load` early, `put` late.  Rows whose bit in `bits` is 0 (dropped
 // keys, rows past the end) become zeros: whatever stands there, infinities and NaN included, must not reach a product.
 template <int NT, int ROWS>
 struct Stage {
     static constexpr int N = ROWS * 8 / NT;
+    static constexpr u64 FULL = ROWS == 64 ? ~0ull : 0xffffffffull;
     f32x4 r[N];
-    __device__ __forceinline__ void load(const u16* base, long long ld, int r0, u64 bits) {
+    __device__ __forceinline__ void load(const u16* base, u32 ld, u64 bits) {      // base: the tile's first row, the same for every lane
+        const char* p = reinterpret_cast<const char*>(base);
+        u32 off = ((threadIdx.x >> 3) * ld + (threadIdx.x & 7) * 8) * 2;
+        if (bits == FULL) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = i * NT + threadIdx.x, row = c >> 3;
-            r[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if ((bits >> row) & 1) r[i] = *reinterpret_cast<const f32x4*>(base + (long long)(r0 + row) * ld + (c & 7) * 8);
+            for (int i = 0; i < N; ++i, off += NT / 8 * 2 * ld) r[i] = *reinterpret_cast<const f32x4*>(p + off);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i, off += NT / 8 * 2 * ld) {
+                r[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if ((bits >> (i * (NT / 8) + (threadIdx.x >> 3))) & 1) r[i] = *reinterpret_cast<const f32x4*>(p + off);
+            }
         }
     }
     __device__ __forceinline__ void put(u16* tile) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = i * NT + threadIdx.x;
-            *reinterpret_cast<f32x4*>(tile + (c >> 3) * TP + (c & 7) * 8) = r[i];
-        }
+        for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4*>(tile + (i * (NT / 8) + (threadIdx.x >> 3)) * TP + (threadIdx.x & 7) * 8) = r[i];
     }
 };
 __device__ __forceinline__ u64 low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
@@ -209,19 +213,57 @@ __device__ __forceinline__ void fill_bias(const RpArgs& a, int h, float* bl, int
         bl[d + mid] = t * LOG2E;
     }
 }
-// bias of a 32 x 32 block: distances key - query with d0 = (first key) - (first query); near = the block touches |d| < R
-struct BlockBias { bool near; float c; const float* p; };
-template <bool KEY_LANE>
-__device__ __forceinline__ BlockBias block_bias(const float* bl, int R, int d0, int lane) {
-    BlockBias x;
-    x.near = d0 - 31 < R && d0 + 31 > -R;
-    x.c = bl[(x.near ? 0 : d0 > 0 ? R : -R) + R + BPAD];
-    // lane = query: d = d0 + key - lane, key = acc_r; lane = key: d = d0 + lane - query, query = acc_r
-    x.p = bl + R + BPAD + (x.near ? d0 : 0) + (KEY_LANE ? (lane & 31) - 4 * (lane >> 5) : 4 * (lane >> 5) - (lane & 31));
-    return x;
+// A tile of 32 rows that a wave owns against `n` staged ones, d0 = (first key) - (first query): whether it touches |d| < R
+__device__ __forceinline__ bool tile_near(int R, int d0, int n, bool key_lane) {
+    return key_lane ? d0 - n + 1 < R && d0 + 31 > -R : d0 - 31 < R && d0 + n - 1 > -R;
+}
+// ... and, where it does not, the one bias it has
+__device__ __forceinline__ float far_bias(const float* bl, int R, int d0) { return bl[(d0 > 0 ? R : -R) + R + BPAD]; }
+// S = A B^T of U blocks of 32 staged rows against a wave's 32; the blocks' chains of four take turns
+template <int U>
+__device__ __forceinline__ void mma_rows(const u16* tile, const bf16x8 (&f)[4], f32x16 (&s)[U], int lane) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(tile, 32 * u, kk, lane), f[kk], s[u], 0, 0, 0);
+}
+// out^T += (tile's columns) (w packed to bf16), contraction over the 32 rows of block u
+__device__ __forceinline__ void mma_cols(const u16* tile, int u, const f32x16& w, f32x16 (&out)[2], int lane) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+        const bf16x8 f = pack_acc(w, kk);
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(tile, 32 * u + 16 * kk, dt, lane), f, out[dt], 0, 0, 0);
+    }
+}
+// dropped keys of block u: -inf (lane = query, registers = keys)
+__device__ __forceinline__ void drop_keys(f32x16& s, u64 bits, int u, int lane) {
+    const u32 in = (u32)(bits >> (32 * u)) >> (4 * (lane >> 5));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = (in >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : -INFINITY;
+}
+// a lane's 32 values of its row, rounded once
+__device__ __forceinline__ void store_row(const f32x16 (&o)[2], u16* row, int lane, float c) {
+    u16* op = row + 4 * (lane >> 5);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint2 v;
+            v.x = pack2(o[dt][4 * g] * c, o[dt][4 * g + 1] * c);
+            v.y = pack2(o[dt][4 * g + 2] * c, o[dt][4 * g + 3] * c);
+            *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
+        }
 }
 __device__ __forceinline__ void lds_add(float* p, float v) { __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
-__device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+// over the two lanes l, l ^ 32 (one VALU instruction instead of a trip through the LDS queue)
+__device__ __forceinline__ float half_max(float v) {
+    const u32 u = __float_as_uint(v);
+    const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // a lane's 32 values of its row in 32 bits: out [64]
 __device__ __forceinline__ void store_part(const f32x16 (&o)[2], float* out, int lane) {
@@ -241,7 +283,7 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     __shared__ __attribute__((aligned(16))) u16 Kt[NB][KT * TP], Vt[NB][KT * TP];
     __shared__ u64 tb[64];
     extern __shared__ float bl[];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = wave_id();
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
@@ -252,112 +294,108 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
-    {
-        const int q0 = qb * NW * 32 + w * 32;
-        bf16x8 qf[4];
-        load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, q0, t.lq, lane, qf);
-        f32x16 o[2];
-        zero16(o[0]); zero16(o[1]);
-        float m = -INFINITY, l = 0.f;
-        for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
-            keys.chunk(c0);
-            u64 left = keys.alive;
-            Stage<NT, KT> ks, vs;
-            int cur = next_tile(left);
-            if (cur < 0) continue;
-            u64 bits = keys.bits(cur);
-            ks.load(kp, a.ldk, c0 + cur * KT, bits);
-            vs.load(vp, a.ldk, c0 + cur * KT, bits);
-            int buf = 0;
-            __syncthreads();                                   // (the tiles' last readers, the bias vector)
-            ks.put(Kt[0]);
-            vs.put(Vt[0]);
-            while (true) {
-                const int k0 = c0 + cur * KT, nxt = next_tile(left);
-                u64 nbits = 0;
-                if (nxt >= 0) {
-                    nbits = keys.bits(nxt);
-                    ks.load(kp, a.ldk, c0 + nxt * KT, nbits);
-                    vs.load(vp, a.ldk, c0 + nxt * KT, nbits);
-                }
-                __syncthreads();
-                f32x16 s[U];
-                float top = -INFINITY;
+    const int q0 = (qb * NW + w) * 32;
+    bf16x8 qf[4];
+    load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, q0, t.lq, lane, qf);
+    f32x16 o[2];
+    zero16(o[0]); zero16(o[1]);
+    // l and o are relative to 2^m.  m follows the running maximum lazily: only when a score passes it by more than 8 are l and o brought
+    // to the new one (p then stays below 2^8; the division by l at the end cancels whatever m is)
+    float m = 0.f, l0 = 0.f, l1 = 0.f;
+    bool first = true;
+    for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
+        keys.chunk(c0);
+        u64 left = keys.alive;
+        Stage<NT, KT> ks, vs;
+        int cur = next_tile(left);
+        if (cur < 0) continue;
+        u64 bits = keys.bits(cur);
+        ks.load(kp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
+        vs.load(vp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
+        int buf = 0;
+        __syncthreads();                                       // (the tiles' last readers, the bias vector)
+        ks.put(Kt[0]);
+        vs.put(Vt[0]);
+        while (true) {
+            const int d0 = c0 + cur * KT - q0, nxt = next_tile(left);
+            u64 nbits = 0;
+            if (nxt >= 0) {
+                nbits = keys.bits(nxt);
+                ks.load(kp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
+                vs.load(vp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
+            }
+            __syncthreads();
+            f32x16 s[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    zero16(s[u]);
+            for (int u = 0; u < U; ++u) zero16(s[u]);
+            mma_rows<U>(Kt[buf], qf, s, lane);
+            if (tile_near(a.R, d0, KT, false)) {
+                const float* bp = bl + a.R + BPAD + d0 + 4 * (lane >> 5) - (lane & 31);
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Kt[buf], 32 * u, kk, lane), qf[kk], s[u], 0, 0, 0);
-                    const BlockBias bb = block_bias<false>(bl, a.R, k0 + 32 * u - q0, lane);
-                    if (bb.near) {
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, bb.p[(r & 3) + 8 * (r >> 2)]);
-                    } else {
+                    for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, bp[32 * u + (r & 3) + 8 * (r >> 2)] - m);
+            } else {
+                const float c = far_bias(bl, a.R, d0) - m;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, bb.c);
-                    }
-                    if (bits != Keys<NW, KT>::FULL) {
-                        const u32 mine = (u32)(bits >> (32 * u)) >> (4 * (lane >> 5));
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[u][r] = (mine >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[u][r] : -INFINITY;
-                    }
+                    for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, c);
+            }
+            if (bits != Keys<NW, KT>::FULL) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-                }
-                top = half_max(top);
-                if (__any(top > m)) {                          // a new maximum somewhere in the wave: bring what is summed to it
-                    const float mn = fmaxf(m, top), shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-                    l *= shrink;
+                for (int u = 0; u < U; ++u) drop_keys(s[u], bits, u, lane);
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+            top = half_max(top);
+            if (first || __any(top > 8.f)) {
+                const float by = first ? top : fmaxf(top, 0.f), shrink = __builtin_amdgcn_exp2f(-by);
+                if (!first) {
+                    l0 *= shrink; l1 *= shrink;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) { o[0][r] *= shrink; o[1][r] *= shrink; }
-                    m = mn;
                 }
+                first = false;
+                m += by;
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - m);
-                        l += s[u][r];
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < 2; ++kk) {
-                        const bf16x8 p = pack_acc(s[u], kk);
-#pragma unroll
-                        for (int dt = 0; dt < 2; ++dt)
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Vt[buf], 32 * u + 16 * kk, dt, lane), p, o[dt], 0, 0, 0);
-                    }
-                }
-                if (nxt < 0) break;
-                if (NB == 1) __syncthreads(); else buf ^= 1;
-                ks.put(Kt[buf]);
-                vs.put(Vt[buf]);
-                cur = nxt;
-                bits = nbits;
+                    for (int r = 0; r < 16; ++r) s[u][r] -= by;
             }
-        }
-        l += __shfl_xor(l, 32, 64);
-        const int row = q0 + (lane & 31);
-        if (a.ns > 1) {
-            if (row < t.lq) {
-                const long long at = ((long long)sp * a.heads + h) * a.rows + t.q0 + row;
-                store_part(o, a.po + at * 64, lane);
-                if (lane < 32) { a.pm[2 * at] = m; a.pm[2 * at + 1] = l; }
-            }
-        } else if (row < t.lq) {
-            const float inv = m == -INFINITY ? 0.f : 1.f / l;
-            u16* op = a.out + (t.q0 + row) * a.ldo + h * 64 + 4 * (lane >> 5);
 #pragma unroll
-            for (int dt = 0; dt < 2; ++dt)
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint2 v;
-                    v.x = pack2(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv);
-                    v.y = pack2(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
-                    *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
+                for (int r = 0; r < 16; r += 2) {
+                    s[u][r] = __builtin_amdgcn_exp2f(s[u][r]);
+                    s[u][r + 1] = __builtin_amdgcn_exp2f(s[u][r + 1]);
+                    l0 += s[u][r];
+                    l1 += s[u][r + 1];
                 }
-            if (a.lse && lane < 32) a.lse[h * a.rows + t.q0 + row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l);
+                mma_cols(Vt[buf], u, s[u], o, lane);
+            }
+            if (nxt < 0) break;
+            if (NB == 1) __syncthreads(); else buf ^= 1;
+            ks.put(Kt[buf]);
+            vs.put(Vt[buf]);
+            cur = nxt;
+            bits = nbits;
         }
+    }
+    float l = l0 + l1;
+    l += __shfl_xor(l, 32, 64);
+    const int row = q0 + (lane & 31);
+    if (row >= t.lq) return;
+    if (a.ns > 1) {
+        const long long at = ((long long)sp * a.heads + h) * a.rows + t.q0 + row;
+        store_part(o, a.po + at * 64, lane);
+        if (lane < 32) { a.pm[2 * at] = first ? -INFINITY : m; a.pm[2 * at + 1] = l; }
+    } else {
+        store_row(o, a.out + (t.q0 + row) * a.ldo + h * 64, lane, first ? 0.f : 1.f / l);
+        if (a.lse && lane < 32) a.lse[h * a.rows + t.q0 + row] = first ? INFINITY : m + __builtin_amdgcn_logf(l);
     }
 }
 
@@ -396,26 +434,15 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     const int nd = 2 * (a.R + BPAD) + 1, mid = a.R + BPAD;
     float* bl = dyn;
     float* dg = dyn + nd;                                      // [2 NW][nd]
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = wave_id();
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
     const Part part = part_of(sp, a.ns, t.lk, KT);
     float* out = a.diag + ((((long long)h * a.B + b) * a.nqb + qb) * a.ns + sp) * a.nb;
     if (a.cu && !a.Lq && qb == 0) clear_rest<NT>(a, t, b, h, sp, a.dq, nullptr, a.lddq);
-    if (qb * NW * 32 >= t.lq || t.lk == 0) {
+    if (qb * NW * 32 >= t.lq) {
         for (int i = threadIdx.x; i < a.nb; i += NT) out[i] = 0.f;
-        if (t.lk == 0 && a.Lq)                                 // queries of their own without a key: no gradient
-            for (int i = threadIdx.x; i < t.lq * 8; i += NT) {
-                const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-                if (a.ns == 1) {
-                    *reinterpret_cast<f32x4*>(a.dq + (t.q0 + (i >> 3)) * a.lddq + h * 64 + (i & 7) * 8) = z;
-                } else {
-                    float* p = a.po + (((long long)sp * a.heads + h) * a.rows + t.q0 + (i >> 3)) * 64 + (i & 7) * 8;
-                    *reinterpret_cast<f32x4*>(p) = z;
-                    *reinterpret_cast<f32x4*>(p + 4) = z;
-                }
-            }
         return;
     }
     const int dlo = max(-(t.lq | (NW * 32 - 1)), -mid), dhi = min(t.lk | (KT - 1), mid);      // (rows past the end are computed with as well)
@@ -423,126 +450,116 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     for (int c = 0; c < 2 * NW; ++c)
         for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) dg[c * nd + d + mid] = 0.f;
     float far_lo = 0.f, far_hi = 0.f;
-    float* mine = dg + (2 * w + (lane >> 5)) * nd;
-    Diag dg_{0.f, 0.f};
-    int dn = INT_MIN;                                          // the distance (first key - first query) that dg_.next belongs to
+    float* mine = dg + (2 * w + (lane >> 5)) * nd + mid - (lane & 31);
+    Diag sums{0.f, 0.f};
+    int dn = INT_MIN;                                          // the distance (first key - first query) that sums.next belongs to
     const auto flush = [&]() {
-        if (dn != INT_MIN) lds_add(mine + mid + dn - (lane & 31), dg_.next);
-        dg_.next = 0.f;
+        if (dn != INT_MIN) lds_add(mine + dn, sums.next);
+        sums.next = 0.f;
     };
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
+    const int q0 = (qb * NW + w) * 32, row = q0 + (lane & 31);
+    const bool live = row < t.lq;
+    bf16x8 qf[4], gf[4];
+    load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, q0, t.lq, lane, qf);
+    load_rows(a.dout + t.q0 * a.ldo + h * 64, a.ldo, q0, t.lq, lane, gf);
+    f32x16 negD;                                               // -D in every register: dp's sum starts from it
     {
-        const int q0 = qb * NW * 32 + w * 32;
-        const int row = q0 + (lane & 31);
-        const bool live = row < t.lq;
-        bf16x8 qf[4], gf[4];
-        load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, q0, t.lq, lane, qf);
-        load_rows(a.dout + t.q0 * a.ldo + h * 64, a.ldo, q0, t.lq, lane, gf);
+        bf16x8 of[4];
+        load_rows(a.o + t.q0 * a.ldo + h * 64, a.ldo, q0, t.lq, lane, of);
         float D = 0.f;
-        {
-            bf16x8 of[4];
-            load_rows(a.o + t.q0 * a.ldo + h * 64, a.ldo, q0, t.lq, lane, of);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
+        for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) D = fmaf((float)of[kk][j], (float)gf[kk][j], D);
-            D += __shfl_xor(D, 32, 64);
-        }
-        const float lse = live ? a.lse[h * a.rows + t.q0 + row] : INFINITY;      // (+inf: p = 0 in every row that does not count)
+            for (int j = 0; j < 8; ++j) D = fmaf((float)of[kk][j], (float)gf[kk][j], D);
+        D += __shfl_xor(D, 32, 64);
         if (live && lane < 32 && sp == 0) a.dsum[h * a.rows + t.q0 + row] = D;
-        f32x16 dq[2];
-        zero16(dq[0]); zero16(dq[1]);
-        for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
-            keys.chunk(c0);
-            u64 left = keys.alive;
-            Stage<NT, KT> ks, vs;
-            int cur = next_tile(left);
-            if (cur < 0) continue;
-            u64 bits = keys.bits(cur);
-            ks.load(kp, a.ldk, c0 + cur * KT, bits);
-            vs.load(vp, a.ldk, c0 + cur * KT, bits);
-            int buf = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) negD[r] = -D;
+    }
+    const float lse = live ? a.lse[h * a.rows + t.q0 + row] : INFINITY;      // (+inf: p = 0 in every row that does not count)
+    f32x16 dq[2];
+    zero16(dq[0]); zero16(dq[1]);
+    for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
+        keys.chunk(c0);
+        u64 left = keys.alive;
+        Stage<NT, KT> ks, vs;
+        int cur = next_tile(left);
+        if (cur < 0) continue;
+        u64 bits = keys.bits(cur);
+        ks.load(kp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
+        vs.load(vp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
+        int buf = 0;
+        __syncthreads();
+        ks.put(Kt[0]);
+        vs.put(Vt[0]);
+        while (true) {
+            const int d0 = c0 + cur * KT - q0, nxt = next_tile(left);
+            u64 nbits = 0;
+            if (nxt >= 0) {
+                nbits = keys.bits(nxt);
+                ks.load(kp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
+                vs.load(vp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
+            }
             __syncthreads();
-            ks.put(Kt[0]);
-            vs.put(Vt[0]);
-            while (true) {
-                const int k0 = c0 + cur * KT, nxt = next_tile(left);
-                u64 nbits = 0;
-                if (nxt >= 0) {
-                    nbits = keys.bits(nxt);
-                    ks.load(kp, a.ldk, c0 + nxt * KT, nbits);
-                    vs.load(vp, a.ldk, c0 + nxt * KT, nbits);
-                }
-                __syncthreads();
+            f32x16 s[U], dp[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) { zero16(s[u]); dp[u] = negD; }
+            mma_rows<U>(Kt[buf], qf, s, lane);
+            mma_rows<U>(Vt[buf], gf, dp, lane);
+            const bool near = tile_near(a.R, d0, KT, false);
+            if (near) {
+                const float* bp = bl + mid + d0 + 4 * (lane >> 5) - (lane & 31);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, bp[32 * u + (r & 3) + 8 * (r >> 2)] - lse);
+            } else {
+                const float c = far_bias(bl, a.R, d0) - lse;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, c);
+            }
+            if (bits != Keys<NW, KT>::FULL) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) drop_keys(s[u], bits, u, lane);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(s[u][r]) * dp[u][r];
+            if (near) {
+                if (d0 != dn) flush();                         // (not the tile after the last near one)
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    f32x16 s, dp;
-                    zero16(s); zero16(dp);
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Kt[buf], 32 * u, kk, lane), qf[kk], s, 0, 0, 0);
-                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Vt[buf], 32 * u, kk, lane), gf[kk], dp, 0, 0, 0);
-                    }
-                    const int d0 = k0 + 32 * u - q0;
-                    const BlockBias bb = block_bias<false>(bl, a.R, d0, lane);
-                    if (bb.near) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], a.scale2, bb.p[(r & 3) + 8 * (r >> 2)] - lse);
-                    } else {
-                        const float c = bb.c - lse;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], a.scale2, c);
-                    }
-                    if (bits != Keys<NW, KT>::FULL) {
-                        const u32 in = (u32)(bits >> (32 * u)) >> (4 * (lane >> 5));
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[r] = (in >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : -INFINITY;
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - D);
-                    if (bb.near) {
-                        if (d0 != dn) flush();                 // (not the block after the last near one)
-                        dg_.add(s, lane);
-                        lds_add(mine + mid + d0 - (lane & 31), dg_.here);
-                        dn = d0 + 32;
-                    } else {
-                        float x = 0.f;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) x += s[r];
-                        if (d0 > 0) far_hi += x; else far_lo += x;
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < 2; ++kk) {
-                        const bf16x8 p = pack_acc(s, kk);
-#pragma unroll
-                        for (int dt = 0; dt < 2; ++dt)
-                            dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Kt[buf], 32 * u + 16 * kk, dt, lane), p, dq[dt], 0, 0, 0);
-                    }
+                    sums.add(s[u], lane);
+                    lds_add(mine + d0 + 32 * u, sums.here);
                 }
-                if (nxt < 0) break;
-                if (NB == 1) __syncthreads(); else buf ^= 1;
-                ks.put(Kt[buf]);
-                vs.put(Vt[buf]);
-                cur = nxt;
-                bits = nbits;
+                dn = d0 + KT;
+            } else {
+                float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 2) { x0 += s[u][r]; x1 += s[u][r + 1]; }
+                if (d0 > 0) far_hi += x0 + x1; else far_lo += x0 + x1;
             }
-        }
-        if (a.ns > 1) {
-            if (live) store_part(dq, a.po + (((long long)sp * a.heads + h) * a.rows + t.q0 + row) * 64, lane);
-        } else if (live) {
-            u16* op = a.dq + (t.q0 + row) * a.lddq + h * 64 + 4 * (lane >> 5);
 #pragma unroll
-            for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint2 v;
-                    v.x = pack2(dq[dt][4 * g] * a.scale, dq[dt][4 * g + 1] * a.scale);
-                    v.y = pack2(dq[dt][4 * g + 2] * a.scale, dq[dt][4 * g + 3] * a.scale);
-                    *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
-                }
+            for (int u = 0; u < U; ++u) mma_cols(Kt[buf], u, s[u], dq, lane);
+            if (nxt < 0) break;
+            if (NB == 1) __syncthreads(); else buf ^= 1;
+            ks.put(Kt[buf]);
+            vs.put(Vt[buf]);
+            cur = nxt;
+            bits = nbits;
         }
+    }
+    if (live) {
+        if (a.ns > 1) store_part(dq, a.po + (((long long)sp * a.heads + h) * a.rows + t.q0 + row) * 64, lane);
+        else store_row(dq, a.dq + (t.q0 + row) * a.lddq + h * 64, lane, a.scale);
     }
     flush();
     // the workgroup's sums per distance ...
@@ -578,9 +595,10 @@ template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, int nkb) {
     constexpr int NT = NW * 64, U = KT / 32;
     __shared__ __attribute__((aligned(16))) u16 Qt[NB][KT * TP], Gt[NB][KT * TP];
-    __shared__ __attribute__((aligned(16))) float ls[NB][KT], ds[NB][KT];
+    __shared__ __attribute__((aligned(16))) float ls[NB][KT], ds[NB][KT];      // -log-sum and -D of the staged queries
     extern __shared__ float bl[];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    float* gone = bl + 2 * (a.R + BPAD) + 1;                   // [KT] of -inf: what a lane reads whose key does not take part
+    const int lane = threadIdx.x & 63, w = wave_id();
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, kb = id / a.ns % nkb, h = id / (a.ns * nkb) % a.heads, b = id / (a.ns * nkb * a.heads);
     const Text t = text_of(a, b);
@@ -588,107 +606,96 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     if (kb * NW * 32 >= t.lk) return;
     const Part part = part_of(sp, a.ns, t.lq, KT);
     fill_bias<NT>(a, h, bl, -(t.lq | (KT - 1)), t.lk | (NW * 32 - 1));
+    for (int i = threadIdx.x; i < KT; i += NT) gone[i] = -INFINITY;
     const unsigned char* mask = a.mask ? a.mask + (long long)b * a.Lk : nullptr;
     const u16* qp = a.q + t.q0 * a.ldq + h * 64;
     const u16* gp = a.dout + t.q0 * a.ldo + h * 64;
     const float* lp = a.lse + h * a.rows + t.q0;
     const float* dp_ = a.dsum + h * a.rows + t.q0;
-    {
-        const int k0 = kb * NW * 32 + w * 32;
-        const int key = k0 + (lane & 31);
-        const bool live = key < t.lk && (!mask || mask[key]);
-        f32x16 dk[2], dv[2];
-        zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]);
-        if (__syncthreads_or(live) && part.from < part.to) {   // (else no key of the workgroup takes part: zeros)
-            bf16x8 kf[4], vf[4];
-            load_rows(a.k + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, kf);
-            load_rows(a.v + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, vf);
-            Stage<NT, KT> qs, gs;
-            float lr = 0.f, dr = 0.f;
-            const auto fetch = [&](int q0) {
-                const u64 bits = low_bits(part.to - q0);
-                qs.load(qp, a.ldq, q0, bits);
-                gs.load(gp, a.ldo, q0, bits);
-                if (threadIdx.x < KT) {
-                    const bool in = q0 + (int)threadIdx.x < part.to;
-                    lr = in ? lp[q0 + threadIdx.x] : INFINITY;
-                    dr = in ? dp_[q0 + threadIdx.x] : 0.f;
-                }
-            };
-            const auto put = [&](int buf) {
-                qs.put(Qt[buf]);
-                gs.put(Gt[buf]);
-                if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
-            };
-            fetch(part.from);
-            int buf = 0;
-            put(0);
-            for (int q0 = part.from; ; ) {
-                const bool more = q0 + KT < part.to;
-                if (more) fetch(q0 + KT);
-                __syncthreads();
+    const int k0 = (kb * NW + w) * 32, key = k0 + (lane & 31);
+    const bool live = key < t.lk && (!mask || mask[key]);
+    f32x16 dk[2], dv[2];
+    zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]);
+    if (__syncthreads_or(live) && part.from < part.to) {       // (else no key of the workgroup takes part: zeros)
+        bf16x8 kf[4], vf[4];
+        load_rows(a.k + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, kf);
+        load_rows(a.v + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, vf);
+        if (!live) {
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    f32x16 s, dp;
-                    zero16(s); zero16(dp);
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Qt[buf], 32 * u, kk, lane), kf[kk], s, 0, 0, 0);
-                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(Gt[buf], 32 * u, kk, lane), vf[kk], dp, 0, 0, 0);
-                    }
-                    const BlockBias bb = block_bias<true>(bl, a.R, k0 - q0 - 32 * u, lane);
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 lse = *reinterpret_cast<const f32x4*>(&ls[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
-                        const f32x4 D = *reinterpret_cast<const f32x4*>(&ds[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = 4 * g + j;
-                            const float bias = bb.near ? bb.p[-(j + 8 * g)] : bb.c;
-                            const float p = live ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bias - lse[j])) : 0.f;
-                            s[r] = p;
-                            dp[r] = live ? p * (dp[r] - D[j]) : 0.f;
-                        }
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < 2; ++kk) {
-                        const bf16x8 p = pack_acc(s, kk), g = pack_acc(dp, kk);
-#pragma unroll
-                        for (int dt = 0; dt < 2; ++dt) {
-                            dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Gt[buf], 32 * u + 16 * kk, dt, lane), p, dv[dt], 0, 0, 0);
-                            dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(Qt[buf], 32 * u + 16 * kk, dt, lane), g, dk[dt], 0, 0, 0);
-                        }
-                    }
-                }
-                if (!more) break;
-                if (NB == 1) __syncthreads(); else buf ^= 1;
-                put(buf);
-                q0 += KT;
-            }
+            for (int kk = 0; kk < 4; ++kk) { kf[kk] = __builtin_bit_cast(bf16x8, z); vf[kk] = __builtin_bit_cast(bf16x8, z); }
         }
-        if (a.ns > 1) {
-            if (key < t.lk) {
-                if (!live) { zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]); }
-                const long long at = (((long long)sp * a.heads + h) * a.krows + t.k0 + key) * 64;
-                store_part(dk, a.po + at, lane);
-                store_part(dv, a.pv + at, lane);
+        Stage<NT, KT> qs, gs;
+        float lr = 0.f, dr = 0.f;
+        const auto fetch = [&](int q0) {
+            const u64 bits = low_bits(min(KT, part.to - q0));
+            qs.load(qp + (long long)q0 * a.ldq, (u32)a.ldq, bits);
+            gs.load(gp + (long long)q0 * a.ldo, (u32)a.ldo, bits);
+            if (threadIdx.x < KT) {
+                const bool in = q0 + (int)threadIdx.x < part.to;
+                lr = in ? -lp[q0 + threadIdx.x] : -INFINITY;
+                dr = in ? -dp_[q0 + threadIdx.x] : 0.f;
             }
-        } else if (key < t.lk) {
-            u16* kq = a.dk + (t.k0 + key) * a.lddk + h * 64 + 4 * (lane >> 5);
-            u16* vq = a.dv + (t.k0 + key) * a.lddk + h * 64 + 4 * (lane >> 5);
+        };
+        const auto put = [&](int buf) {
+            qs.put(Qt[buf]);
+            gs.put(Gt[buf]);
+            if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
+        };
+        fetch(part.from);
+        int buf = 0;
+        put(0);
+        for (int q0 = part.from; ; ) {
+            const bool more = q0 + KT < part.to;
+            if (more) fetch(q0 + KT);
+            __syncthreads();
+            const int d0 = k0 - q0;
+            const bool near = tile_near(a.R, d0, KT, true);
+            const float* bp = live ? bl + a.R + BPAD + (near ? d0 : 0) + (lane & 31) - 4 * (lane >> 5) : gone + KT - 1;
+            const float c = live ? far_bias(bl, a.R, near ? 0 : d0) : -INFINITY;
 #pragma unroll
-            for (int dt = 0; dt < 2; ++dt)
+            for (int u = 0; u < U; ++u) {
+                f32x16 s[1], dp[1], nl;
+                zero16(s[0]);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    uint2 v;
-                    v.x = live ? pack2(dk[dt][4 * g] * a.scale, dk[dt][4 * g + 1] * a.scale) : 0u;
-                    v.y = live ? pack2(dk[dt][4 * g + 2] * a.scale, dk[dt][4 * g + 3] * a.scale) : 0u;
-                    *reinterpret_cast<uint2*>(kq + 32 * dt + 8 * g) = v;
-                    v.x = live ? pack2(dv[dt][4 * g], dv[dt][4 * g + 1]) : 0u;
-                    v.y = live ? pack2(dv[dt][4 * g + 2], dv[dt][4 * g + 3]) : 0u;
-                    *reinterpret_cast<uint2*>(vq + 32 * dt + 8 * g) = v;
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(&ls[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(&ds[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { nl[4 * g + j] = x[j]; dp[0][4 * g + j] = y[j]; }
                 }
+                mma_rows<1>(Qt[buf] + 32 * u * TP, kf, s, lane);
+                mma_rows<1>(Gt[buf] + 32 * u * TP, vf, dp, lane);
+                if (near) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) nl[r] += bp[-(32 * u + (r & 3) + 8 * (r >> 2))];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) nl[r] += c;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], a.scale2, nl[r]));
+                    dp[0][r] *= s[0][r];
+                }
+                mma_cols(Gt[buf], u, s[0], dv, lane);
+                mma_cols(Qt[buf], u, dp[0], dk, lane);
+            }
+            if (!more) break;
+            if (NB == 1) __syncthreads(); else buf ^= 1;
+            put(buf);
+            q0 += KT;
         }
+    }
+    if (key >= t.lk) return;
+    if (!live) { zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]); }
+    if (a.ns > 1) {
+        const long long at = (((long long)sp * a.heads + h) * a.krows + t.k0 + key) * 64;
+        store_part(dk, a.po + at, lane);
+        store_part(dv, a.pv + at, lane);
+    } else {
+        store_row(dk, a.dk + (t.k0 + key) * a.lddk + h * 64, lane, a.scale);
+        store_row(dv, a.dv + (t.k0 + key) * a.lddk + h * 64, lane, 1.f);
     }
 }
 
@@ -895,16 +902,16 @@ __global__ __launch_bounds__(256) void cfl_relpos_dtable_kernel(const float* __r
 struct Shape { int nw, kt, blocks, ns; bool small; };
 inline Shape rp_shape(long long BH, int L, int K) {
     Shape p;
-    p.kt = K <= 32 ? 32 : 64;
     p.small = L <= 32 && K <= 32;
     const long long waves = BH * cfl_cdiv(L, 32);
-    // few waves against a long axis: split it, into parts of four tiles at least, until every SIMD has a wave
+    // few waves against a long axis: split it, into parts of 256 rows at least, until every SIMD has a wave
     long long ns = 1024 / waves;
     const int most = K / 256 < 16 ? K / 256 : 16;
     p.ns = (int)(ns > most ? most : ns);
     if (p.ns < 1) p.ns = 1;
     // four waves share what is staged, where that leaves a workgroup for every CU
     p.nw = L > 32 && BH * cfl_cdiv(L, 128) * p.ns >= 256 ? 4 : 1;
+    p.kt = p.nw == 1 || K <= 32 ? 32 : 64;
     p.blocks = cfl_cdiv(L, 32 * p.nw);
     return p;
 }
@@ -912,6 +919,8 @@ inline Shape rp_shape(long long BH, int L, int K) {
 inline int rp_check(const RpArgs& a, int head_dim) {
     if (!a.q || !a.k || !a.v || !a.table || !a.bucket || a.B < 1 || a.Lq < 0 || a.Lk < 1 || a.heads < 1 || a.nb < 1 || a.R < 0 ||
         (a.cu ? a.T < 1 || a.mask != nullptr : a.Lq < 1)) return CFL_EINVAL;
+    if (a.ldq >= 1 << 24 || a.ldk >= 1 << 24 || a.ldo >= 1 << 24) return CFL_ELIMIT;
+    if (a.ldq < 64 * a.heads || a.ldk < 64 * a.heads || a.ldo < 64 * a.heads) return CFL_EINVAL;
     if (a.ldq % 8 || a.ldk % 8 || a.ldo % 8 || (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15)) return CFL_EALIGN;
     const int L = a.Lq > a.Lk ? a.Lq : a.Lk;
     if (head_dim != 64 || a.R > MAXR || a.heads > 65535 || a.nb > 65535 ||
@@ -919,12 +928,12 @@ inline int rp_check(const RpArgs& a, int head_dim) {
     return 0;
 }
 
-#define RP_LAUNCH(ID, KERN, P, LDS1, ...)                                                                                              \
+#define RP_LAUNCH(ID, KERN, P, K, LDS1, ...)                                                                                           \
     do {                                                                                                                               \
         const dim3 grid_((unsigned)((long long)a.B * a.heads * (P).blocks * (P).ns));                                                  \
         if ((P).nw == 4 && (P).kt == 64) { CFL_LAUNCH(ID, (KERN<4, 64, 2>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }         \
         else if ((P).nw == 4) { CFL_LAUNCH(ID, (KERN<4, 32, 1>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }                    \
-        else if ((P).kt == 64) { CFL_LAUNCH(ID, (KERN<1, 64, 1>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                    \
+        else if ((K) > 32) { CFL_LAUNCH(ID, (KERN<1, 32, 2>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                        \
         else { CFL_LAUNCH(ID, (KERN<1, 32, 1>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                                      \
     } while (0)
 
@@ -970,7 +979,7 @@ int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, l
     a.pm = p.ns > 1 ? (float*)((char*)ws + rp_part_bytes(p, heads, a.rows)) : nullptr;
     const size_t lds = (2 * (R + BPAD) + 1) * 4;
 #define RP_LDS(NW) lds
-    RP_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel, p, RP_LDS, a);
+    RP_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel, p, Lk, RP_LDS, a);
 #undef RP_LDS
     if (p.ns > 1)
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_kernel, dim3((unsigned)((a.rows * heads + 3) / 4)), dim3(256), 0, stream, a.po, a.pm, p.ns, heads,
@@ -1011,7 +1020,7 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     at += rp_part_bytes(p, heads, a.rows);
     a.nqb = p.blocks; a.ns = p.ns;
 #define RP_LDS(NW) bl * (1 + 2 * (NW))
-    RP_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel, p, RP_LDS, a);
+    RP_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel, p, Lk, RP_LDS, a);
 #undef RP_LDS
     const int* qend = cu && !Lq ? cu + B : nullptr;
     if (p.ns > 1)
@@ -1022,8 +1031,8 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     a.po = (float*)at;
     a.pv = (float*)(at + rp_part_bytes(kp, heads, a.krows));
     a.ns = kp.ns;
-#define RP_LDS(NW) bl
-    RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, RP_LDS, a, kp.blocks);
+#define RP_LDS(NW) bl + 64 * 4
+    RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, L, RP_LDS, a, kp.blocks);
 #undef RP_LDS
     if (kp.ns > 1) {
         const dim3 g((unsigned)((a.krows * heads + 3) / 4));

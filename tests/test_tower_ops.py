@@ -123,7 +123,8 @@ def test_entries_refuse_bad_arguments():
                dict(o=None), dict(cu=P, t=0), dict(cu=P, t=8, mask=P)):
         assert fwd(**kw) == EINVAL, kw
     assert fwd(ldq=100) == EALIGN and fwd(q=P + 2) == EALIGN and fwd(ldo=66) == EALIGN and fwd(o=P + 8) == EALIGN
-    assert fwd(hd=32) == ELIMIT and fwd(r=513) == ELIMIT and fwd(b=1 << 30, heads=64) == ELIMIT
+    assert fwd(hd=32) == ELIMIT and fwd(r=513) == ELIMIT and fwd(b=1 << 30) == ELIMIT and fwd(ldq=1 << 24) == ELIMIT
+    assert fwd(heads=4) == EINVAL                          # (rows shorter than the heads)
     assert lib.cfl_relpos_bwd(P, 192, P, P, 192, None, None, 2, 4, 4, 0, 1, 64, 0.125, P, 1, 4, P, 2, P, P, 64, P, None, P, 192, P, P, 192, P, P,
                               None) == EINVAL
     assert lib.cfl_relpos_bwd_ws_bytes(0, 4, 4, 0, 1, 4) == 0 and lib.cfl_relpos_bwd_ws_bytes(2, 0, 4, 8, 1, 4) > 0
