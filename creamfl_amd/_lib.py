@@ -62,7 +62,7 @@ SIGNATURES = {
     'cfl_gn_fwd': (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, _P, _P, _P, _P]),
     'cfl_gn_bwd': (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P]),
     'cfl_relpos_fwd_ws_bytes': (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
-    'cfl_relpos_bwd_ws_bytes': (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    'cfl_relpos_bwd_ws_bytes': (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     'cfl_relpos_fwd': (c_int, [_P, c_longlong, _P, _P, c_longlong, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_int,
                                c_int, _P, c_int, _P, c_longlong, _P, _P, _P]),
     'cfl_relpos_bwd': (c_int, [_P, c_longlong, _P, _P, c_longlong, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_int,

@@ -47,11 +47,14 @@ struct RpArgs {
     const int* bucket;                      // [2 R + 1]
     float* lse;                             // [heads][rows]: log2-sum of a row's scores (+inf: no key)
     float* dsum;                            // [heads][rows]: D
-    float* diag;                            // [heads][B nqb][nb]: the bias gradient's parts
+    float* diag;                            // [heads][slots][nd]: the bias gradient's parts per distance
     int nqb;                                // query blocks of the longest text
     int ns;                                 // parts a text's keys (forward, dQ) or queries (dK, dV) are split into
     float *po, *pm;                         // the parts' results: [ns][heads][rows][64], and of the forward [ns][heads][rows][2] (maximum, sum)
     float* pv;                              // dV's
+    float* share;                           // [heads][nshare][nb]: the bias gradient by blocks of distances
+    int nshare;
+    void* dtable;
     long long rows, krows;                  // query rows, key rows in all
 };
 
@@ -202,15 +205,23 @@ __device__ __forceinline__ Part part_of(int sp, int ns, int n, int tile) {
     return Part{min(sp * per, n), min((sp + 1) * per, n)};
 }
 
-// head h's bias over the distances lo .. hi, in units of log2: bl[d + R + BPAD]
+// head h's bias over the distances lo .. hi, in units of log2: bl[d + R + BPAD].  Two dependent loads a distance; those of four distances
+// travel together.
 template <int NT>
 __device__ __forceinline__ void fill_bias(const RpArgs& a, int h, float* bl, int lo, int hi) {
     const int mid = a.R + BPAD, first = max(lo, -mid), last = min(hi, mid);
-    for (int d = first + (int)threadIdx.x; d <= last; d += NT) {
-        const int b = min(max(a.bucket[min(max(d, -a.R), a.R) + a.R], 0), a.nb - 1);
-        const float t = a.table_bf16 ? __uint_as_float((u32)((const u16*)a.table)[(long long)b * a.heads + h] << 16)
-                                     : ((const float*)a.table)[(long long)b * a.heads + h];
-        bl[d + mid] = t * LOG2E;
+    for (int d = first + (int)threadIdx.x; d <= last; d += 4 * NT) {
+        int bk[4];
+        float t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bk[i] = a.bucket[min(max(min(d + i * NT, last), -a.R), a.R) + a.R];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long at = (long long)min(max(bk[i], 0), a.nb - 1) * a.heads + h;
+            t[i] = a.table_bf16 ? __uint_as_float((u32)((const u16*)a.table)[at] << 16) : ((const float*)a.table)[at];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (d + i * NT <= last) bl[d + i * NT + mid] = t[i] * LOG2E;
     }
 }
 // A tile of 32 rows that a wave owns against `n` staged ones, d0 = (first key) - (first query): whether it touches |d| < R
@@ -423,8 +434,8 @@ struct Diag {
 // The bias gradient of a distance is the sum of ds along a diagonal.  A lane's 16 values of a near block lie on 16 diagonals: each is moved
 // to the lane of its diagonal (key - query mod 32; `Diag`) and summed in registers, with one LDS addition per block into words of the
 // wave's own (the addresses of one instruction are distinct and a wave's LDS operations stay in order, so the sum's order is fixed;
-// adding all 16 in LDS took 340 us instead of @DQ@ at 32 texts of 512 tokens, 12 heads).  Far blocks are summed in registers.  At the end the
-// workgroup's sums per distance are gathered by bucket: part [heads][slots][nb], one slot per (text, query block, part).
+// adding all 16 in LDS took 340 us instead of @DQ@ at 32 texts of 512 tokens, 12 heads).  Far tiles are summed in registers.  At the end the
+// workgroup's sums per distance go to part [heads][slots][nd], one slot per (text, query block, part), place d + R + BPAD.
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     constexpr int NT = NW * 64, U = KT / 32;
@@ -439,10 +450,10 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
     const Part part = part_of(sp, a.ns, t.lk, KT);
-    float* out = a.diag + ((((long long)h * a.B + b) * a.nqb + qb) * a.ns + sp) * a.nb;
+    float* out = a.diag + ((((long long)h * a.B + b) * a.nqb + qb) * a.ns + sp) * nd;
     if (a.cu && !a.Lq && qb == 0) clear_rest<NT>(a, t, b, h, sp, a.dq, nullptr, a.lddq);
     if (qb * NW * 32 >= t.lq) {
-        for (int i = threadIdx.x; i < a.nb; i += NT) out[i] = 0.f;
+        for (int i = threadIdx.x; i < nd; i += NT) out[i] = 0.f;
         return;
     }
     const int dlo = max(-(t.lq | (NW * 32 - 1)), -mid), dhi = min(t.lk | (KT - 1), mid);      // (rows past the end are computed with as well)
@@ -562,33 +573,25 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
         else store_row(dq, a.dq + (t.q0 + row) * a.lddq + h * 64, lane, a.scale);
     }
     flush();
-    // the workgroup's sums per distance ...
+    // the workgroup's sums per distance
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
-    if (lane == 0) {                                           // (far blocks exist only where the range reaches beyond +-R)
+    if (lane == 0) {                                           // (far tiles exist only where the range reaches beyond +-R)
         if (dlo <= -a.R) dg[2 * w * nd + mid - a.R] += far_lo;
         if (dhi >= a.R) dg[2 * w * nd + mid + a.R] += far_hi;
     }
     __syncthreads();
-    for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) {
+    for (int i = threadIdx.x; i < nd; i += NT) {
         float x = 0.f;
+        if (i >= dlo + mid && i <= dhi + mid) {
 #pragma unroll
-        for (int c = 0; c < 2 * NW; ++c) x += dg[c * nd + d + mid];
-        dg[d + mid] = x;                                       // (read above by this thread alone)
-        bl[d + mid] = __int_as_float(min(max(a.bucket[min(max(d, -a.R), a.R) + a.R], 0), a.nb - 1));      // the bias is not read any more
-    }
-    __syncthreads();
-    // ... and per bucket: L lanes each
-    int L = 1;
-    while (L < 64 && 2 * L * a.nb <= NT) L *= 2;
-    for (int b0 = 0; b0 < a.nb; b0 += NT / L) {
-        const int bk = b0 + threadIdx.x / L;
-        float x = 0.f;
-        for (int d = dlo + (int)(threadIdx.x % L); d <= dhi; d += L) x += __float_as_int(bl[d + mid]) == bk ? dg[d + mid] : 0.f;
-        for (int o = L >> 1; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-        if (bk < a.nb && threadIdx.x % L == 0) out[bk] = x;
+            for (int c = 0; c < 2 * NW; ++c) x += dg[c * nd + i];
+        }
+        out[i] = x;
     }
 }
+
+__device__ __forceinline__ void put_dtable(void* dtable, int bf16, long long at, float v);
 
 // ---- backward, keys: dK and dV.  A wave owns 32 keys; the staged rows are queries.
 template <int NW, int KT, int NB>
@@ -603,6 +606,12 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     const int sp = id % a.ns, kb = id / a.ns % nkb, h = id / (a.ns * nkb) % a.heads, b = id / (a.ns * nkb * a.heads);
     const Text t = text_of(a, b);
     if (a.cu && kb == 0) clear_rest<NT>(a, t, b, h, sp, a.dk, a.dv, a.lddk);
+    if (b == 0 && kb == 0 && sp == 0)                          // the head's bias gradient: the last step of cfl_relpos_dtable_kernel
+        for (int i = threadIdx.x; i < a.nb; i += NT) {
+            float y = 0.f;
+            for (int k = 0; k < a.nshare; ++k) y += a.share[((long long)h * a.nshare + k) * a.nb + i];
+            put_dtable(a.dtable, a.table_bf16, (long long)i * a.heads + h, y);
+        }
     if (kb * NW * 32 >= t.lk) return;
     const Part part = part_of(sp, a.ns, t.lq, KT);
     fill_bias<NT>(a, h, bl, -(t.lq | (KT - 1)), t.lk | (NW * 32 - 1));
@@ -709,6 +718,7 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     __shared__ __attribute__((aligned(16))) float ls[32], Ds[32];
     const int lane = threadIdx.x, x = lane & 31, half = lane >> 5;
     const int id = xcd_remap(blockIdx.x, gridDim.x), h = id % a.heads, b = id / a.heads;
+    const int bk = a.bucket[min(max(lane - 31, -a.R), a.R) + a.R];      // (first: a second load hangs on it)
     const Text t = text_of(a, b);
     float* part = a.diag + ((long long)h * a.B + b) * 64;
     if (a.cu) {
@@ -720,6 +730,8 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
         zero_rows<64>(a.dq, a.lddq, h, t.q0, t.q0 + t.lq);
         return;
     }
+    const long long ti = (long long)min(max(bk, 0), a.nb - 1) * a.heads + h;
+    const float bias = a.table_bf16 ? __uint_as_float((u32)((const u16*)a.table)[ti] << 16) : ((const float*)a.table)[ti];
     const u32 bits = (u32)__ballot(lane < t.lk && (!a.mask || a.mask[(long long)b * a.Lk + min(lane, t.lk - 1)] != 0));
     const bool keep = (bits >> x) & 1;
     bf16x8 kf[4], vf[4], qf[4], gf[4];
@@ -728,12 +740,7 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, 0, t.lq, lane, qf);
     load_rows(a.dout + t.q0 * a.ldo + h * 64, a.ldo, 0, t.lq, lane, gf);
     const float lse = x < t.lq ? a.lse[h * a.rows + t.q0 + x] : INFINITY;
-    {
-        const int d = min(max(lane - 31, -a.R), a.R);
-        const int bk = min(max(a.bucket[d + a.R], 0), a.nb - 1);
-        bl[lane] = LOG2E * (a.table_bf16 ? __uint_as_float((u32)((const u16*)a.table)[(long long)bk * a.heads + h] << 16)
-                                         : ((const float*)a.table)[(long long)bk * a.heads + h]);
-    }
+    bl[lane] = LOG2E * bias;
     const f32x4 z4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
@@ -815,32 +822,6 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     apply(Qt, dp);
     store(a.dk + t.k0 * a.lddk + h * 64, a.lddk, x < t.lk, keep, a.scale);
 }
-// ... and its bias gradient: the texts' sums per distance, then the buckets.  grid = heads
-__global__ __launch_bounds__(1024) void cfl_relpos_dtable32_kernel(const float* __restrict__ part, const int* __restrict__ bucket, int R, int nb,
-                                                                   int heads, int B, void* dtable, int bf16) {
-    __shared__ float red[16][64];
-    __shared__ int bk[64];
-    const int h = blockIdx.x, d = threadIdx.x & 63, strand = threadIdx.x >> 6;
-    const float* p = part + (long long)h * B * 64 + d;
-    float x = 0.f;
-    for (int b = strand; b < B; b += 16) x += p[(long long)b * 64];
-    red[strand][d] = x;
-    if (strand == 0) bk[d] = min(max(bucket[min(max(d - 32, -R), R) + R], 0), nb - 1);
-    __syncthreads();
-    if (strand == 0) {
-#pragma unroll
-        for (int k = 1; k < 16; ++k) x += red[k][d];
-        red[0][d] = x;                                         // (its own place)
-    }
-    __syncthreads();
-    for (int b = threadIdx.x; b < nb; b += 1024) {
-        float y = 0.f;
-        for (int i = 0; i < 64; ++i) y += bk[i] == b ? red[0][i] : 0.f;
-        if (bf16) ((__bf16*)dtable)[(long long)b * heads + h] = (__bf16)y;
-        else ((float*)dtable)[(long long)b * heads + h] = y;
-    }
-}
-
 // ---- joins of the parts: a wave per (row, head), a lane per d
 __global__ __launch_bounds__(256) void cfl_relpos_join_kernel(const float* __restrict__ po, const float* __restrict__ pm, int ns, int heads,
                                                               long long rows, long long last, const int* __restrict__ end, u16* o, long long ldo,
@@ -872,29 +853,52 @@ __global__ __launch_bounds__(256) void cfl_relpos_join_sum_kernel(const float* _
     reinterpret_cast<__bf16*>(o)[row * ldo + h * 64 + lane] = (__bf16)(x * scale);
 }
 
-// ---- dtable[bucket][h]: the slots' sums, in a fixed order.  grid = (ceil(nb / 32), heads): 32 buckets x 8 strands of slots
-__global__ __launch_bounds__(256) void cfl_relpos_dtable_kernel(const float* __restrict__ part, int nb, int heads, long long slots, void* dtable,
-                                                                int bf16) {
-    __shared__ float red[8][32];
-    const int h = blockIdx.y, b = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
-    float x = 0.f;
-    if (b < nb) {
-        const float* p = part + (long long)h * slots * nb + b;
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
+// ---- the bias gradient from part [heads][slots][nd] (place i: distance i - mid): the slots' sums of 64 distances, then of these every
+// bucket's share, in a fixed order.  grid = (heads, ceil(nd / 64)), 64 distances x 16 strands of slots.  One block of distances: that is the
+// table's gradient; more: share [heads][blocks][nb], which the dK / dV kernel's first workgroups add up.
+__device__ __forceinline__ void put_dtable(void* dtable, int bf16, long long at, float v) {
+    if (bf16) ((__bf16*)dtable)[at] = (__bf16)v;
+    else ((float*)dtable)[at] = v;
+}
+__global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __restrict__ part, int nd, int mid, long long slots,
+                                                                 const int* __restrict__ bucket, int R, int nb, int heads, float* share,
+                                                                 void* dtable, int bf16) {
+    __shared__ float red[16][64];
+    __shared__ int bk[64];
+    const int h = blockIdx.x, lane = threadIdx.x & 63, strand = threadIdx.x >> 6, i = blockIdx.y * 64 + lane;
+    if (strand == 0) bk[lane] = i < nd ? min(max(bucket[min(max(i - mid, -R), R) + R], 0), nb - 1) : -1;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (i < nd) {
+        const float* p = part + (long long)h * slots * nd + i;
         long long s = strand;
-        for (; s + 24 < slots; s += 32)
+        for (; s + 112 < slots; s += 128) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] += p[(s + 8 * k) * nb];
-        for (; s < slots; s += 8) y[0] += p[s * nb];
-        x = (y[0] + y[1]) + (y[2] + y[3]);
+            for (int k = 0; k < 8; ++k) x[k] += p[(s + 16 * k) * nd];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (s + 16 * k < slots) x[k] += p[(s + 16 * k) * nd];
     }
-    red[strand][threadIdx.x & 31] = x;
+    red[strand][lane] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     __syncthreads();
-    if (strand == 0 && b < nb) {
+    if (strand == 0) {
+        float y = 0.f;
 #pragma unroll
-        for (int k = 1; k < 8; ++k) x += red[k][threadIdx.x];
-        if (bf16) ((__bf16*)dtable)[b * heads + h] = (__bf16)x;
-        else ((float*)dtable)[b * heads + h] = x;
+        for (int k = 0; k < 16; ++k) y += red[k][lane];
+        red[0][lane] = y;                                      // (its own place)
+    }
+    __syncthreads();
+    int L = 16;                                                // lanes a bucket
+    while (L > 1 && (long long)nb * L > 1024) L >>= 1;
+    for (int b0 = 0; b0 < nb; b0 += 1024 / L) {
+        const int b = b0 + threadIdx.x / L;
+        float y = 0.f;
+        for (int k = threadIdx.x & (L - 1); k < 64; k += L) y += bk[k] == b ? red[0][k] : 0.f;
+        for (int o = L >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
+        if (b < nb && (threadIdx.x & (L - 1)) == 0) {
+            if (share) share[((long long)h * gridDim.y + blockIdx.y) * nb + b] = y;
+            else put_dtable(dtable, bf16, (long long)b * heads + h, y);
+        }
     }
 }
 
@@ -937,6 +941,7 @@ inline int rp_check(const RpArgs& a, int head_dim) {
         else { CFL_LAUNCH(ID, (KERN<1, 32, 1>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                                      \
     } while (0)
 
+inline int rp_nd(int R) { return 2 * (R + BPAD) + 1; }
 inline size_t rp_part_bytes(const Shape& p, int heads, long long rows) {
     return p.ns > 1 ? cfl_align256((size_t)p.ns * heads * rows * 64 * 4) : 0;
 }
@@ -952,12 +957,13 @@ size_t cfl_relpos_fwd_ws_bytes(int B, int Lq, int Lk, int T, int heads) {
     return p.ns > 1 ? rp_part_bytes(p, heads, rows) + (size_t)p.ns * heads * rows * 2 * 4 : 0;
 }
 
-size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb) {
-    if (B < 1 || Lq < 0 || Lk < 1 || T < 0 || heads < 1 || nb < 1 || (Lq == 0 && T == 0)) return 0;
+size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb, int R) {
+    if (B < 1 || Lq < 0 || Lk < 1 || T < 0 || heads < 1 || nb < 1 || R < 0 || R > MAXR || (Lq == 0 && T == 0)) return 0;
     const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk), k = rp_shape((long long)B * heads, Lk, Lq ? Lq : Lk);
     const long long rows = Lq ? (long long)B * Lq : T, krows = T ? T : (long long)B * Lk;
     if (p.small) return (size_t)B * heads * 64 * 4;
-    return cfl_align256((size_t)B * heads * p.blocks * p.ns * nb * 4) + rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
+    return cfl_align256((size_t)B * heads * p.blocks * p.ns * rp_nd(R) * 4) + cfl_align256((size_t)heads * cfl_cdiv(rp_nd(R), 64) * nb * 4) +
+           rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
 }
 
 int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
@@ -977,7 +983,7 @@ int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, l
     a.nqb = p.blocks; a.ns = p.ns;
     a.po = (float*)ws;
     a.pm = p.ns > 1 ? (float*)((char*)ws + rp_part_bytes(p, heads, a.rows)) : nullptr;
-    const size_t lds = (2 * (R + BPAD) + 1) * 4;
+    const size_t lds = (size_t)rp_nd(R) * 4;
 #define RP_LDS(NW) lds
     RP_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel, p, Lk, RP_LDS, a);
 #undef RP_LDS
@@ -1005,17 +1011,17 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     hipStream_t stream = (hipStream_t)stream_;
     const int L = Lq ? Lq : Lk;
     const Shape p = rp_shape((long long)B * heads, L, Lk), kp = rp_shape((long long)B * heads, Lk, L);
-    const size_t bl = (2 * (R + BPAD) + 1) * 4;
+    const size_t bl = (size_t)rp_nd(R) * 4;
     char* at = (char*)ws;
     a.diag = (float*)at;
     if (p.small) {
         a.ns = 1;
         CFL_LAUNCH(K_RELPOS_BWD32, cfl_relpos_bwd32_kernel, dim3((unsigned)(B * heads)), dim3(64), 0, stream, a);
-        CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable32_kernel, dim3(heads), dim3(1024), 0, stream, a.diag, bucket, R, nb, heads, B, dtable,
-                   table_bf16);
+        CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, 1), dim3(1024), 0, stream, a.diag, 64, 32, (long long)B, bucket, R, nb,
+                   heads, (float*)nullptr, dtable, table_bf16);
         return 0;
     }
-    at += cfl_align256((size_t)B * heads * p.blocks * p.ns * nb * 4);
+    at += cfl_align256((size_t)B * heads * p.blocks * p.ns * rp_nd(R) * 4);
     a.po = (float*)at;
     at += rp_part_bytes(p, heads, a.rows);
     a.nqb = p.blocks; a.ns = p.ns;
@@ -1026,8 +1032,13 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     if (p.ns > 1)
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, dim3((unsigned)((a.rows * heads + 3) / 4)), dim3(256), 0, stream, a.po, p.ns, heads,
                    a.rows, a.rows, qend, scale, (u16*)dq, lddq);
-    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(cfl_cdiv(nb, 32), heads), dim3(256), 0, stream, a.diag, nb, heads,
-               (long long)B * p.blocks * p.ns, dtable, table_bf16);
+    const int nd = rp_nd(R);
+    a.nshare = cfl_cdiv(nd, 64);
+    a.share = (float*)at;
+    a.dtable = dtable;
+    at += cfl_align256((size_t)heads * a.nshare * nb * 4);
+    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, a.nshare), dim3(1024), 0, stream, a.diag, nd, R + BPAD,
+               (long long)B * p.blocks * p.ns, bucket, R, nb, heads, a.share, dtable, table_bf16);
     a.po = (float*)at;
     a.pv = (float*)(at + rp_part_bytes(kp, heads, a.krows));
     a.ns = kp.ns;

@@ -2459,7 +2459,7 @@ class _RelposFn(torch.autograd.Function):
         dq = torch.empty_like(q)
         dkv = None if kv is None else torch.empty_like(kv)
         dtable = torch.empty_like(table)
-        ws = _ws(_lib.load().cfl_relpos_bwd_ws_bytes(B, Lq, Lk, T, heads, nb), q.device)
+        ws = _ws(_lib.load().cfl_relpos_bwd_ws_bytes(B, Lq, Lk, T, heads, nb, buckets.numel() // 2), q.device)
         kb, ldk = (q.data_ptr() + 2 * H, 3 * H) if kv is None else (kv.data_ptr(), 2 * H)
         gb = dq.data_ptr() + 2 * H if kv is None else dkv.data_ptr()
         _launch('cfl_relpos_bwd', q, q.data_ptr(), q.shape[1], kb, kb + 2 * H, ldk, _ptr(mask), _ptr(cu), B, Lq, Lk, T, heads, 64, scale,

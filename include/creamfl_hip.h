@@ -226,7 +226,7 @@ int cfl_gn_bwd(const void* dy, const void* dy2, const void* x, const void* res, 
  * All ld % 8 == 0, 16-byte aligned bases.
  * ws: cfl_relpos_fwd_ws_bytes (0: may be NULL) / cfl_relpos_bwd_ws_bytes (T = 0: padded). */
 size_t cfl_relpos_fwd_ws_bytes(int B, int Lq, int Lk, int T, int heads);
-size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb);
+size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb, int R);
 int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
                    int B, int Lq, int Lk, int T, int heads, int head_dim, float scale, const void* table, int table_bf16, int nb,
                    const int* bucket, int R, void* o, long long ldo, float* lse, void* ws, void* stream);

@@ -127,7 +127,7 @@ def test_entries_refuse_bad_arguments():
     assert fwd(heads=4) == EINVAL                          # (rows shorter than the heads)
     assert lib.cfl_relpos_bwd(P, 192, P, P, 192, None, None, 2, 4, 4, 0, 1, 64, 0.125, P, 1, 4, P, 2, P, P, 64, P, None, P, 192, P, P, 192, P, P,
                               None) == EINVAL
-    assert lib.cfl_relpos_bwd_ws_bytes(0, 4, 4, 0, 1, 4) == 0 and lib.cfl_relpos_bwd_ws_bytes(2, 0, 4, 8, 1, 4) > 0
+    assert lib.cfl_relpos_bwd_ws_bytes(0, 4, 4, 0, 1, 4, 2) == 0 and lib.cfl_relpos_bwd_ws_bytes(2, 0, 4, 8, 1, 4, 2) > 0
     assert lib.cfl_relpos_fwd_ws_bytes(1, 1, 4096, 0, 1) > 0 and lib.cfl_relpos_fwd_ws_bytes(64, 64, 64, 0, 12) == 0
     assert fwd(b=1, lq=1, lk=4096) == EINVAL               # (a split forward without its workspace)
 
