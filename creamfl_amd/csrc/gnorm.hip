@@ -52,10 +52,11 @@ __device__ __forceinline__ float gn_act_grad(int act, float z) {
 // 8 channels rounded once (hardware conversion, two values an instruction)
 __device__ __forceinline__ void gn_store(U4* p, const float (&f)[8]) {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
-    v8 o;
+    typedef float w8 __attribute__((ext_vector_type(8)));
+    w8 o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = (__bf16)f[j];
-    *reinterpret_cast<v8*>(p) = o;
+    for (int j = 0; j < 8; ++j) o[j] = f[j];
+    *reinterpret_cast<v8*>(p) = __builtin_convertvector(o, v8);
 }
 __device__ __forceinline__ void gn_store(F8* p, const float (&f)[8]) { *p = pack8g<F8>(f); }
 // group (from the slice's first) of each of a thread's 8 channels cl .. cl + 7

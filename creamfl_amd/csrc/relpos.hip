@@ -21,7 +21,10 @@
 
 namespace {
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16;
 typedef unsigned int u32;
@@ -104,16 +107,16 @@ __device__ __forceinline__ void zero16(f32x16& a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) a[r] = 0.f;
 }
+// (as a vector: one instruction for two values; converted one by one they are put together by two more)
 __device__ __forceinline__ u32 pack2(float a, float b) {
-    union { __bf16 h[2]; u32 u; } x;
-    x.h[0] = (__bf16)a; x.h[1] = (__bf16)b;
-    return x.u;
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(u32, __builtin_convertvector(v, bf16x2));
 }
 __device__ __forceinline__ bf16x8 pack_acc(const f32x16& a, int kk) {
-    f32x4 v;
+    f32x8 v;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) v[t] = __uint_as_float(pack2(a[8 * kk + 2 * t], a[8 * kk + 2 * t + 1]));
-    return __builtin_bit_cast(bf16x8, v);
+    for (int t = 0; t < 8; ++t) v[t] = a[8 * kk + t];
+    return __builtin_convertvector(v, bf16x8);
 }
 // operand whose lane owns row `row0 + (lane & 31)` of a staged tile, contraction over d: 16 kk + 8 (lane >> 5) .. + 7
 __device__ __forceinline__ bf16x8 frag_rows(const u16* t, int row0, int kk, int lane) {
