@@ -16,7 +16,6 @@
 // one query and its keys sit in the lane's registers; registers 8 kk .. 8 kk + 7 are then, packed to bf16, the second operand of the
 // following product (o^T = V^T P^T) whose first operand is read transposed out of LDS in the same key order (ds_read_b64_tr_b16).
 // P and ds are rounded to bf16 there (2^-9 relative, the precision of v and k themselves); sums stay in 32 bits.
-#include <limits.h>
 #include "common.h"
 
 namespace {
@@ -30,7 +29,7 @@ typedef unsigned short u16;
 typedef unsigned int u32;
 typedef unsigned long long u64;
 
-constexpr int TP = 72;                      // LDS row pitch in bf16 (144 bytes: 16-byte rows and both kinds of reads spread over the banks)
+constexpr int TP = 72;                      // LDS row pitch in bf16 of the kernel for short texts (144 bytes: spread over the banks)
 constexpr int BPAD = 96;                    // the bias vector reaches this far beyond +-R: a tile of 32 x 64 that touches |d| < R needs no clipping
 constexpr int MAXR = 512;                   // largest R (LDS)
 constexpr float LOG2E = 1.4426950408889634f;
@@ -118,10 +117,6 @@ __device__ __forceinline__ bf16x8 pack_acc(const f32x16& a, int kk) {
     for (int t = 0; t < 8; ++t) v[t] = a[8 * kk + t];
     return __builtin_convertvector(v, bf16x8);
 }
-// operand whose lane owns row `row0 + (lane & 31)` of a staged tile, contraction over d: 16 kk + 8 (lane >> 5) .. + 7
-__device__ __forceinline__ bf16x8 frag_rows(const u16* t, int row0, int kk, int lane) {
-    return __builtin_bit_cast(bf16x8, *reinterpret_cast<const f32x4*>(t + (row0 + (lane & 31)) * TP + kk * 16 + (lane >> 5) * 8));
-}
 // operand whose lane owns column 32 dt + (lane & 31) of a staged tile, contraction over rows in the accumulators' order:
 // row0 + 4 (lane >> 5) + {0..3} and + 8 (a 16-lane group's transposing read takes a [4 rows x 16 columns] block)
 __device__ __forceinline__ bf16x8 frag_cols(const u16* t, int row0, int dt, int lane) {
@@ -139,30 +134,43 @@ __device__ __forceinline__ void load_rows(const u16* base, long long ld, int row
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) f[kk] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const f32x4*>(p + kk * 16));
 }
-// One tile of ROWS rows on its way from memory to LDS through registers: `load` early, `put` late.  Rows whose bit in `bits` is 0 (dropped
-// keys, rows past the end) become zeros: whatever stands there, infinities and NaN included, must not reach a product.
-template <int NT, int ROWS>
-struct Stage {
-    static constexpr int N = ROWS * 8 / NT;
-    static constexpr u64 FULL = ROWS == 64 ? ~0ull : 0xffffffffull;
-    f32x4 r[N];
-    __device__ __forceinline__ void load(const u16* base, u32 ld, u64 bits) {      // base: the tile's first row, the same for every lane
-        const char* p = reinterpret_cast<const char*>(base);
-        u32 off = ((threadIdx.x >> 3) * ld + (threadIdx.x & 7) * 8) * 2;
-        if (bits == FULL) {
+// A staged tile: ROWS rows of 128 bytes, the 16-byte piece p of row r at place p ^ (r & 7) of its row: both kinds of reads below, and the
+// copy, spread over the banks without padding.  The copy goes straight to LDS, 8 rows an instruction, issued from inline assembly: the
+// compiler would wait for all of it before the next LDS read, while here it has a whole tile's computation to land (`landed`, then a
+// barrier).  Rows past the end repeat the last one; rows whose bit in `bits` is 0 (these, and dropped keys) are cleared by the lanes that
+// copied them: whatever stands there, infinities and NaN included, must not reach a product.
+template <int NW, int ROWS>
+struct Tile {
+    static __device__ __forceinline__ void copy(const u16* base, u32 ld, int valid, const u16* tile, int w, int lane) {
+        const u32 dst = (u32)(size_t)(__attribute__((address_space(3))) const u16*)tile;
 #pragma unroll
-            for (int i = 0; i < N; ++i, off += NT / 8 * 2 * ld) r[i] = *reinterpret_cast<const f32x4*>(p + off);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i, off += NT / 8 * 2 * ld) {
-                r[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if ((bits >> (i * (NT / 8) + (threadIdx.x >> 3))) & 1) r[i] = *reinterpret_cast<const f32x4*>(p + off);
-            }
+        for (int i = 0; i < ROWS / 8 / NW; ++i) {
+            const int ins = w + i * NW;
+            const u32 off = (u32)min(ins * 8 + (lane >> 3), valid - 1) * ld * 2 + (((lane & 7) ^ (lane >> 3)) << 4);
+            const u32 to = __builtin_amdgcn_readfirstlane(dst + ins * 1024);
+            u32 keep;
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                         : "=&s"(keep) : "v"(off), "s"(base), "s"(to) : "memory");
         }
     }
-    __device__ __forceinline__ void put(u16* tile) const {
+    static __device__ __forceinline__ void landed(u16* tile, u64 bits, int w, int lane) {
+        if (bits == (ROWS == 64 ? ~0ull : 0xffffffffull)) return;
+        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4*>(tile + (i * (NT / 8) + (threadIdx.x >> 3)) * TP + (threadIdx.x & 7) * 8) = r[i];
+        for (int i = 0; i < ROWS / 8 / NW; ++i) {
+            const int ins = w + i * NW;
+            if (!((bits >> (ins * 8 + (lane >> 3))) & 1)) *reinterpret_cast<f32x4*>(tile + ins * 512 + lane * 8) = z;
+        }
+    }
+};
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// byte offsets of a lane's reads: row (lane & 31), piece (lane >> 5); row 4 (lane >> 5) + ..., column 16 ((lane >> 4) & 1) + ...
+struct Places {
+    u32 row, col;
+    __device__ __forceinline__ explicit Places(int lane) {
+        const int p = lane & 15, g = lane >> 4, r = 4 * (g >> 1) + (p >> 2);
+        row = (lane & 31) * 128 + (((lane >> 5) ^ (lane & 7)) << 4);
+        col = r * 128 + (((2 * (g & 1) + ((p & 3) >> 1)) ^ r) << 4) + (p & 1) * 8;
     }
 };
 __device__ __forceinline__ u64 low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
@@ -233,22 +241,32 @@ __device__ __forceinline__ bool tile_near(int R, int d0, int n, bool key_lane) {
 }
 // ... and, where it does not, the one bias it has
 __device__ __forceinline__ float far_bias(const float* bl, int R, int d0) { return bl[(d0 > 0 ? R : -R) + R + BPAD]; }
-// S = A B^T of U blocks of 32 staged rows against a wave's 32; the blocks' chains of four take turns
+// S += A B^T of U blocks of 32 staged rows against a wave's 32; the blocks' chains of four take turns.  The lane's operand: its row's d
+// 16 kk + 8 (lane >> 5) .. + 7
 template <int U>
-__device__ __forceinline__ void mma_rows(const u16* tile, const bf16x8 (&f)[4], f32x16 (&s)[U], int lane) {
+__device__ __forceinline__ void mma_rows(const u16* tile, const Places& at, const bf16x8 (&f)[4], f32x16 (&s)[U]) {
+    const char* t = reinterpret_cast<const char*>(tile);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-        for (int u = 0; u < U; ++u) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows(tile, 32 * u, kk, lane), f[kk], s[u], 0, 0, 0);
+        for (int u = 0; u < U; ++u)
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(t + 4096 * u + (at.row ^ (kk << 5))), f[kk], s[u], 0, 0, 0);
 }
-// out^T += (tile's columns) (w packed to bf16), contraction over the 32 rows of block u
-__device__ __forceinline__ void mma_cols(const u16* tile, int u, const f32x16& w, f32x16 (&out)[2], int lane) {
+// out^T += (tile's columns) (w packed to bf16), contraction over the 32 rows of block u; the lane's operand: column 32 dt + (lane & 31), rows
+// in the accumulators' order (a 16-lane group's transposing read takes a [4 rows x 16 columns] block)
+__device__ __forceinline__ void mma_cols(const u16* tile, const Places& at, int u, const f32x16& w, f32x16 (&out)[2]) {
+    const char* t = reinterpret_cast<const char*>(tile);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
         const bf16x8 f = pack_acc(w, kk);
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt)
-            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(tile, 32 * u + 16 * kk, dt, lane), f, out[dt], 0, 0, 0);
+        for (int dt = 0; dt < 2; ++dt) {
+            const char* a = t + (2 * u + kk) * 2048 + (at.col ^ (dt << 6));
+            union { s16x4 h[2]; bf16x8 v; } x;
+            x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+            x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 1024));
+            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v, f, out[dt], 0, 0, 0);
+        }
     }
 }
 // dropped keys of block u: -inf (lane = query, registers = keys)
@@ -294,10 +312,11 @@ __device__ __forceinline__ void store_part(const f32x16 (&o)[2], float* out, int
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     constexpr int NT = NW * 64, U = KT / 32;
-    __shared__ __attribute__((aligned(16))) u16 Kt[NB][KT * TP], Vt[NB][KT * TP];
+    __shared__ __attribute__((aligned(1024))) u16 Kt[NB][KT * 64], Vt[NB][KT * 64];
     __shared__ u64 tb[64];
     extern __shared__ float bl[];
     const int lane = threadIdx.x & 63, w = wave_id();
+    const Places at(lane);
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
@@ -320,29 +339,28 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
         keys.chunk(c0);
         u64 left = keys.alive;
-        Stage<NT, KT> ks, vs;
         int cur = next_tile(left);
         if (cur < 0) continue;
         u64 bits = keys.bits(cur);
-        ks.load(kp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
-        vs.load(vp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
         int buf = 0;
+        const auto copy = [&](int tile, int to) {
+            const int k0 = c0 + tile * KT;
+            Tile<NW, KT>::copy(kp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Kt[to], w, lane);
+            Tile<NW, KT>::copy(vp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Vt[to], w, lane);
+        };
         __syncthreads();                                       // (the tiles' last readers, the bias vector)
-        ks.put(Kt[0]);
-        vs.put(Vt[0]);
+        copy(cur, 0);
         while (true) {
             const int d0 = c0 + cur * KT - q0, nxt = next_tile(left);
-            u64 nbits = 0;
-            if (nxt >= 0) {
-                nbits = keys.bits(nxt);
-                ks.load(kp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
-                vs.load(vp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
-            }
-            __syncthreads();
+            wait_copies();
+            Tile<NW, KT>::landed(Kt[buf], bits, w, lane);
+            Tile<NW, KT>::landed(Vt[buf], bits, w, lane);
+            __syncthreads();                                   // (this tile for every wave; the other buffer's readers are done)
+            if (NB > 1 && nxt >= 0) copy(nxt, buf ^ 1);
             f32x16 s[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) zero16(s[u]);
-            mma_rows<U>(Kt[buf], qf, s, lane);
+            mma_rows<U>(Kt[buf], at, qf, s);
             if (tile_near(a.R, d0, KT, false)) {
                 const float* bp = bl + a.R + BPAD + d0 + 4 * (lane >> 5) - (lane & 31);
 #pragma unroll
@@ -389,14 +407,17 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
                     l0 += s[u][r];
                     l1 += s[u][r + 1];
                 }
-                mma_cols(Vt[buf], u, s[u], o, lane);
+                mma_cols(Vt[buf], at, u, s[u], o);
             }
             if (nxt < 0) break;
-            if (NB == 1) __syncthreads(); else buf ^= 1;
-            ks.put(Kt[buf]);
-            vs.put(Vt[buf]);
+            if (NB > 1) {
+                buf ^= 1;
+            } else {
+                __syncthreads();
+                copy(nxt, 0);
+            }
             cur = nxt;
-            bits = nbits;
+            bits = keys.bits(nxt);
         }
     }
     float l = l0 + l1;
@@ -404,51 +425,57 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     const int row = q0 + (lane & 31);
     if (row >= t.lq) return;
     if (a.ns > 1) {
-        const long long at = ((long long)sp * a.heads + h) * a.rows + t.q0 + row;
-        store_part(o, a.po + at * 64, lane);
-        if (lane < 32) { a.pm[2 * at] = first ? -INFINITY : m; a.pm[2 * at + 1] = l; }
+        const long long to = ((long long)sp * a.heads + h) * a.rows + t.q0 + row;
+        store_part(o, a.po + to * 64, lane);
+        if (lane < 32) { a.pm[2 * to] = first ? -INFINITY : m; a.pm[2 * to + 1] = l; }
     } else {
         store_row(o, a.out + (t.q0 + row) * a.ldo + h * 64, lane, first ? 0.f : 1.f / l);
         if (a.lse && lane < 32) a.lse[h * a.rows + t.q0 + row] = first ? INFINITY : m + __builtin_amdgcn_logf(l);
     }
 }
 
-// Sums of a 32 x 32 block along its diagonals.  Register r of lane (x, half) holds query x and key kr = (r & 3) + 8 (r >> 2) + 4 half; read
-// from lane (x + kr) mod 32 it is the value of distance d0 - x, or d0 - x + 32 where that wrapped.  `here` + the block before's `next` are
-// the sums of the distances d0 - x.
-struct Diag {
-    float here, next;
-    __device__ __forceinline__ void add(const f32x16& v, int lane) {
-        const int at = 4 * ((lane & 31) + 4 * (lane >> 5)), half = 4 * (lane & 32);
-        here = next;
-        next = 0.f;
+// Sums of a 32 x 32 block along its diagonals, added to dst[d0 .. ] in LDS (dst: the place of distance 0).  Register r of lane (x, half)
+// holds query x and key j = (r & 3) + 8 (r >> 2) + 4 half, distance d0 + j - x.  With the queries in lanes 32 .. 63 and zeros below, the sums
+// are  t <- (t moved down one lane) + v_j  for j from the highest down: lane i then holds the distance d0 + 32 - i.  One instruction moves
+// and adds; two chains of 16 keys take turns.  The 64 addresses of an LDS addition are distinct and a wave's LDS operations stay in order,
+// so the order of every sum is fixed.
+__device__ __forceinline__ float down_one(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x130, 0xf, 0xf, true));
+}
+__device__ __forceinline__ void diag_add(const f32x16& v, float* dst, int lane) {
+    float hi = 0.f, lo = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int to = at + 4 * ((r & 3) + 8 * (r >> 2));
-            const float f = __int_as_float(__builtin_amdgcn_ds_bpermute((to & 124) | half, __float_as_int(v[r])));
-            const bool over = to >= 128;
-            here += over ? 0.f : f;
-            next += over ? f : 0.f;
+    for (int g = 1; g >= 0; --g) {
+        u32 low[8], up[8];                                     // half 0's and half 1's values of the groups g + 2 and g, in lanes 32 .. 63
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const auto w = __builtin_amdgcn_permlane32_swap(0u, __float_as_uint(v[4 * (g + (k < 4 ? 2 : 0)) + (k & 3)]), false, false);
+            low[k] = w[0]; up[k] = w[1];
         }
+#pragma unroll
+        for (int k = 3; k >= 0; --k) { hi = down_one(hi) + __uint_as_float(up[k]); lo = down_one(lo) + __uint_as_float(up[k + 4]); }
+#pragma unroll
+        for (int k = 3; k >= 0; --k) { hi = down_one(hi) + __uint_as_float(low[k]); lo = down_one(lo) + __uint_as_float(low[k + 4]); }
     }
-};
+    lds_add(dst + 16 + 32 - lane, hi);
+    lds_add(dst + 32 - lane, lo);
+}
 
 // ---- backward, queries: D, dQ and the bias gradient.  Same ownership as the forward.
-// The bias gradient of a distance is the sum of ds along a diagonal.  A lane's 16 values of a near block lie on 16 diagonals: each is moved
-// to the lane of its diagonal (key - query mod 32; `Diag`) and summed in registers, with one LDS addition per block into words of the
-// wave's own (the addresses of one instruction are distinct and a wave's LDS operations stay in order, so the sum's order is fixed;
-// adding all 16 in LDS took 340 us instead of @DQ@ at 32 texts of 512 tokens, 12 heads).  Far tiles are summed in registers.  At the end the
-// workgroup's sums per distance go to part [heads][slots][nd], one slot per (text, query block, part), place d + R + BPAD.
+// The bias gradient of a distance is the sum of ds along a diagonal (diag_add, into words of the wave's own; adding every value in LDS took
+// 340 us instead of @DQ@ at 32 texts of 512 tokens, 12 heads).  Tiles beyond +-R are summed in registers.  At the end the workgroup's sums per
+// distance go to part [heads][slots][nd], one slot per (text, query block, part), place d + R + BPAD.
 template <int NW, int KT, int NB>
-__global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel(RpArgs a) {
     constexpr int NT = NW * 64, U = KT / 32;
-    __shared__ __attribute__((aligned(16))) u16 Kt[NB][KT * TP], Vt[NB][KT * TP];
+    __shared__ __attribute__((aligned(1024))) u16 Kt[NB][KT * 64], Vt[NB][KT * 64];
     __shared__ u64 tb[64];
     extern __shared__ float dyn[];
     const int nd = 2 * (a.R + BPAD) + 1, mid = a.R + BPAD;
     float* bl = dyn;
-    float* dg = dyn + nd;                                      // [2 NW][nd]
+    float* dg = dyn + nd;                                      // [NW][nd]
     const int lane = threadIdx.x & 63, w = wave_id();
+    const Places at(lane);
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
@@ -461,16 +488,10 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     }
     const int dlo = max(-(t.lq | (NW * 32 - 1)), -mid), dhi = min(t.lk | (KT - 1), mid);      // (rows past the end are computed with as well)
     fill_bias<NT>(a, h, bl, dlo, dhi);
-    for (int c = 0; c < 2 * NW; ++c)
+    for (int c = 0; c < NW; ++c)
         for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) dg[c * nd + d + mid] = 0.f;
     float far_lo = 0.f, far_hi = 0.f;
-    float* mine = dg + (2 * w + (lane >> 5)) * nd + mid - (lane & 31);
-    Diag sums{0.f, 0.f};
-    int dn = INT_MIN;                                          // the distance (first key - first query) that sums.next belongs to
-    const auto flush = [&]() {
-        if (dn != INT_MIN) lds_add(mine + dn, sums.next);
-        sums.next = 0.f;
-    };
+    float* mine = dg + w * nd + mid;
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
@@ -479,19 +500,16 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     bf16x8 qf[4], gf[4];
     load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, q0, t.lq, lane, qf);
     load_rows(a.dout + t.q0 * a.ldo + h * 64, a.ldo, q0, t.lq, lane, gf);
-    f32x16 negD;                                               // -D in every register: dp's sum starts from it
+    float D = 0.f;
     {
         bf16x8 of[4];
         load_rows(a.o + t.q0 * a.ldo + h * 64, a.ldo, q0, t.lq, lane, of);
-        float D = 0.f;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int j = 0; j < 8; ++j) D = fmaf((float)of[kk][j], (float)gf[kk][j], D);
         D += __shfl_xor(D, 32, 64);
         if (live && lane < 32 && sp == 0) a.dsum[h * a.rows + t.q0 + row] = D;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) negD[r] = -D;
     }
     const float lse = live ? a.lse[h * a.rows + t.q0 + row] : INFINITY;      // (+inf: p = 0 in every row that does not count)
     f32x16 dq[2];
@@ -499,96 +517,81 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dq_kernel(RpArgs a) {
     for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
         keys.chunk(c0);
         u64 left = keys.alive;
-        Stage<NT, KT> ks, vs;
         int cur = next_tile(left);
         if (cur < 0) continue;
         u64 bits = keys.bits(cur);
-        ks.load(kp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
-        vs.load(vp + (long long)(c0 + cur * KT) * a.ldk, (u32)a.ldk, bits);
         int buf = 0;
+        const auto copy = [&](int tile, int to) {
+            const int k0 = c0 + tile * KT;
+            Tile<NW, KT>::copy(kp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Kt[to], w, lane);
+            Tile<NW, KT>::copy(vp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Vt[to], w, lane);
+        };
         __syncthreads();
-        ks.put(Kt[0]);
-        vs.put(Vt[0]);
+        copy(cur, 0);
         while (true) {
             const int d0 = c0 + cur * KT - q0, nxt = next_tile(left);
-            u64 nbits = 0;
-            if (nxt >= 0) {
-                nbits = keys.bits(nxt);
-                ks.load(kp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
-                vs.load(vp + (long long)(c0 + nxt * KT) * a.ldk, (u32)a.ldk, nbits);
-            }
-            __syncthreads();
-            f32x16 s[U], dp[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) { zero16(s[u]); dp[u] = negD; }
-            mma_rows<U>(Kt[buf], qf, s, lane);
-            mma_rows<U>(Vt[buf], gf, dp, lane);
+            wait_copies();
+            Tile<NW, KT>::landed(Kt[buf], bits, w, lane);
+            Tile<NW, KT>::landed(Vt[buf], bits, w, lane);
+            __syncthreads();                                   // (this tile for every wave; the other buffer's readers are done)
+            if (NB > 1 && nxt >= 0) copy(nxt, buf ^ 1);
             const bool near = tile_near(a.R, d0, KT, false);
-            if (near) {
-                const float* bp = bl + mid + d0 + 4 * (lane >> 5) - (lane & 31);
+            const float* bp = bl + mid + (near ? d0 : 0) + 4 * (lane >> 5) - (lane & 31);
+            const float c = far_bias(bl, a.R, near ? 0 : d0) - lse;
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                f32x16 s[1], dp[1];
+                zero16(s[0]); zero16(dp[0]);
+                mma_rows<1>(Kt[buf] + 2048 * u, at, qf, s);
+                mma_rows<1>(Vt[buf] + 2048 * u, at, gf, dp);
+                if (near) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, bp[32 * u + (r & 3) + 8 * (r >> 2)] - lse);
-            } else {
-                const float c = far_bias(bl, a.R, d0) - lse;
+                    for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], a.scale2, bp[32 * u + (r & 3) + 8 * (r >> 2)] - lse);
+                } else {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], a.scale2, c);
-            }
-            if (bits != Keys<NW, KT>::FULL) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) drop_keys(s[u], bits, u, lane);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(s[u][r]) * dp[u][r];
-            if (near) {
-                if (d0 != dn) flush();                         // (not the tile after the last near one)
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    sums.add(s[u], lane);
-                    lds_add(mine + d0 + 32 * u, sums.here);
+                    for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], a.scale2, c);
                 }
-                dn = d0 + KT;
-            } else {
-                float x0 = 0.f, x1 = 0.f;
+                if (bits != Keys<NW, KT>::FULL) drop_keys(s[0], bits, u, lane);
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(s[0][r]) * (dp[0][r] - D);
+                if (near) {
+                    diag_add(s[0], mine + d0 + 32 * u, lane);
+                } else {
+                    float x0 = 0.f, x1 = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; r += 2) { x0 += s[u][r]; x1 += s[u][r + 1]; }
-                if (d0 > 0) far_hi += x0 + x1; else far_lo += x0 + x1;
+                    for (int r = 0; r < 16; r += 2) { x0 += s[0][r]; x1 += s[0][r + 1]; }
+                    if (d0 > 0) far_hi += x0 + x1; else far_lo += x0 + x1;
+                }
+                mma_cols(Kt[buf], at, u, s[0], dq);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) mma_cols(Kt[buf], u, s[u], dq, lane);
             if (nxt < 0) break;
-            if (NB == 1) __syncthreads(); else buf ^= 1;
-            ks.put(Kt[buf]);
-            vs.put(Vt[buf]);
+            if (NB > 1) {
+                buf ^= 1;
+            } else {
+                __syncthreads();
+                copy(nxt, 0);
+            }
             cur = nxt;
-            bits = nbits;
+            bits = keys.bits(nxt);
         }
     }
     if (live) {
         if (a.ns > 1) store_part(dq, a.po + (((long long)sp * a.heads + h) * a.rows + t.q0 + row) * 64, lane);
         else store_row(dq, a.dq + (t.q0 + row) * a.lddq + h * 64, lane, a.scale);
     }
-    flush();
     // the workgroup's sums per distance
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
     if (lane == 0) {                                           // (far tiles exist only where the range reaches beyond +-R)
-        if (dlo <= -a.R) dg[2 * w * nd + mid - a.R] += far_lo;
-        if (dhi >= a.R) dg[2 * w * nd + mid + a.R] += far_hi;
+        if (dlo <= -a.R) dg[w * nd + mid - a.R] += far_lo;
+        if (dhi >= a.R) dg[w * nd + mid + a.R] += far_hi;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < nd; i += NT) {
         float x = 0.f;
         if (i >= dlo + mid && i <= dhi + mid) {
 #pragma unroll
-            for (int c = 0; c < 2 * NW; ++c) x += dg[c * nd + i];
+            for (int c = 0; c < NW; ++c) x += dg[c * nd + i];
         }
         out[i] = x;
     }
@@ -600,11 +603,12 @@ __device__ __forceinline__ void put_dtable(void* dtable, int bf16, long long at,
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, int nkb) {
     constexpr int NT = NW * 64, U = KT / 32;
-    __shared__ __attribute__((aligned(16))) u16 Qt[NB][KT * TP], Gt[NB][KT * TP];
+    __shared__ __attribute__((aligned(1024))) u16 Qt[NB][KT * 64], Gt[NB][KT * 64];
     __shared__ __attribute__((aligned(16))) float ls[NB][KT], ds[NB][KT];      // -log-sum and -D of the staged queries
     extern __shared__ float bl[];
     float* gone = bl + 2 * (a.R + BPAD) + 1;                   // [KT] of -inf: what a lane reads whose key does not take part
     const int lane = threadIdx.x & 63, w = wave_id();
+    const Places at(lane);
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, kb = id / a.ns % nkb, h = id / (a.ns * nkb) % a.heads, b = id / (a.ns * nkb * a.heads);
     const Text t = text_of(a, b);
@@ -637,30 +641,26 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) { kf[kk] = __builtin_bit_cast(bf16x8, z); vf[kk] = __builtin_bit_cast(bf16x8, z); }
         }
-        Stage<NT, KT> qs, gs;
         float lr = 0.f, dr = 0.f;
-        const auto fetch = [&](int q0) {
-            const u64 bits = low_bits(min(KT, part.to - q0));
-            qs.load(qp + (long long)q0 * a.ldq, (u32)a.ldq, bits);
-            gs.load(gp + (long long)q0 * a.ldo, (u32)a.ldo, bits);
+        const auto fetch = [&](int q0, int to) {
+            Tile<NW, KT>::copy(qp + (long long)q0 * a.ldq, (u32)a.ldq, part.to - q0, Qt[to], w, lane);
+            Tile<NW, KT>::copy(gp + (long long)q0 * a.ldo, (u32)a.ldo, part.to - q0, Gt[to], w, lane);
             if (threadIdx.x < KT) {
                 const bool in = q0 + (int)threadIdx.x < part.to;
                 lr = in ? -lp[q0 + threadIdx.x] : -INFINITY;
                 dr = in ? -dp_[q0 + threadIdx.x] : 0.f;
             }
         };
-        const auto put = [&](int buf) {
-            qs.put(Qt[buf]);
-            gs.put(Gt[buf]);
-            if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
-        };
-        fetch(part.from);
         int buf = 0;
-        put(0);
+        fetch(part.from, 0);
         for (int q0 = part.from; ; ) {
             const bool more = q0 + KT < part.to;
-            if (more) fetch(q0 + KT);
+            if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
+            wait_copies();
+            Tile<NW, KT>::landed(Qt[buf], low_bits(min(KT, part.to - q0)), w, lane);
+            Tile<NW, KT>::landed(Gt[buf], low_bits(min(KT, part.to - q0)), w, lane);
             __syncthreads();
+            if (NB > 1 && more) fetch(q0 + KT, buf ^ 1);
             const int d0 = k0 - q0;
             const bool near = tile_near(a.R, d0, KT, true);
             const float* bp = live ? bl + a.R + BPAD + (near ? d0 : 0) + (lane & 31) - 4 * (lane >> 5) : gone + KT - 1;
@@ -676,8 +676,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
 #pragma unroll
                     for (int j = 0; j < 4; ++j) { nl[4 * g + j] = x[j]; dp[0][4 * g + j] = y[j]; }
                 }
-                mma_rows<1>(Qt[buf] + 32 * u * TP, kf, s, lane);
-                mma_rows<1>(Gt[buf] + 32 * u * TP, vf, dp, lane);
+                mma_rows<1>(Qt[buf] + 2048 * u, at, kf, s);
+                mma_rows<1>(Gt[buf] + 2048 * u, at, vf, dp);
                 if (near) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) nl[r] += bp[-(32 * u + (r & 3) + 8 * (r >> 2))];
@@ -690,21 +690,25 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                     s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], a.scale2, nl[r]));
                     dp[0][r] *= s[0][r];
                 }
-                mma_cols(Gt[buf], u, s[0], dv, lane);
-                mma_cols(Qt[buf], u, dp[0], dk, lane);
+                mma_cols(Gt[buf], at, u, s[0], dv);
+                mma_cols(Qt[buf], at, u, dp[0], dk);
             }
             if (!more) break;
-            if (NB == 1) __syncthreads(); else buf ^= 1;
-            put(buf);
             q0 += KT;
+            if (NB > 1) {
+                buf ^= 1;
+            } else {
+                __syncthreads();
+                fetch(q0, 0);
+            }
         }
     }
     if (key >= t.lk) return;
     if (!live) { zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]); }
     if (a.ns > 1) {
-        const long long at = (((long long)sp * a.heads + h) * a.krows + t.k0 + key) * 64;
-        store_part(dk, a.po + at, lane);
-        store_part(dv, a.pv + at, lane);
+        const long long to = (((long long)sp * a.heads + h) * a.krows + t.k0 + key) * 64;
+        store_part(dk, a.po + to, lane);
+        store_part(dv, a.pv + to, lane);
     } else {
         store_row(dk, a.dk + (t.k0 + key) * a.lddk + h * 64, lane, a.scale);
         store_row(dv, a.dv + (t.k0 + key) * a.lddk + h * 64, lane, 1.f);
@@ -717,7 +721,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
 // 256 packed captions of 8 to 32 tokens, 12 heads: @B32@ us, against @B32OLD@ with the kernels for long texts.
 __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     __shared__ __attribute__((aligned(16))) u16 Kt[32 * TP], Qt[32 * TP], Gt[32 * TP];
-    __shared__ float bl[64];
+    __shared__ float bl[64], dgs[128];
     __shared__ __attribute__((aligned(16))) float ls[32], Ds[32];
     const int lane = threadIdx.x, x = lane & 31, half = lane >> 5;
     const int id = xcd_remap(blockIdx.x, gridDim.x), h = id % a.heads, b = id / a.heads;
@@ -775,11 +779,11 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     if (lane < 32) { ls[x] = lse; Ds[x] = D; }
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] *= dp[r] - D;
-    Diag dg{0.f, 0.f};
-    dg.add(s, lane);
-    dg.here += __shfl_xor(dg.here, 32, 64);
-    dg.next += __shfl_xor(dg.next, 32, 64);
-    part[half && x ? 64 - x : half ? 0 : 32 - x] = half ? dg.next : dg.here;      // (distance 32 does not occur: next of x = 0 is zero)
+    dgs[lane] = 0.f;
+    dgs[lane + 64] = 0.f;
+    diag_add(s, dgs + 32, lane);                               // (distances -31 .. 48: what lies beyond 31 is zero)
+    __syncthreads();
+    part[lane] = dgs[lane];
     f32x16 out[2];
     const auto store = [&](u16* p, long long ld, bool on, bool live, float c) {
         if (!on) return;
@@ -1028,7 +1032,7 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     a.po = (float*)at;
     at += rp_part_bytes(p, heads, a.rows);
     a.nqb = p.blocks; a.ns = p.ns;
-#define RP_LDS(NW) bl * (1 + 2 * (NW))
+#define RP_LDS(NW) bl * (1 + (NW))
     RP_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel, p, Lk, RP_LDS, a);
 #undef RP_LDS
     const int* qend = cu && !Lq ? cu + B : nullptr;
