@@ -16,6 +16,7 @@
 // one query and its keys sit in the lane's registers; registers 8 kk .. 8 kk + 7 are then, packed to bf16, the second operand of the
 // following product (o^T = V^T P^T) whose first operand is read transposed out of LDS in the same key order (ds_read_b64_tr_b16).
 // P and ds are rounded to bf16 there (2^-9 relative, the precision of v and k themselves); sums stay in 32 bits.
+#include <type_traits>
 #include "common.h"
 
 namespace {
@@ -53,10 +54,9 @@ struct RpArgs {
     int nqb;                                // query blocks of the longest text
     int ns;                                 // parts a text's keys (forward, dQ) or queries (dK, dV) are split into
     float *po, *pm;                         // the parts' results: [ns][heads][rows][64], and of the forward [ns][heads][rows][2] (maximum, sum)
+    float* pr;                              // of dQ [ns][heads][rows]: the rows' sums of ds
     float* pv;                              // dV's
-    float* share;                           // [heads][nshare][nb]: the bias gradient by blocks of distances
-    int nshare;
-    void* dtable;
+    u32* done;                              // [heads]: counted by cfl_relpos_dtable_kernel, started at 0 by dQ's kernel
     long long rows, krows;                  // query rows, key rows in all
 };
 
@@ -117,6 +117,14 @@ __device__ __forceinline__ bf16x8 pack_acc(const f32x16& a, int kk) {
     for (int t = 0; t < 8; ++t) v[t] = a[8 * kk + t];
     return __builtin_convertvector(v, bf16x8);
 }
+// what pack_acc's rounding left off
+__device__ __forceinline__ bf16x8 pack_rest(const f32x16& a, const bf16x8& f, int kk) {
+    const f32x8 w = __builtin_convertvector(f, f32x8);
+    f32x8 v;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] = a[8 * kk + t] - w[t];
+    return __builtin_convertvector(v, bf16x8);
+}
 // operand whose lane owns column 32 dt + (lane & 31) of a staged tile, contraction over rows in the accumulators' order:
 // row0 + 4 (lane >> 5) + {0..3} and + 8 (a 16-lane group's transposing read takes a [4 rows x 16 columns] block)
 __device__ __forceinline__ bf16x8 frag_cols(const u16* t, int row0, int dt, int lane) {
@@ -139,14 +147,16 @@ __device__ __forceinline__ void load_rows(const u16* base, long long ld, int row
 // compiler would wait for all of it before the next LDS read, while here it has a whole tile's computation to land (`landed`, then a
 // barrier).  Rows past the end repeat the last one; rows whose bit in `bits` is 0 (these, and dropped keys) are cleared by the lanes that
 // copied them: whatever stands there, infinities and NaN included, must not reach a product.
-template <int NW, int ROWS>
+// APART: rows 32 .. 63 are at place p ^ 4 ^ (r & 7), for the reader that takes rows r and r + 32 together (Apart below).
+template <int NW, int ROWS, bool APART = false>
 struct Tile {
     static __device__ __forceinline__ void copy(const u16* base, u32 ld, int valid, const u16* tile, int w, int lane) {
         const u32 dst = (u32)(size_t)(__attribute__((address_space(3))) const u16*)tile;
 #pragma unroll
         for (int i = 0; i < ROWS / 8 / NW; ++i) {
             const int ins = w + i * NW;
-            const u32 off = (u32)min(ins * 8 + (lane >> 3), valid - 1) * ld * 2 + (((lane & 7) ^ (lane >> 3)) << 4);
+            const u32 off = (u32)min(ins * 8 + (lane >> 3), valid - 1) * ld * 2 +
+                            (((lane & 7) ^ (lane >> 3) ^ (APART ? (ins >> 2) << 2 : 0)) << 4);
             const u32 to = __builtin_amdgcn_readfirstlane(dst + ins * 1024);
             u32 keep;
             asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
@@ -171,6 +181,16 @@ struct Places {
         const int p = lane & 15, g = lane >> 4, r = 4 * (g >> 1) + (p >> 2);
         row = (lane & 31) * 128 + (((lane >> 5) ^ (lane & 7)) << 4);
         col = r * 128 + (((2 * (g & 1) + ((p & 3) >> 1)) ^ r) << 4) + (p & 1) * 8;
+    }
+};
+// Of 64 staged rows in two blocks: block u of the product S = rows x columns takes row 32 (1 - half) + 16 u + r as the one whose scores stand in
+// register r of the lanes `half`, so that both halves' rows follow one another in the registers, 32 apart; byte offsets as above.
+struct Apart {
+    u32 row, col;
+    __device__ __forceinline__ explicit Apart(int lane) {
+        const int p = lane & 15, g = lane >> 4, r = (lane & 3) + 4 * ((lane & 31) >> 3), h = (lane >> 2) & 1;
+        row = (32 * (1 - h) + r) * 128 + (((lane >> 5) ^ (r & 7) ^ (4 * (1 - h))) << 4);
+        col = (32 * (1 - (g >> 1)) + (p >> 2)) * 128 + (((2 * (g & 1) + ((p & 3) >> 1)) ^ (p >> 2) ^ (4 * (1 - (g >> 1)))) << 4) + (p & 1) * 8;
     }
 };
 __device__ __forceinline__ u64 low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
@@ -207,6 +227,18 @@ __device__ __forceinline__ int next_tile(u64& alive) {         // the lowest til
     const int t = __builtin_ctzll(alive);
     alive &= alive - 1;
     return t;
+}
+
+// step(buffer) for the NB buffers in turn until it is done.  The buffer is a constant in each copy of the loop: its LDS addresses are offsets in the
+// instructions, where a variable one costs an addition for every read.
+template <int NB, class Step>
+__device__ __forceinline__ void in_turn(const Step& step) {
+    while (true) {
+        if (step(std::integral_constant<int, 0>{})) break;
+        if constexpr (NB > 1) {
+            if (step(std::integral_constant<int, 1>{})) break;
+        }
+    }
 }
 
 // part `sp` of `ns` of n rows in whole tiles: [from, to)
@@ -265,6 +297,28 @@ __device__ __forceinline__ void mma_cols(const u16* tile, const Places& at, int 
             union { s16x4 h[2]; bf16x8 v; } x;
             x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
             x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 1024));
+            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v, f, out[dt], 0, 0, 0);
+        }
+    }
+}
+// ... the same two products of block u with the rows taken as by Apart
+__device__ __forceinline__ void mma_rows_apart(const u16* tile, const Apart& at, int u, const bf16x8 (&f)[4], f32x16& s) {
+    const char* t = reinterpret_cast<const char*>(tile) + 2048 * u;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(t + (at.row ^ (kk << 5))), f[kk], s, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_cols_apart(const u16* tile, const Apart& at, int u, const f32x16& w, f32x16 (&out)[2]) {
+    const char* t = reinterpret_cast<const char*>(tile);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+        const bf16x8 f = pack_acc(w, kk);
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+            union { s16x4 h[2]; bf16x8 v; } x;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)                        // (four rows on: the other place of a pair)
+                x.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(t + (2 * u + kk) * 1024 + i * 512 +
+                                                                                                           (at.col ^ ((dt ^ i) << 6))));
             out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v, f, out[dt], 0, 0, 0);
         }
     }
@@ -342,7 +396,6 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
         int cur = next_tile(left);
         if (cur < 0) continue;
         u64 bits = keys.bits(cur);
-        int buf = 0;
         const auto copy = [&](int tile, int to) {
             const int k0 = c0 + tile * KT;
             Tile<NW, KT>::copy(kp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Kt[to], w, lane);
@@ -350,7 +403,8 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
         };
         __syncthreads();                                       // (the tiles' last readers, the bias vector)
         copy(cur, 0);
-        while (true) {
+        const auto step = [&](auto buf_) {                     // one tile; whether it was the last
+            constexpr int buf = decltype(buf_)::value;
             const int d0 = c0 + cur * KT - q0, nxt = next_tile(left);
             wait_copies();
             Tile<NW, KT>::landed(Kt[buf], bits, w, lane);
@@ -409,16 +463,16 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
                 }
                 mma_cols(Vt[buf], at, u, s[u], o);
             }
-            if (nxt < 0) break;
-            if (NB > 1) {
-                buf ^= 1;
-            } else {
+            if (nxt < 0) return true;
+            if (NB == 1) {
                 __syncthreads();
                 copy(nxt, 0);
             }
             cur = nxt;
             bits = keys.bits(nxt);
-        }
+            return false;
+        };
+        in_turn<NB>(step);
     }
     float l = l0 + l1;
     l += __shfl_xor(l, 32, 64);
@@ -434,13 +488,25 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     }
 }
 
-// Sums of a 32 x 32 block along its diagonals, added to dst[d0 .. ] in LDS (dst: the place of distance 0).  Register r of lane (x, half)
-// holds query x and key j = (r & 3) + 8 (r >> 2) + 4 half, distance d0 + j - x.  With the queries in lanes 32 .. 63 and zeros below, the sums
-// are  t <- (t moved down one lane) + v_j  for j from the highest down: lane i then holds the distance d0 + 32 - i.  One instruction moves
-// and adds; two chains of 16 keys take turns.  The 64 addresses of an LDS addition are distinct and a wave's LDS operations stay in order,
-// so the order of every sum is fixed.
+// Sums of a 32 x 32 block along its diagonals.  Register r of lane (x, half) holds column x and row j = (r & 3) + 8 (r >> 2) + 4 half; the sum
+// over j - x = e is added to dst[-e] in LDS.  With the columns in lanes 32 .. 63 and zeros below, the sums are  t <- (t moved down one
+// lane) + v_j  for j from the highest down: lane i then holds e = 32 - i.  One instruction moves and adds; two chains of 16 rows take turns.
+// The 64 addresses of an LDS addition are distinct and a wave's LDS operations stay in order, so the order of every sum is fixed.
 __device__ __forceinline__ float down_one(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x130, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float down_one_round(float v) {     // (lane 0's goes to lane 63)
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x134, 0xf, 0xf, true));
+}
+// With rows taken as by Apart no lane stands idle: register r of lane l holds e = (row) - (column) = 32 + 16 u + r - l, so after the same steps lane i
+// holds e = 32 + 16 u - i; what has left at lane 0 is the difference to the same sums with the lanes in a ring: at lane i >= 49 e = 96 + 16 u - i.
+// dst: the place of e = 0, places fall with e.  32 instructions for 16 rows of 64 lanes, against 80 with the zeros below.
+__device__ __forceinline__ void diag_add_apart(const f32x16& v, float* dst, int u, int lane) {
+    float a = v[15], b = v[15];
+#pragma unroll
+    for (int r = 14; r >= 0; --r) { a = down_one(a) + v[r]; b = down_one_round(b) + v[r]; }
+    lds_add(dst + lane - 32 - 16 * u, a);
+    if (lane >= 49) lds_add(dst + lane - 96 - 16 * u, b - a);
 }
 __device__ __forceinline__ void diag_add(const f32x16& v, float* dst, int lane) {
     float hi = 0.f, lo = 0.f;
@@ -457,41 +523,30 @@ __device__ __forceinline__ void diag_add(const f32x16& v, float* dst, int lane) 
 #pragma unroll
         for (int k = 3; k >= 0; --k) { hi = down_one(hi) + __uint_as_float(low[k]); lo = down_one(lo) + __uint_as_float(low[k + 4]); }
     }
-    lds_add(dst + 16 + 32 - lane, hi);
-    lds_add(dst + 32 - lane, lo);
+    lds_add(dst + lane - 48, hi);
+    lds_add(dst + lane - 32, lo);
 }
 
-// ---- backward, queries: D, dQ and the bias gradient.  Same ownership as the forward.
-// The bias gradient of a distance is the sum of ds along a diagonal (diag_add, into words of the wave's own; adding every value in LDS took
-// 340 us instead of @DQ@ at 32 texts of 512 tokens, 12 heads).  Tiles beyond +-R are summed in registers.  At the end the workgroup's sums per
-// distance go to part [heads][slots][nd], one slot per (text, query block, part), place d + R + BPAD.
+// ---- backward, queries: dQ and D.  Same ownership as the forward.
+// D is formed from the rounded o, whose error is the same for a whole row of ds: the bias gradient would add it up along every diagonal.  But a
+// row of ds sums to nothing, so the row's sum here is that error, and D goes to dK / dV's kernel, which sums the diagonals, without it.
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel(RpArgs a) {
     constexpr int NT = NW * 64, U = KT / 32;
     __shared__ __attribute__((aligned(1024))) u16 Kt[NB][KT * 64], Vt[NB][KT * 64];
     __shared__ u64 tb[64];
-    extern __shared__ float dyn[];
-    const int nd = 2 * (a.R + BPAD) + 1, mid = a.R + BPAD;
-    float* bl = dyn;
-    float* dg = dyn + nd;                                      // [NW][nd]
+    extern __shared__ float bl[];
+    const int mid = a.R + BPAD;
     const int lane = threadIdx.x & 63, w = wave_id();
     const Places at(lane);
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, qb = id / a.ns % a.nqb, h = id / (a.ns * a.nqb) % a.heads, b = id / (a.ns * a.nqb * a.heads);
     const Text t = text_of(a, b);
     const Part part = part_of(sp, a.ns, t.lk, KT);
-    float* out = a.diag + ((((long long)h * a.B + b) * a.nqb + qb) * a.ns + sp) * nd;
     if (a.cu && !a.Lq && qb == 0) clear_rest<NT>(a, t, b, h, sp, a.dq, nullptr, a.lddq);
-    if (qb * NW * 32 >= t.lq) {
-        for (int i = threadIdx.x; i < nd; i += NT) out[i] = 0.f;
-        return;
-    }
-    const int dlo = max(-(t.lq | (NW * 32 - 1)), -mid), dhi = min(t.lk | (KT - 1), mid);      // (rows past the end are computed with as well)
-    fill_bias<NT>(a, h, bl, dlo, dhi);
-    for (int c = 0; c < NW; ++c)
-        for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) dg[c * nd + d + mid] = 0.f;
-    float far_lo = 0.f, far_hi = 0.f;
-    float* mine = dg + w * nd + mid;
+    if (blockIdx.x == 0) for (int i = threadIdx.x; i < a.heads; i += NT) a.done[i] = 0;
+    if (qb * NW * 32 >= t.lq) return;
+    fill_bias<NT>(a, h, bl, -(t.lq | (NW * 32 - 1)), t.lk | (KT - 1));     // (rows past the end are computed with as well)
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
@@ -509,9 +564,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
 #pragma unroll
             for (int j = 0; j < 8; ++j) D = fmaf((float)of[kk][j], (float)gf[kk][j], D);
         D += __shfl_xor(D, 32, 64);
-        if (live && lane < 32 && sp == 0) a.dsum[h * a.rows + t.q0 + row] = D;
     }
     const float lse = live ? a.lse[h * a.rows + t.q0 + row] : INFINITY;      // (+inf: p = 0 in every row that does not count)
+    float r0 = 0.f, r1 = 0.f;                                  // the row's sum of ds
     f32x16 dq[2];
     zero16(dq[0]); zero16(dq[1]);
     for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
@@ -520,7 +575,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
         int cur = next_tile(left);
         if (cur < 0) continue;
         u64 bits = keys.bits(cur);
-        int buf = 0;
         const auto copy = [&](int tile, int to) {
             const int k0 = c0 + tile * KT;
             Tile<NW, KT>::copy(kp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Kt[to], w, lane);
@@ -528,7 +582,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
         };
         __syncthreads();
         copy(cur, 0);
-        while (true) {
+        const auto step = [&](auto buf_) {                     // one tile; whether it was the last
+            constexpr int buf = decltype(buf_)::value;
             const int d0 = c0 + cur * KT - q0, nxt = next_tile(left);
             wait_copies();
             Tile<NW, KT>::landed(Kt[buf], bits, w, lane);
@@ -554,74 +609,71 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
                 if (bits != Keys<NW, KT>::FULL) drop_keys(s[0], bits, u, lane);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(s[0][r]) * (dp[0][r] - D);
-                if (near) {
-                    diag_add(s[0], mine + d0 + 32 * u, lane);
-                } else {
-                    float x0 = 0.f, x1 = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; r += 2) { x0 += s[0][r]; x1 += s[0][r + 1]; }
-                    if (d0 > 0) far_hi += x0 + x1; else far_lo += x0 + x1;
-                }
+                for (int r = 0; r < 16; r += 2) { r0 += s[0][r]; r1 += s[0][r + 1]; }
                 mma_cols(Kt[buf], at, u, s[0], dq);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (nxt < 0) break;
-            if (NB > 1) {
-                buf ^= 1;
-            } else {
+            if (nxt < 0) return true;
+            if (NB == 1) {
                 __syncthreads();
                 copy(nxt, 0);
             }
             cur = nxt;
             bits = keys.bits(nxt);
+            return false;
+        };
+        in_turn<NB>(step);
+    }
+    r0 += r1;
+    r0 += __shfl_xor(r0, 32, 64);
+    if (!live) return;
+    if (a.ns > 1) {
+        const long long to = ((long long)sp * a.heads + h) * a.rows + t.q0 + row;
+        store_part(dq, a.po + to * 64, lane);
+        if (lane < 32) {
+            a.pr[to] = r0;
+            if (sp == 0) a.dsum[h * a.rows + t.q0 + row] = D;  // (the join adds the sums)
         }
-    }
-    if (live) {
-        if (a.ns > 1) store_part(dq, a.po + (((long long)sp * a.heads + h) * a.rows + t.q0 + row) * 64, lane);
-        else store_row(dq, a.dq + (t.q0 + row) * a.lddq + h * 64, lane, a.scale);
-    }
-    // the workgroup's sums per distance
-    far_lo = wave_sum(far_lo);
-    far_hi = wave_sum(far_hi);
-    if (lane == 0) {                                           // (far tiles exist only where the range reaches beyond +-R)
-        if (dlo <= -a.R) dg[w * nd + mid - a.R] += far_lo;
-        if (dhi >= a.R) dg[w * nd + mid + a.R] += far_hi;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < nd; i += NT) {
-        float x = 0.f;
-        if (i >= dlo + mid && i <= dhi + mid) {
-#pragma unroll
-            for (int c = 0; c < NW; ++c) x += dg[c * nd + i];
-        }
-        out[i] = x;
+    } else {
+        store_row(dq, a.dq + (t.q0 + row) * a.lddq + h * 64, lane, a.scale);
+        if (lane < 32) a.dsum[h * a.rows + t.q0 + row] = D + r0;
     }
 }
 
-__device__ __forceinline__ void put_dtable(void* dtable, int bf16, long long at, float v);
-
-// ---- backward, keys: dK and dV.  A wave owns 32 keys; the staged rows are queries.
+// ---- backward, keys: dK, dV and the bias gradient.  A wave owns 32 keys; the staged rows are queries.
+// The bias gradient of a distance is the sum of ds along a diagonal (diag_add, into words of the wave's own; adding every value in LDS took
+// @DQ@ at 32 texts of 512 tokens, 12 heads).  Tiles beyond +-R are summed in registers.  At the end the workgroup's sums per distance go to
+// part [heads][slots][nd], one slot per (text, key block, part), place d + R + BPAD.
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, int nkb) {
     constexpr int NT = NW * 64, U = KT / 32;
     __shared__ __attribute__((aligned(1024))) u16 Qt[NB][KT * 64], Gt[NB][KT * 64];
     __shared__ __attribute__((aligned(16))) float ls[NB][KT], ds[NB][KT];      // -log-sum and -D of the staged queries
     extern __shared__ float bl[];
-    float* gone = bl + 2 * (a.R + BPAD) + 1;                   // [KT] of -inf: what a lane reads whose key does not take part
+    const int nd = 2 * (a.R + BPAD) + 1, mid = a.R + BPAD;
+    float* gone = bl + nd;                                     // [KT] of -inf: what a lane reads whose key does not take part
+    float* dg = gone + KT;                                     // [NW][nd]
     const int lane = threadIdx.x & 63, w = wave_id();
-    const Places at(lane);
+    constexpr bool APART = KT == 64;
+    typedef Tile<NW, KT, APART> TileQ;
+    const std::conditional_t<APART, Apart, Places> at(lane);
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int sp = id % a.ns, kb = id / a.ns % nkb, h = id / (a.ns * nkb) % a.heads, b = id / (a.ns * nkb * a.heads);
     const Text t = text_of(a, b);
     if (a.cu && kb == 0) clear_rest<NT>(a, t, b, h, sp, a.dk, a.dv, a.lddk);
-    if (b == 0 && kb == 0 && sp == 0)                          // the head's bias gradient: the last step of cfl_relpos_dtable_kernel
-        for (int i = threadIdx.x; i < a.nb; i += NT) {
-            float y = 0.f;
-            for (int k = 0; k < a.nshare; ++k) y += a.share[((long long)h * a.nshare + k) * a.nb + i];
-            put_dtable(a.dtable, a.table_bf16, (long long)i * a.heads + h, y);
-        }
-    if (kb * NW * 32 >= t.lk) return;
+    float* out = a.diag + ((((long long)h * a.B + b) * nkb + kb) * a.ns + sp) * nd;
+    if (kb * NW * 32 >= t.lk) {
+        for (int i = threadIdx.x; i < nd; i += NT) out[i] = 0.f;
+        return;
+    }
     const Part part = part_of(sp, a.ns, t.lq, KT);
-    fill_bias<NT>(a, h, bl, -(t.lq | (KT - 1)), t.lk | (NW * 32 - 1));
+    const int dlo = max(-(t.lq | (KT - 1)), -mid), dhi = min(t.lk | (NW * 32 - 1), mid);      // (rows past the end are computed with as well)
+    fill_bias<NT>(a, h, bl, dlo, dhi);
+    for (int c = 0; c < NW; ++c)
+        for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) dg[c * nd + d + mid] = 0.f;
+    float far_lo = 0.f, far_hi = 0.f;
+    float* mine = dg + w * nd + mid;
     for (int i = threadIdx.x; i < KT; i += NT) gone[i] = -INFINITY;
     const unsigned char* mask = a.mask ? a.mask + (long long)b * a.Lk : nullptr;
     const u16* qp = a.q + t.q0 * a.ldq + h * 64;
@@ -643,8 +695,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
         }
         float lr = 0.f, dr = 0.f;
         const auto fetch = [&](int q0, int to) {
-            Tile<NW, KT>::copy(qp + (long long)q0 * a.ldq, (u32)a.ldq, part.to - q0, Qt[to], w, lane);
-            Tile<NW, KT>::copy(gp + (long long)q0 * a.ldo, (u32)a.ldo, part.to - q0, Gt[to], w, lane);
+            TileQ::copy(qp + (long long)q0 * a.ldq, (u32)a.ldq, part.to - q0, Qt[to], w, lane);
+            TileQ::copy(gp + (long long)q0 * a.ldo, (u32)a.ldo, part.to - q0, Gt[to], w, lane);
             if (threadIdx.x < KT) {
                 const bool in = q0 + (int)threadIdx.x < part.to;
                 lr = in ? -lp[q0 + threadIdx.x] : -INFINITY;
@@ -657,13 +709,16 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
             const bool more = q0 + KT < part.to;
             if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
             wait_copies();
-            Tile<NW, KT>::landed(Qt[buf], low_bits(min(KT, part.to - q0)), w, lane);
-            Tile<NW, KT>::landed(Gt[buf], low_bits(min(KT, part.to - q0)), w, lane);
+            TileQ::landed(Qt[buf], low_bits(min(KT, part.to - q0)), w, lane);
+            TileQ::landed(Gt[buf], low_bits(min(KT, part.to - q0)), w, lane);
             __syncthreads();
             if (NB > 1 && more) fetch(q0 + KT, buf ^ 1);
             const int d0 = k0 - q0;
             const bool near = tile_near(a.R, d0, KT, true);
-            const float* bp = live ? bl + a.R + BPAD + (near ? d0 : 0) + (lane & 31) - 4 * (lane >> 5) : gone + KT - 1;
+            // the lane's first query in the tile, and how its registers go on from it
+            const int i0 = APART ? 32 - 32 * (lane >> 5) : 4 * (lane >> 5);
+            const auto query = [](int u, int r) { return APART ? 16 * u + r : 32 * u + (r & 3) + 8 * (r >> 2); };
+            const float* bp = live ? bl + mid + (near ? d0 : 0) + (lane & 31) - i0 : gone + KT - 1;
             const float c = live ? far_bias(bl, a.R, near ? 0 : d0) : -INFINITY;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -671,16 +726,21 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                 zero16(s[0]);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(&ls[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(&ds[buf][32 * u + 8 * g + 4 * (lane >> 5)]);
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(&ls[buf][i0 + query(u, 4 * g)]);
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(&ds[buf][i0 + query(u, 4 * g)]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) { nl[4 * g + j] = x[j]; dp[0][4 * g + j] = y[j]; }
                 }
-                mma_rows<1>(Qt[buf] + 2048 * u, at, kf, s);
-                mma_rows<1>(Gt[buf] + 2048 * u, at, vf, dp);
+                if constexpr (APART) {
+                    mma_rows_apart(Qt[buf], at, u, kf, s[0]);
+                    mma_rows_apart(Gt[buf], at, u, vf, dp[0]);
+                } else {
+                    mma_rows<1>(Qt[buf], at, kf, s);
+                    mma_rows<1>(Gt[buf], at, vf, dp);
+                }
                 if (near) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) nl[r] += bp[-(32 * u + (r & 3) + 8 * (r >> 2))];
+                    for (int r = 0; r < 16; ++r) nl[r] += bp[-query(u, r)];
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) nl[r] += c;
@@ -690,8 +750,22 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                     s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], a.scale2, nl[r]));
                     dp[0][r] *= s[0][r];
                 }
-                mma_cols(Gt[buf], at, u, s[0], dv);
-                mma_cols(Qt[buf], at, u, dp[0], dk);
+                if (near) {
+                    if constexpr (APART) diag_add_apart(dp[0], mine + d0, u, lane);
+                    else diag_add(dp[0], mine + d0, lane);
+                } else {
+                    float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; r += 2) { x0 += dp[0][r]; x1 += dp[0][r + 1]; }
+                    if (d0 > 0) far_hi += x0 + x1; else far_lo += x0 + x1;
+                }
+                if constexpr (APART) {
+                    mma_cols_apart(Gt[buf], at, u, s[0], dv);
+                    mma_cols_apart(Qt[buf], at, u, dp[0], dk);
+                } else {
+                    mma_cols(Gt[buf], at, 0, s[0], dv);
+                    mma_cols(Qt[buf], at, 0, dp[0], dk);
+                }
             }
             if (!more) break;
             q0 += KT;
@@ -702,6 +776,22 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                 fetch(q0, 0);
             }
         }
+    }
+    // the workgroup's sums per distance
+    far_lo = wave_sum(far_lo);
+    far_hi = wave_sum(far_hi);
+    if (lane == 0) {                                           // (far tiles exist only where the range reaches beyond +-R)
+        if (dlo <= -a.R) dg[w * nd + mid - a.R] += far_lo;
+        if (dhi >= a.R) dg[w * nd + mid + a.R] += far_hi;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nd; i += NT) {
+        float x = 0.f;
+        if (i >= dlo + mid && i <= dhi + mid) {
+#pragma unroll
+            for (int c = 0; c < NW; ++c) x += dg[c * nd + i];
+        }
+        out[i] = x;
     }
     if (key >= t.lk) return;
     if (!live) { zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]); }
@@ -717,7 +807,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
 
 // ---- backward of texts of at most 32 tokens: everything in one kernel, a wave per (text, head).  The rows come straight from memory as
 // operands; K, Q and dO pass through LDS for the products that contract over rows.  D is summed from p and dp themselves, so the
-// rounding of o plays no part.  The bias gradient's diagonals go to memory as they are: part [heads][B][64], place d + 32.
+// rounding of o plays no part; P and ds are taken as two bf16 terms: few products, and waiting for memory bounds this kernel.  The bias gradient's diagonals go to memory as they are: part [heads][B][64], place d + 32.
 // 256 packed captions of 8 to 32 tokens, 12 heads: @B32@ us, against @B32OLD@ with the kernels for long texts.
 __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     __shared__ __attribute__((aligned(16))) u16 Kt[32 * TP], Qt[32 * TP], Gt[32 * TP];
@@ -781,9 +871,6 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     for (int r = 0; r < 16; ++r) s[r] *= dp[r] - D;
     dgs[lane] = 0.f;
     dgs[lane + 64] = 0.f;
-    diag_add(s, dgs + 32, lane);                               // (distances -31 .. 48: what lies beyond 31 is zero)
-    __syncthreads();
-    part[lane] = dgs[lane];
     f32x16 out[2];
     const auto store = [&](u16* p, long long ld, bool on, bool live, float c) {
         if (!on) return;
@@ -802,9 +889,13 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
         zero16(out[0]); zero16(out[1]);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            const bf16x8 f = pack_acc(w, kk);
+            const bf16x8 f = pack_acc(w, kk), rest = pack_rest(w, f, kk);
 #pragma unroll
-            for (int dt = 0; dt < 2; ++dt) out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols(tile, 16 * kk, dt, lane), f, out[dt], 0, 0, 0);
+            for (int dt = 0; dt < 2; ++dt) {
+                const bf16x8 c = frag_cols(tile, 16 * kk, dt, lane);
+                out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c, f, out[dt], 0, 0, 0);
+                out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c, rest, out[dt], 0, 0, 0);
+            }
         }
     };
     apply(Kt, s);
@@ -826,8 +917,11 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     }
     apply(Gt, s);
     store(a.dv + t.k0 * a.lddk + h * 64, a.lddk, x < t.lk, keep, 1.f);
+    diag_add(dp, dgs + 64, lane);                              // (distances -48 .. 31: what lies below -31 is zero)
     apply(Qt, dp);
     store(a.dk + t.k0 * a.lddk + h * 64, a.lddk, x < t.lk, keep, a.scale);
+    __syncthreads();
+    part[lane] = dgs[lane + 32];
 }
 // ---- joins of the parts: a wave per (row, head), a lane per d
 __global__ __launch_bounds__(256) void cfl_relpos_join_kernel(const float* __restrict__ po, const float* __restrict__ pm, int ns, int heads,
@@ -850,7 +944,8 @@ __global__ __launch_bounds__(256) void cfl_relpos_join_kernel(const float* __res
     if (lse && lane == 0) lse[h * rows + row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 __global__ __launch_bounds__(256) void cfl_relpos_join_sum_kernel(const float* __restrict__ po, int ns, int heads, long long rows, long long last,
-                                                                  const int* __restrict__ end, float scale, u16* o, long long ldo) {
+                                                                  const int* __restrict__ end, float scale, u16* o, long long ldo,
+                                                                  const float* __restrict__ pr, float* dsum) {
     const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const long long row = i / heads, h = i % heads;
@@ -858,18 +953,24 @@ __global__ __launch_bounds__(256) void cfl_relpos_join_sum_kernel(const float* _
     float x = 0.f;
     for (int s = 0; s < ns; ++s) x += po[((s * heads + h) * rows + row) * 64 + lane];
     reinterpret_cast<__bf16*>(o)[row * ldo + h * 64 + lane] = (__bf16)(x * scale);
+    if (dsum && lane == 0) {
+        float y = 0.f;
+        for (int s = 0; s < ns; ++s) y += pr[(s * heads + h) * rows + row];
+        dsum[h * rows + row] += y;
+    }
 }
 
 // ---- the bias gradient from part [heads][slots][nd] (place i: distance i - mid): the slots' sums of 64 distances, then of these every
 // bucket's share, in a fixed order.  grid = (heads, ceil(nd / 64)), 64 distances x 16 strands of slots.  One block of distances: that is the
-// table's gradient; more: share [heads][blocks][nb], which the dK / dV kernel's first workgroups add up.
+// table's gradient; more: share [heads][blocks][nb], and the head's last workgroup (whichever it is) adds the blocks up in their order.
 __device__ __forceinline__ void put_dtable(void* dtable, int bf16, long long at, float v) {
     if (bf16) ((__bf16*)dtable)[at] = (__bf16)v;
     else ((float*)dtable)[at] = v;
 }
 __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __restrict__ part, int nd, int mid, long long slots,
-                                                                 const int* __restrict__ bucket, int R, int nb, int heads, float* share,
+                                                                 const int* __restrict__ bucket, int R, int nb, int heads, float* share, u32* done,
                                                                  void* dtable, int bf16) {
+    __shared__ u32 before;
     __shared__ float red[16][64];
     __shared__ int bk[64];
     const int h = blockIdx.x, lane = threadIdx.x & 63, strand = threadIdx.x >> 6, i = blockIdx.y * 64 + lane;
@@ -903,9 +1004,22 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
         for (int k = threadIdx.x & (L - 1); k < 64; k += L) y += bk[k] == b ? red[0][k] : 0.f;
         for (int o = L >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
         if (b < nb && (threadIdx.x & (L - 1)) == 0) {
-            if (share) share[((long long)h * gridDim.y + blockIdx.y) * nb + b] = y;
+            if (share) __hip_atomic_store(share + ((long long)h * gridDim.y + blockIdx.y) * nb + b, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             else put_dtable(dtable, bf16, (long long)b * heads + h, y);
         }
+    }
+    if (!share) return;
+    // (the shares are written through to memory and read from there: a fence would write back and drop whole caches, 30 us)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(done + h, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (before != gridDim.y - 1) return;
+    for (int i = threadIdx.x; i < nb; i += 1024) {
+        float y = 0.f;
+        for (int k = 0; k < (int)gridDim.y; ++k)
+            y += __hip_atomic_load(share + ((long long)h * gridDim.y + k) * nb + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        put_dtable(dtable, bf16, (long long)i * heads + h, y);
     }
 }
 
@@ -953,6 +1067,8 @@ inline size_t rp_part_bytes(const Shape& p, int heads, long long rows) {
     return p.ns > 1 ? cfl_align256((size_t)p.ns * heads * rows * 64 * 4) : 0;
 }
 
+inline size_t rp_row_bytes(const Shape& p, int heads, long long rows) { return p.ns > 1 ? cfl_align256((size_t)p.ns * heads * rows * 4) : 0; }
+
 }  // namespace
 
 extern "C" {
@@ -969,8 +1085,8 @@ size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb, 
     const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk), k = rp_shape((long long)B * heads, Lk, Lq ? Lq : Lk);
     const long long rows = Lq ? (long long)B * Lq : T, krows = T ? T : (long long)B * Lk;
     if (p.small) return (size_t)B * heads * 64 * 4;
-    return cfl_align256((size_t)B * heads * p.blocks * p.ns * rp_nd(R) * 4) + cfl_align256((size_t)heads * cfl_cdiv(rp_nd(R), 64) * nb * 4) +
-           rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
+    return cfl_align256((size_t)B * heads * k.blocks * k.ns * rp_nd(R) * 4) + cfl_align256((size_t)heads * cfl_cdiv(rp_nd(R), 64) * nb * 4) +
+           cfl_align256((size_t)heads * 4) + rp_row_bytes(p, heads, rows) + rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
 }
 
 int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
@@ -1025,40 +1141,42 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
         a.ns = 1;
         CFL_LAUNCH(K_RELPOS_BWD32, cfl_relpos_bwd32_kernel, dim3((unsigned)(B * heads)), dim3(64), 0, stream, a);
         CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, 1), dim3(1024), 0, stream, a.diag, 64, 32, (long long)B, bucket, R, nb,
-                   heads, (float*)nullptr, dtable, table_bf16);
+                   heads, (float*)nullptr, (u32*)nullptr, dtable, table_bf16);
         return 0;
     }
-    at += cfl_align256((size_t)B * heads * p.blocks * p.ns * rp_nd(R) * 4);
+    const int nd = rp_nd(R), nshare = cfl_cdiv(nd, 64);
+    at += cfl_align256((size_t)B * heads * kp.blocks * kp.ns * nd * 4);
+    float* share = (float*)at;
+    at += cfl_align256((size_t)heads * nshare * nb * 4);
+    a.done = (u32*)at;
+    at += cfl_align256((size_t)heads * 4);
+    a.pr = (float*)at;
+    at += rp_row_bytes(p, heads, a.rows);
     a.po = (float*)at;
     at += rp_part_bytes(p, heads, a.rows);
     a.nqb = p.blocks; a.ns = p.ns;
-#define RP_LDS(NW) bl * (1 + (NW))
+#define RP_LDS(NW) bl
     RP_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel, p, Lk, RP_LDS, a);
 #undef RP_LDS
     const int* qend = cu && !Lq ? cu + B : nullptr;
     if (p.ns > 1)
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, dim3((unsigned)((a.rows * heads + 3) / 4)), dim3(256), 0, stream, a.po, p.ns, heads,
-                   a.rows, a.rows, qend, scale, (u16*)dq, lddq);
-    const int nd = rp_nd(R);
-    a.nshare = cfl_cdiv(nd, 64);
-    a.share = (float*)at;
-    a.dtable = dtable;
-    at += cfl_align256((size_t)heads * a.nshare * nb * 4);
-    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, a.nshare), dim3(1024), 0, stream, a.diag, nd, R + BPAD,
-               (long long)B * p.blocks * p.ns, bucket, R, nb, heads, a.share, dtable, table_bf16);
+                   a.rows, a.rows, qend, scale, (u16*)dq, lddq, a.pr, dsum);
     a.po = (float*)at;
     a.pv = (float*)(at + rp_part_bytes(kp, heads, a.krows));
     a.ns = kp.ns;
-#define RP_LDS(NW) bl + 64 * 4
+#define RP_LDS(NW) bl * (1 + (NW)) + 64 * 4
     RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, L, RP_LDS, a, kp.blocks);
 #undef RP_LDS
+    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, nshare), dim3(1024), 0, stream, a.diag, nd, R + BPAD,
+               (long long)B * kp.blocks * kp.ns, bucket, R, nb, heads, share, a.done, dtable, table_bf16);
     if (kp.ns > 1) {
         const dim3 g((unsigned)((a.krows * heads + 3) / 4));
         const int* kend = cu ? cu + B : nullptr;
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, g, dim3(256), 0, stream, a.po, kp.ns, heads, a.krows, a.krows, kend, scale, (u16*)dk,
-                   lddk);
+                   lddk, (const float*)nullptr, (float*)nullptr);
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_sum_kernel, g, dim3(256), 0, stream, a.pv, kp.ns, heads, a.krows, a.krows, kend, 1.f, (u16*)dv,
-                   lddk);
+                   lddk, (const float*)nullptr, (float*)nullptr);
     }
     return 0;
 }
