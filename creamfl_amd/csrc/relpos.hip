@@ -285,12 +285,13 @@ __device__ __forceinline__ void mma_rows(const u16* tile, const Places& at, cons
             s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(t + 4096 * u + (at.row ^ (kk << 5))), f[kk], s[u], 0, 0, 0);
 }
 // out^T += (tile's columns) (w packed to bf16), contraction over the 32 rows of block u; the lane's operand: column 32 dt + (lane & 31), rows
-// in the accumulators' order (a 16-lane group's transposing read takes a [4 rows x 16 columns] block)
+// in the accumulators' order (a 16-lane group's transposing read takes a [4 rows x 16 columns] block).  TWO: w in two bf16 terms
+template <bool TWO = false>
 __device__ __forceinline__ void mma_cols(const u16* tile, const Places& at, int u, const f32x16& w, f32x16 (&out)[2]) {
     const char* t = reinterpret_cast<const char*>(tile);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-        const bf16x8 f = pack_acc(w, kk);
+        const bf16x8 f = pack_acc(w, kk), rest = pack_rest(w, f, kk);
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) {
             const char* a = t + (2 * u + kk) * 2048 + (at.col ^ (dt << 6));
@@ -298,6 +299,7 @@ __device__ __forceinline__ void mma_cols(const u16* tile, const Places& at, int 
             x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
             x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 1024));
             out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v, f, out[dt], 0, 0, 0);
+            if (TWO) out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.v, rest, out[dt], 0, 0, 0);
         }
     }
 }
@@ -763,8 +765,9 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                     mma_cols_apart(Gt[buf], at, u, s[0], dv);
                     mma_cols_apart(Qt[buf], at, u, dp[0], dk);
                 } else {
-                    mma_cols(Gt[buf], at, 0, s[0], dv);
-                    mma_cols(Qt[buf], at, 0, dp[0], dk);
+                    // (at most 32 queries: the roundings of few products would show, and they cost nothing)
+                    mma_cols<NB == 1>(Gt[buf], at, 0, s[0], dv);
+                    mma_cols<NB == 1>(Qt[buf], at, 0, dp[0], dk);
                 }
             }
             if (!more) break;
@@ -808,6 +811,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
 // ---- backward of texts of at most 32 tokens: everything in one kernel, a wave per (text, head).  The rows come straight from memory as
 // operands; K, Q and dO pass through LDS for the products that contract over rows.  D is summed from p and dp themselves, so the
 // rounding of o plays no part; P and ds are taken as two bf16 terms: few products, and waiting for memory bounds this kernel.  The bias gradient's diagonals go to memory as they are: part [heads][B][64], place d + 32.
+// The log-sum is taken off the score as the forward formed it: a row of one key has p = 1 and ds = 0 to the bit.
 // 256 packed captions of 8 to 32 tokens, 12 heads: @B32@ us, against @B32OLD@ with the kernels for long texts.
 __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     __shared__ __attribute__((aligned(16))) u16 Kt[32 * TP], Qt[32 * TP], Gt[32 * TP];
@@ -861,7 +865,7 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     for (int r = 0; r < 16; ++r) {
         const int kr = (r & 3) + 8 * (r >> 2);
         const bool ok = (bits >> (kr + 4 * half)) & 1;
-        const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bl[31 + 4 * half - x + kr] - lse)) : 0.f;
+        const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bl[31 + 4 * half - x + kr]) - lse) : 0.f;
         s[r] = p;
         D = fmaf(p, dp[r], D);
     }
@@ -911,7 +915,7 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const int i = acc_r(r, lane);
-        const float p = keep ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bl[31 + x - i] - ls[i])) : 0.f;
+        const float p = keep ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bl[31 + x - i]) - ls[i]) : 0.f;
         s[r] = p;
         dp[r] = keep ? p * (dp[r] - Ds[i]) : 0.f;
     }

@@ -77,7 +77,7 @@ def keep_flags(seed, p, n):
 def relpos_attention_text(q, k, v, table, buckets, keep=None, scale=0.125, do=None):
     """One text: q [Lq, heads, 64], k, v [Lk, heads, 64], table [nb, heads], buckets [2 R + 1], keep [Lk] flags.  Returns {name: (value,
     bound)} for o and, with do [Lq, heads, 64], dq, dk, dv and (in the bound without the output's own rounding) dtable.
-    Bounds count: p and ds rounded to bf16 before they meet v, k, q, do; o rounded before D = do . o is formed; outputs rounded."""
+    Bounds count: p and ds rounded to bf16 before they meet v, k, q, do; o rounded before D = do . o is formed (but for dtable); outputs rounded."""
     q, k, v, table = (t.detach().cpu().double() for t in (q, k, v, table))
     buckets = buckets.detach().cpu().long()
     lq, heads, hd = q.shape
@@ -91,7 +91,7 @@ def relpos_attention_text(q, k, v, table, buckets, keep=None, scale=0.125, do=No
     none = not bool(keep.any())
     p = torch.zeros_like(s) if none else torch.softmax(s, 2)
     # a score's 32-bit error moves p by its size: products of 64 terms, the bias, the log-sum
-    es = 80 * U32 * (scale * qh.abs() @ kh.abs().transpose(1, 2) + table.abs().max() + torch.where(keep[None, None], s, torch.zeros_like(s)).abs() + 8)
+    es = 80 * U32 * (abs(scale) * qh.abs() @ kh.abs().transpose(1, 2) + table.abs().max() + torch.where(keep[None, None], s, torch.zeros_like(s)).abs() + 8)
     ep = p * (4 * es + 1e-6)
     o = p @ vh
     eo = (U16 * p + ep) @ vh.abs()
@@ -110,11 +110,14 @@ def relpos_attention_text(q, k, v, table, buckets, keep=None, scale=0.125, do=No
     eds = ep * (dp - D).abs() + p * (edp + eD)             # of ds in 32 bits
     er = eds + U16 * (ds.abs() + eds)                      # ... and rounded to bf16
     dq, dk, dv = scale * ds @ kh, scale * ds.transpose(1, 2) @ qh, p.transpose(1, 2) @ g
-    edq, edk, edv = scale * er @ kh.abs(), scale * er.transpose(1, 2) @ qh.abs(), (U16 * p + ep).transpose(1, 2) @ g.abs()
+    edq, edk, edv = abs(scale) * er @ kh.abs(), abs(scale) * er.transpose(1, 2) @ qh.abs(), (U16 * p + ep).transpose(1, 2) @ g.abs()
     for name, t, e in (('dq', dq, edq), ('dk', dk, edk), ('dv', dv, edv)):
         res[name] = (rows(t), rows(1.02 * e + U16 * t.abs() + 1e-30))
     dt, et = torch.zeros(nb, heads, dtype=torch.float64), torch.zeros(nb, heads, dtype=torch.float64)
     dt.index_add_(0, which.reshape(-1), ds.permute(1, 2, 0).reshape(-1, heads))
+    # the table's gradient adds up a whole row's error of D, so its D is held in 32 bits: sums of p dp over the row, and of ds with the rounded D
+    eD = (p * edp + ep * dp.abs() + 80 * U32 * p * (dp.abs() + D.abs() + eD)).sum(2, keepdim=True)
+    eds = ep * (dp - D).abs() + p * (edp + eD)
     et.index_add_(0, which.reshape(-1), (eds + 64 * U32 * ds.abs()).permute(1, 2, 0).reshape(-1, heads))
     res['dtable'] = (dt, et)
     return res

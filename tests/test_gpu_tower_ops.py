@@ -255,12 +255,30 @@ def test_relpos_attention_tables(dev, nb, far, dtype):
     check_padded(dev, attn_inputs(nb + far, 2, 170, 2, nb, far, dtype), None)
 
 
+@pytest.mark.parametrize('B,L,heads,cut', [(3, 1, 2, False), (64, 1, 12, False), (3, 9, 2, True), (2, 32, 1, True)])
+def test_relpos_attention_of_one_key_has_no_score_gradient(dev, B, L, heads, cut):
+    """p = 1 in a row of one key: the gradients of q, k and the table are zero to the bit, in every kernel for short texts."""
+    from creamfl_amd import ops
+    t = attn_inputs(B * 31 + L, B, L, heads)
+    qkv, table = t['qkv'].to(dev).requires_grad_(True), t['table'].to(dev).requires_grad_(True)
+    mask = None
+    if cut:
+        mask = torch.zeros(B, L, dtype=torch.bool, device=dev)
+        mask[torch.arange(B), torch.arange(B) * 5 % L] = True
+    o = ops.relpos_attention(qkv, table, t['buckets'].to(dev), heads, key_mask=mask)
+    dqkv, dtable = torch.autograd.grad(o, [qkv, table], t['do'].to(dev))
+    H = heads * 64
+    assert not dqkv[:, :, :2 * H].any() and not dtable.any()
+    check_padded(dev, t, None if mask is None else mask.cpu())
+
+
 def test_relpos_attention_scale_and_maps(dev):
     t = attn_inputs(5, 2, 70, 2, 32, 128)
     t['table'] = t['table'] * 8                            # (a strong bias: far distances win)
     check_padded(dev, t, None, scale=0.5)
     t['buckets'] = torch.zeros(1, dtype=torch.int32)       # R = 0: one bucket for every distance, the bias cancels
     check_padded(dev, t, None, scale=0.03)
+    check_padded(dev, t, None, scale=-0.2)
     t['buckets'] = torch.randint(-3, 40, (41,), generator=torch.Generator().manual_seed(1)).to(torch.int32)    # any map; ends are clipped
     check_padded(dev, t, None)
 
