@@ -31,7 +31,7 @@ typedef unsigned int u32;
 typedef unsigned long long u64;
 
 constexpr int TP = 72;                      // LDS row pitch in bf16 of the kernel for short texts (144 bytes: spread over the banks)
-constexpr int BPAD = 96;                    // the bias vector reaches this far beyond +-R: a tile of 32 x 64 that touches |d| < R needs no clipping
+constexpr int BPAD = 192;                   // the bias vector reaches this far beyond +-R: a tile of 128 x 64 that touches |d| < R needs no clipping
 constexpr int MAXR = 512;                   // largest R (LDS)
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -504,6 +504,7 @@ __device__ __forceinline__ float down_one_round(float v) {     // (lane 0's goes
 // holds e = 32 + 16 u - i; what has left at lane 0 is the difference to the same sums with the lanes in a ring: at lane i >= 49 e = 96 + 16 u - i.
 // dst: the place of e = 0, places fall with e.  32 instructions for 16 rows of 64 lanes, against 80 with the zeros below.
 __device__ __forceinline__ void diag_add_apart(const f32x16& v, float* dst, int u, int lane) {
+#pragma clang fp contract(off)                                  // (a fused product would take the shift out of the addition)
     float a = v[15], b = v[15];
 #pragma unroll
     for (int r = 14; r >= 0; --r) { a = down_one(a) + v[r]; b = down_one_round(b) + v[r]; }
@@ -705,80 +706,81 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                 dr = in ? -dp_[q0 + threadIdx.x] : 0.f;
             }
         };
-        int buf = 0;
-        fetch(part.from, 0);
-        for (int q0 = part.from; ; ) {
-            const bool more = q0 + KT < part.to;
-            if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
-            wait_copies();
-            TileQ::landed(Qt[buf], low_bits(min(KT, part.to - q0)), w, lane);
-            TileQ::landed(Gt[buf], low_bits(min(KT, part.to - q0)), w, lane);
-            __syncthreads();
-            if (NB > 1 && more) fetch(q0 + KT, buf ^ 1);
-            const int d0 = k0 - q0;
-            const bool near = tile_near(a.R, d0, KT, true);
-            // the lane's first query in the tile, and how its registers go on from it
-            const int i0 = APART ? 32 - 32 * (lane >> 5) : 4 * (lane >> 5);
-            const auto query = [](int u, int r) { return APART ? 16 * u + r : 32 * u + (r & 3) + 8 * (r >> 2); };
-            const float* bp = live ? bl + mid + (near ? d0 : 0) + (lane & 31) - i0 : gone + KT - 1;
-            const float c = live ? far_bias(bl, a.R, near ? 0 : d0) : -INFINITY;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                f32x16 s[1], dp[1], nl;
-                zero16(s[0]);
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(&ls[buf][i0 + query(u, 4 * g)]);
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(&ds[buf][i0 + query(u, 4 * g)]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) { nl[4 * g + j] = x[j]; dp[0][4 * g + j] = y[j]; }
-                }
-                if constexpr (APART) {
-                    mma_rows_apart(Qt[buf], at, u, kf, s[0]);
-                    mma_rows_apart(Gt[buf], at, u, vf, dp[0]);
-                } else {
-                    mma_rows<1>(Qt[buf], at, kf, s);
-                    mma_rows<1>(Gt[buf], at, vf, dp);
-                }
-                if (near) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) nl[r] += bp[-query(u, r)];
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) nl[r] += c;
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], a.scale2, nl[r]));
-                    dp[0][r] *= s[0][r];
-                }
-                if (near) {
-                    if constexpr (APART) diag_add_apart(dp[0], mine + d0, u, lane);
-                    else diag_add(dp[0], mine + d0, lane);
-                } else {
-                    float x0 = 0.f, x1 = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; r += 2) { x0 += dp[0][r]; x1 += dp[0][r + 1]; }
-                    if (d0 > 0) far_hi += x0 + x1; else far_lo += x0 + x1;
-                }
-                if constexpr (APART) {
-                    mma_cols_apart(Gt[buf], at, u, s[0], dv);
-                    mma_cols_apart(Qt[buf], at, u, dp[0], dk);
-                } else {
-                    // (at most 32 queries: the roundings of few products would show, and they cost nothing)
-                    mma_cols<NB == 1>(Gt[buf], at, 0, s[0], dv);
-                    mma_cols<NB == 1>(Qt[buf], at, 0, dp[0], dk);
-                }
-            }
-            if (!more) break;
-            q0 += KT;
-            if (NB > 1) {
-                buf ^= 1;
-            } else {
+        int buf = 0, q0 = part.from;
+        fetch(q0, 0);
+        // the lane's first query in the tile, and how its registers go on from it
+        const int i0 = APART ? 32 - 32 * (lane >> 5) : 4 * (lane >> 5);
+        const auto query = [](int u, int r) { return APART ? 16 * u + r : 32 * u + (r & 3) + 8 * (r >> 2); };
+        // the tiles up to query `until`, all near or all far for the whole workgroup, far ones with the bias c; `sum`: theirs of ds
+        const auto tiles = [&](auto near_, int until, float c, float& sum) {
+            constexpr bool near = decltype(near_)::value;
+            for (; q0 < until; q0 += KT) {
+                const bool more = q0 + KT < part.to;
+                if (threadIdx.x < KT) { ls[buf][threadIdx.x] = lr; ds[buf][threadIdx.x] = dr; }
+                wait_copies();
+                TileQ::landed(Qt[buf], low_bits(min(KT, part.to - q0)), w, lane);
+                TileQ::landed(Gt[buf], low_bits(min(KT, part.to - q0)), w, lane);
                 __syncthreads();
-                fetch(q0, 0);
+                if (NB > 1 && more) fetch(q0 + KT, buf ^ 1);
+                const int d0 = k0 - q0;
+                const float* bp = live ? bl + mid + d0 + (lane & 31) - i0 : gone + KT - 1;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    f32x16 s[1], dp[1], nl;
+                    zero16(s[0]);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(&ls[buf][i0 + query(u, 4 * g)]);
+                        const f32x4 y = *reinterpret_cast<const f32x4*>(&ds[buf][i0 + query(u, 4 * g)]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { nl[4 * g + j] = x[j]; dp[0][4 * g + j] = y[j]; }
+                    }
+                    if constexpr (APART) {
+                        mma_rows_apart(Qt[buf], at, u, kf, s[0]);
+                        mma_rows_apart(Gt[buf], at, u, vf, dp[0]);
+                    } else {
+                        mma_rows<1>(Qt[buf], at, kf, s);
+                        mma_rows<1>(Gt[buf], at, vf, dp);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        nl[r] += near ? bp[-query(u, r)] : c;
+                        s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], a.scale2, nl[r]));
+                        dp[0][r] *= s[0][r];
+                    }
+                    if constexpr (!near) {
+                        float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; r += 2) { x0 += dp[0][r]; x1 += dp[0][r + 1]; }
+                        sum += x0 + x1;
+                    } else if constexpr (APART) {
+                        diag_add_apart(dp[0], mine + d0, u, lane);
+                    } else {
+                        diag_add(dp[0], mine + d0, lane);
+                    }
+                    if constexpr (APART) {
+                        mma_cols_apart(Gt[buf], at, u, s[0], dv);
+                        mma_cols_apart(Qt[buf], at, u, dp[0], dk);
+                    } else {
+                        // (at most 32 queries: the roundings of few products would show, and they cost nothing)
+                        mma_cols<NB == 1>(Gt[buf], at, 0, s[0], dv);
+                        mma_cols<NB == 1>(Qt[buf], at, 0, dp[0], dk);
+                    }
+                }
+                if (NB > 1) {
+                    buf ^= 1;
+                } else if (more) {
+                    __syncthreads();
+                    fetch(q0 + KT, 0);
+                }
             }
-        }
+        };
+        // queries so far before the workgroup's keys that every distance is R or more, then the near ones, then those far behind
+        const int first = kb * NW * 32, before = first - a.R - KT + 2, behind = first + NW * 32 - 1 + a.R;
+        const float clo = live ? far_bias(bl, a.R, -1) : -INFINITY, chi = live ? far_bias(bl, a.R, 1) : -INFINITY;
+        tiles(std::false_type{}, min(before, part.to), chi, far_hi);
+        tiles(std::true_type{}, min(behind, part.to), 0.f, far_hi);
+        tiles(std::false_type{}, part.to, clo, far_lo);
     }
     // the workgroup's sums per distance
     far_lo = wave_sum(far_lo);
