@@ -379,7 +379,6 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     if (a.cu && !a.Lq && qb == 0) clear_rest<NT>(a, t, b, h, sp, a.out, nullptr, a.ldo);
     if (qb * NW * 32 >= t.lq) return;
     const Part part = part_of(sp, a.ns, t.lk, KT);
-    fill_bias<NT>(a, h, bl, -(t.lq | (NW * 32 - 1)), t.lk | (KT - 1));     // (rows past the end are computed with as well)
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
     const u16* kp = a.k + t.k0 * a.ldk + h * 64;
     const u16* vp = a.v + t.k0 * a.ldk + h * 64;
@@ -391,7 +390,7 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     // l and o are relative to 2^m.  m follows the running maximum lazily: only when a score passes it by more than 8 are l and o brought
     // to the new one (p then stays below 2^8; the division by l at the end cancels whatever m is)
     float m = 0.f, l0 = 0.f, l1 = 0.f;
-    bool first = true;
+    bool first = true, filled = false;
     for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
         keys.chunk(c0);
         u64 left = keys.alive;
@@ -403,8 +402,10 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
             Tile<NW, KT>::copy(kp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Kt[to], w, lane);
             Tile<NW, KT>::copy(vp + (long long)k0 * a.ldk, (u32)a.ldk, t.lk - k0, Vt[to], w, lane);
         };
-        __syncthreads();                                       // (the tiles' last readers, the bias vector)
+        __syncthreads();                                       // (the tiles' last readers)
         copy(cur, 0);
+        if (!filled) fill_bias<NT>(a, h, bl, -(t.lq | (NW * 32 - 1)), t.lk | (KT - 1));      // (rows past the end are computed with as well)
+        filled = true;                                         // (its loads travel with the first tile's)
         const auto step = [&](auto buf_) {                     // one tile; whether it was the last
             constexpr int buf = decltype(buf_)::value;
             const int d0 = c0 + cur * KT - q0, nxt = next_tile(left);
@@ -672,7 +673,6 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     }
     const Part part = part_of(sp, a.ns, t.lq, KT);
     const int dlo = max(-(t.lq | (KT - 1)), -mid), dhi = min(t.lk | (NW * 32 - 1), mid);      // (rows past the end are computed with as well)
-    fill_bias<NT>(a, h, bl, dlo, dhi);
     for (int c = 0; c < NW; ++c)
         for (int d = dlo + (int)threadIdx.x; d <= dhi; d += NT) dg[c * nd + d + mid] = 0.f;
     float far_lo = 0.f, far_hi = 0.f;
@@ -708,6 +708,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
         };
         int buf = 0, q0 = part.from;
         fetch(q0, 0);
+        fill_bias<NT>(a, h, bl, dlo, dhi);                     // (its loads travel with the first tile's)
+        __syncthreads();
         // the lane's first query in the tile, and how its registers go on from it
         const int i0 = APART ? 32 - 32 * (lane >> 5) : 4 * (lane >> 5);
         const auto query = [](int u, int r) { return APART ? 16 * u + r : 32 * u + (r & 3) + 8 * (r >> 2); };
