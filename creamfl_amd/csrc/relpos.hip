@@ -1,6 +1,6 @@
 // relpos.hip -- self-attention with a learned relative position bias by buckets, head dim 64, any length; forward and backward.
 //
-//   s_ij = scale q_i . k_j + table[bucket[clip(j - i, -R, R) + R]][h]   (keys that the mask drops: -inf),  p = softmax_j(s),  o_i = sum_j p_ij v_j
+//   s_ij = scale q_i . k_j + table[bucket[clip(j - i, -R, R) + R]][h]   (keys that the mask drops, or whose bias is -1e30 or less: -inf),  p = softmax_j(s),  o_i = sum_j p_ij v_j
 //   backward: D_i = sum_d do_id o_id,  ds_ij = p_ij (do_i . v_j - D_i),  dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,
 //             dk_j = scale sum_i ds_ij q_i,  dtable[b][h] = sum of ds_ij over all texts and pairs (i, j) whose bucket is b
 //   A row whose mask leaves no key has o = 0 and no gradient.
@@ -248,6 +248,8 @@ __device__ __forceinline__ Part part_of(int sp, int ns, int n, int tile) {
     return Part{min(sp * per, n), min((sp + 1) * per, n)};
 }
 
+// the bias in units of log2; -1e30 and less (a type's lowest value, -inf) drops the key, as a mask does
+__device__ __forceinline__ float bias_of(float t) { return t > -1e30f || t != t ? t * LOG2E : -INFINITY; }
 // head h's bias over the distances lo .. hi, in units of log2: bl[d + R + BPAD].  Two dependent loads a distance; those of four distances
 // travel together.
 template <int NT>
@@ -264,7 +266,7 @@ __device__ __forceinline__ void fill_bias(const RpArgs& a, int h, float* bl, int
             t[i] = a.table_bf16 ? __uint_as_float((u32)((const u16*)a.table)[at] << 16) : ((const float*)a.table)[at];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (d + i * NT <= last) bl[d + i * NT + mid] = t[i] * LOG2E;
+        for (int i = 0; i < 4; ++i) if (d + i * NT <= last) bl[d + i * NT + mid] = bias_of(t[i]);
     }
 }
 // A tile of 32 rows that a wave owns against `n` staged ones, d0 = (first key) - (first query): whether it touches |d| < R
@@ -388,9 +390,10 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     f32x16 o[2];
     zero16(o[0]); zero16(o[1]);
     // l and o are relative to 2^m.  m follows the running maximum lazily: only when a score passes it by more than 8 are l and o brought
-    // to the new one (p then stays below 2^8; the division by l at the end cancels whatever m is)
+    // to the new one (p then stays below 2^8; the division by l at the end cancels whatever m is).  seen: the row has met a key; one whose
+    // tiles so far were all dropped by the bias waits
     float m = 0.f, l0 = 0.f, l1 = 0.f;
-    bool first = true, filled = false;
+    bool first = true, seen = false, filled = false;
     for (int c0 = part.from; c0 < part.to; c0 += 64 * KT) {
         keys.chunk(c0);
         u64 left = keys.alive;
@@ -441,14 +444,16 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
             top = half_max(top);
-            if (first || __any(top > 8.f)) {
-                const float by = first ? top : fmaxf(top, 0.f), shrink = __builtin_amdgcn_exp2f(-by);
+            const bool met = top > -INFINITY;
+            if (__any(top > 8.f || (met && !seen))) {
+                const float by = !met ? 0.f : seen ? fmaxf(top, 0.f) : top, shrink = seen ? __builtin_amdgcn_exp2f(-by) : 1.f;
                 if (!first) {
                     l0 *= shrink; l1 *= shrink;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) { o[0][r] *= shrink; o[1][r] *= shrink; }
                 }
                 first = false;
+                seen |= met;
                 m += by;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -479,15 +484,16 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
     }
     float l = l0 + l1;
     l += __shfl_xor(l, 32, 64);
+    const bool none = !seen && l == 0.f;                       // (not so where NaN scores made l one)
     const int row = q0 + (lane & 31);
     if (row >= t.lq) return;
     if (a.ns > 1) {
         const long long to = ((long long)sp * a.heads + h) * a.rows + t.q0 + row;
         store_part(o, a.po + to * 64, lane);
-        if (lane < 32) { a.pm[2 * to] = first ? -INFINITY : m; a.pm[2 * to + 1] = l; }
+        if (lane < 32) { a.pm[2 * to] = none ? -INFINITY : m; a.pm[2 * to + 1] = l; }
     } else {
-        store_row(o, a.out + (t.q0 + row) * a.ldo + h * 64, lane, first ? 0.f : 1.f / l);
-        if (a.lse && lane < 32) a.lse[h * a.rows + t.q0 + row] = first ? INFINITY : m + __builtin_amdgcn_logf(l);
+        store_row(o, a.out + (t.q0 + row) * a.ldo + h * 64, lane, none ? 0.f : 1.f / l);
+        if (a.lse && lane < 32) a.lse[h * a.rows + t.q0 + row] = none ? INFINITY : m + __builtin_amdgcn_logf(l);
     }
 }
 
@@ -845,7 +851,7 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     load_rows(a.q + t.q0 * a.ldq + h * 64, a.ldq, 0, t.lq, lane, qf);
     load_rows(a.dout + t.q0 * a.ldo + h * 64, a.ldo, 0, t.lq, lane, gf);
     const float lse = x < t.lq ? a.lse[h * a.rows + t.q0 + x] : INFINITY;
-    bl[lane] = LOG2E * bias;
+    bl[lane] = bias_of(bias);
     const f32x4 z4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
@@ -871,6 +877,7 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
         const bool ok = (bits >> (kr + 4 * half)) & 1;
         const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, bl[31 + 4 * half - x + kr]) - lse) : 0.f;
         s[r] = p;
+        dp[r] = ok ? dp[r] : 0.f;                              // (a text without a key: 0, whatever its gradient holds)
         D = fmaf(p, dp[r], D);
     }
     D += __shfl_xor(D, 32, 64);

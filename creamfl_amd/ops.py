@@ -2481,8 +2481,9 @@ def _relpos_check(name, q, width_of_q, table, buckets, heads, mask, cu, B, L):
         raise _lib.CreamflHipError(f'{name}: buckets must be an int32 [2 R + 1] tensor on {q.device}, R <= {RELPOS_MAX_DISTANCE} '
                                    '(relpos_buckets)')
     if mask is not None:
-        if not torch.is_tensor(mask) or mask.numel() != B * L or mask.shape[0] != B or mask.device != q.device:
-            raise _lib.CreamflHipError(f'{name}: key_mask must hold [{B}, {L}] flags on {q.device}')
+        if not torch.is_tensor(mask) or mask.numel() != B * L or mask.shape[:1] != (B,) or mask.device != q.device \
+                or mask.is_floating_point():                   # (0 / -inf to be added would read as the opposite)
+            raise _lib.CreamflHipError(f'{name}: key_mask must hold [{B}, {L}] flags (bool or integers) on {q.device}')
         mask = (mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0).reshape(B, L).contiguous()
     if cu is not None and (not torch.is_tensor(cu) or cu.dtype != torch.int32 or cu.device != q.device or not cu.is_contiguous()
                            or cu.dim() != 1 or cu.numel() < 2):
@@ -2502,7 +2503,7 @@ def relpos_attention(qkv, table, buckets, heads, key_mask=None, scale=None):
     """softmax_j(scale q_i . k_j + table[bucket of j - i, head]) V per text and head for a fused projection qkv [B, L, 3H] (Q | K | V along
     the last axis), head dim 64, any length (csrc/relpos.hip).  table: [num_buckets, heads], bf16 or fp32; buckets: `relpos_buckets`, or
     any int32 [2 R + 1] map of the clipped distance; key_mask [B, L] (True = the key takes part; what stands at a dropped key does not
-    matter), scale 1 / 8 by default.  A text without a key gives zeros.  Differentiable in qkv and table (once).  -> [B, L, H] bf16."""
+    matter), scale 1 / 8 by default.  A bias of -1e30 or less drops its keys too; a row without a key gives zeros.  Differentiable in qkv and table (once).  -> [B, L, H] bf16."""
     qkv = _aligned16(_bf16c(qkv, 'qkv'))
     heads = int(heads)
     if qkv.dim() != 3 or qkv.numel() == 0:
@@ -2536,7 +2537,7 @@ def relpos_attention_cls(q, kv, table, buckets, heads, key_mask=None, cu_seqlens
                                    f'got {tuple(q.shape)}, {tuple(kv.shape)}')
     B, L = q.shape[0], kv.shape[0] if packed else kv.shape[1]
     if kv.shape[-1] != 2 * q.shape[1] or (not packed and kv.shape[0] != B) or (packed and (key_mask is not None or max_len is None
-                                                                                         or cu_seqlens.numel() != B + 1)):
+                                                                                         or not torch.is_tensor(cu_seqlens) or cu_seqlens.numel() != B + 1)):
         raise _lib.CreamflHipError('relpos_attention_cls: q, kv, key_mask and cu_seqlens do not belong together')
     table, buckets, mask = _relpos_check('relpos_attention_cls', q, 1, table, buckets, heads, key_mask, cu_seqlens, B, L)
     Lk = min(max(int(max_len), 1), L) if packed else L

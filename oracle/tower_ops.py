@@ -86,12 +86,15 @@ def relpos_attention_text(q, k, v, table, buckets, keep=None, scale=0.125, do=No
     k, v = (torch.where(keep[:, None, None], t, torch.zeros_like(t)) for t in (k, v))
     which = buckets[(torch.arange(lk)[None] - torch.arange(lq)[:, None]).clamp(-R, R) + R].clamp(0, nb - 1)      # [Lq, Lk]
     qh, kh, vh = (t.permute(1, 0, 2) for t in (q, k, v))                                        # [heads, L, 64]
+    drop = (table <= -1e30)[which].permute(2, 0, 1)         # a bias that low drops the key as the mask does
+    table = torch.where(table <= -1e30, torch.zeros_like(table), table)
     s = scale * qh @ kh.transpose(1, 2) + table[which].permute(2, 0, 1)
-    s = torch.where(keep[None, None], s, torch.full_like(s, -np.inf))
-    none = not bool(keep.any())
-    p = torch.zeros_like(s) if none else torch.softmax(s, 2)
+    s = torch.where(keep[None, None] & ~drop, s, torch.full_like(s, -np.inf))
+    p = torch.softmax(s, 2)
+    p = torch.where(torch.isnan(p), torch.zeros_like(p), p) # a row without a key
+    s = torch.where(torch.isinf(s), torch.zeros_like(s), s)
     # a score's 32-bit error moves p by its size: products of 64 terms, the bias, the log-sum
-    es = 80 * U32 * (abs(scale) * qh.abs() @ kh.abs().transpose(1, 2) + table.abs().max() + torch.where(keep[None, None], s, torch.zeros_like(s)).abs() + 8)
+    es = 80 * U32 * (abs(scale) * qh.abs() @ kh.abs().transpose(1, 2) + table.abs().max() + s.abs() + 8)
     ep = p * (4 * es + 1e-6)
     o = p @ vh
     eo = (U16 * p + ep) @ vh.abs()

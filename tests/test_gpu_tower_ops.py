@@ -272,6 +272,40 @@ def test_relpos_attention_of_one_key_has_no_score_gradient(dev, B, L, heads, cut
     check_padded(dev, t, None if mask is None else mask.cpu())
 
 
+@pytest.mark.parametrize('B,L,heads', [(3, 20, 2), (2, 33, 2), (2, 200, 3), (1, 900, 1), (40, 300, 8)])
+@pytest.mark.parametrize('low', [-float('inf'), torch.finfo(torch.float32).min, -1e30])
+def test_relpos_attention_bias_that_drops_keys(dev, B, L, heads, low):
+    """A window by the bias: far buckets at -inf or the type's lowest value, so that a query's first tiles leave it nothing; scores far below zero in
+    what is left (2^-s would underflow if the waiting rows' maximum stayed at zero); one head without any key; NaN gradients in a text that the mask
+    empties."""
+    t = attn_inputs(B * 3 + L, B, L, heads, 32, 16)
+    t['table'] = t['table'] - 300.0
+    far = t['buckets'][[0, -1]].long()
+    t['table'][far] = low
+    t['table'][t['buckets'][t['buckets'].numel() // 2 + 9].long()] = low
+    if heads > 1:
+        t['table'][:, 1] = low
+    mask = torch.ones(B, L, dtype=torch.bool)
+    mask[:, 4:7] = False
+    if B > 1:
+        mask[1] = False
+    check_padded(dev, t, mask)
+
+
+def test_relpos_attention_nan_gradient_of_a_text_without_keys(dev):
+    from creamfl_amd import ops
+    for L in (20, 70):
+        t = attn_inputs(L, 2, L, 2)
+        mask = torch.ones(2, L, dtype=torch.bool, device=dev)
+        mask[0] = False
+        qkv, table = t['qkv'].to(dev).requires_grad_(True), t['table'].to(dev).requires_grad_(True)
+        do = t['do'].to(dev)
+        want = torch.autograd.grad(ops.relpos_attention(qkv, table, t['buckets'].to(dev), 2, key_mask=mask), [qkv, table], do)
+        do[0] = float('nan')
+        got = torch.autograd.grad(ops.relpos_attention(qkv, table, t['buckets'].to(dev), 2, key_mask=mask), [qkv, table], do)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and not got[0][0].any()
+
+
 def test_relpos_attention_scale_and_maps(dev):
     t = attn_inputs(5, 2, 70, 2, 32, 128)
     t['table'] = t['table'] * 8                            # (a strong bias: far distances win)
@@ -364,7 +398,7 @@ def test_relpos_attention_views_and_refusals(dev):
     assert torch.equal(ops.relpos_attention(qkv, table, b, 2, key_mask=m), want)
     ok = dict(qkv=qkv, table=table, buckets=b, heads=2)
     for kw in (dict(heads=3), dict(heads=0), dict(table=table[:, :1]), dict(table=table[0]), dict(buckets=b[:-1]), dict(buckets=b.long()),
-               dict(buckets=b.cpu()), dict(qkv=qkv[0]), dict(key_mask=m[:1]), dict(key_mask=m[:, :-1]), dict(key_mask=m.cpu()), dict(qkv=qkv[:0]),
+               dict(buckets=b.cpu()), dict(qkv=qkv[0]), dict(key_mask=m[:1]), dict(key_mask=m[:, :-1]), dict(key_mask=m.cpu()), dict(key_mask=m.float()), dict(qkv=qkv[:0]),
                dict(table=table.cpu())):
         with pytest.raises(_lib.CreamflHipError):
             ops.relpos_attention(**{**ok, **kw})
@@ -376,7 +410,7 @@ def test_relpos_attention_views_and_refusals(dev):
             ops.relpos_attention_varlen(**{**ok, **kw})
     q, kv = qkv[:, 0, :128].contiguous(), qkv[..., 128:].contiguous()
     ok = dict(q=q, kv=kv, table=table, buckets=b, heads=2)
-    for kw in (dict(q=q[:1]), dict(kv=kv[..., :128]), dict(kv=kv[0]), dict(cu_seqlens=cu), dict(kv=kv.view(40, 256), cu_seqlens=cu),
+    for kw in (dict(q=q[:1]), dict(kv=kv.view(40, 256), cu_seqlens=[0, 20, 40], max_len=20), dict(kv=kv[..., :128]), dict(kv=kv[0]), dict(cu_seqlens=cu), dict(kv=kv.view(40, 256), cu_seqlens=cu),
                dict(kv=kv.view(40, 256), cu_seqlens=cu, max_len=20, key_mask=m)):
         with pytest.raises(_lib.CreamflHipError):
             ops.relpos_attention_cls(**{**ok, **kw})
