@@ -125,22 +125,38 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_stats_kernel(const E* __restrict_
     }
 }
 
-// merge of the chunks' pairs: mean and 1 / sqrt(var + eps) of every group of sample n into LDS
+// merge of the chunks' pairs: mean and 1 / sqrt(var + eps) of every group of sample n into mu, rs.  Thread t of T takes every T-th group, L lanes
+// of a wave to a group, their partial merges by the same formula.
+template <int T, int L>
 __device__ __forceinline__ void gn_merge(const float* __restrict__ part, int n, int chunks, int rows, int HW, int cpg, int G, float eps,
                                          float* mu, float* rs) {
-    for (int g = threadIdx.x; g < G; g += GN_T) {
-        const float* p = part + ((long long)n * chunks * G + g) * 2;
+    const int l = threadIdx.x % L;
+    for (int g0 = 0; g0 < G; g0 += T / L) {
+        const int g = g0 + threadIdx.x / L;
+        const float* p = part + ((long long)n * chunks * G + min(g, G - 1)) * 2;
         float sum = 0.f;
-        for (int k = 0; k < chunks; ++k) sum = fmaf((float)min(rows, HW - k * rows), p[(long long)k * G * 2], sum);
+        for (int k = l; k < chunks; k += L) sum = fmaf((float)min(rows, HW - k * rows), p[(long long)k * G * 2], sum);
+        for (int o = L >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         const float mean = sum / (float)HW;
         float m2 = 0.f;
-        for (int k = 0; k < chunks; ++k) {
+        for (int k = l; k < chunks; k += L) {
             const float d = p[(long long)k * G * 2] - mean;
             m2 += fmaf((float)(min(rows, HW - k * rows) * cpg) * d, d, p[(long long)k * G * 2 + 1]);
         }
-        mu[g] = mean;
-        rs[g] = 1.f / sqrtf(m2 / ((float)HW * (float)cpg) + eps);
+        for (int o = L >> 1; o > 0; o >>= 1) m2 += __shfl_xor(m2, o, 64);
+        if (g < G && l == 0) {
+            mu[g] = mean;
+            rs[g] = 1.f / sqrtf(m2 / ((float)HW * (float)cpg) + eps);
+        }
     }
+}
+// More than GN_MERGE chunks: every workgroup of the second pass merging them for itself would cost their number squared; one small launch does it
+// once, a workgroup a sample.  stats: [2][N][G].
+constexpr int GN_MERGE = 64;
+__global__ __launch_bounds__(1024) void cfl_gn_merge_kernel(const float* __restrict__ part, int chunks, int rows, int HW, int cpg, int G, float eps,
+                                                            float* __restrict__ stats) {
+    float* mu = stats + (long long)blockIdx.x * G;
+    gn_merge<1024, 64>(part, blockIdx.x, chunks, rows, HW, cpg, G, eps, mu, mu + (long long)gridDim.x * G);
 }
 
 // ---- forward, pass 2: y = act(xh gamma + beta (+ res)); the first chunk keeps mean / rstd for the backward
@@ -148,11 +164,16 @@ template <class E, int ACT, bool RES>
 __global__ __launch_bounds__(GN_T) void cfl_gn_apply_kernel(const E* __restrict__ x, const E* __restrict__ res, const float* __restrict__ gamma,
                                                             const float* __restrict__ beta, const float* __restrict__ part, int HW, int C,
                                                             int G, int rows, float eps, E* __restrict__ y, float* __restrict__ mean,
-                                                            float* __restrict__ rstd) {
+                                                            float* __restrict__ rstd, const float* __restrict__ stats) {
     __shared__ float mu[GN_MAXC], rs[GN_MAXC];
     const GMap m = gn_map(C);
     const int n = blockIdx.y, cpg = C / G;
-    gn_merge(part, n, gridDim.x, rows, HW, cpg, G, eps, mu, rs);
+    if (stats) {
+        const float* p = stats + (long long)n * G;
+        for (int g = threadIdx.x; g < G; g += GN_T) { mu[g] = p[g]; rs[g] = p[(long long)gridDim.y * G + g]; }
+    } else {
+        gn_merge<GN_T, 1>(part, n, gridDim.x, rows, HW, cpg, G, eps, mu, rs);
+    }
     __syncthreads();
     if (blockIdx.x == 0 && mean) for (int g = threadIdx.x; g < G; g += GN_T) { mean[(long long)n * G + g] = mu[g]; rstd[(long long)n * G + g] = rs[g]; }
     if (!m.active) return;
@@ -262,20 +283,30 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_bwd_reduce_kernel(const E* __rest
     }
 }
 
+// the chunks' group sums of a sample added up, where they are many (as cfl_gn_merge_kernel): to the place of its chunk 0.  grid = (G, N)
+__global__ __launch_bounds__(64) void cfl_gn_bwd_merge_kernel(float* __restrict__ pg, int chunks, int G) {
+    float* p = pg + ((long long)blockIdx.y * chunks * G + blockIdx.x) * 2;
+    float a = 0.f, b = 0.f;
+    for (int k = threadIdx.x; k < chunks; k += 64) { a += p[(long long)k * G * 2]; b += p[(long long)k * G * 2 + 1]; }
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if (threadIdx.x == 0) { p[0] = a; p[1] = b; }
+}
+
 // ---- backward, pass 2: dx (and dz = dres)
 template <class E, int ACT, bool RES>
 __global__ __launch_bounds__(GN_T) void cfl_gn_bwd_apply_kernel(const E* __restrict__ x, const E* __restrict__ dy, const E* __restrict__ dy2,
                                                                 const E* __restrict__ res, const float* __restrict__ gamma,
                                                                 const float* __restrict__ beta, const float* __restrict__ mean,
                                                                 const float* __restrict__ rstd, const float* __restrict__ pg, int HW, int C,
-                                                                int G, int rows, E* __restrict__ dx, E* __restrict__ dres) {
+                                                                int G, int rows, int sums, E* __restrict__ dx, E* __restrict__ dres) {
     __shared__ float s1[GN_MAXC], s2[GN_MAXC];
     const GMap m = gn_map(C);
     const int n = blockIdx.y, cpg = C / G, C8 = C >> 3;
     for (int g = threadIdx.x; g < G; g += GN_T) {
         const float* p = pg + ((long long)n * gridDim.x * G + g) * 2;
         float a = 0.f, b = 0.f;
-        for (int k = 0; k < (int)gridDim.x; ++k) { a += p[(long long)k * G * 2]; b += p[(long long)k * G * 2 + 1]; }
+        for (int k = 0; k < sums; ++k) { a += p[(long long)k * G * 2]; b += p[(long long)k * G * 2 + 1]; }
         const float inv = 1.f / ((float)HW * (float)cpg);
         s1[g] = a * inv; s2[g] = b * inv;
     }
@@ -821,7 +852,7 @@ inline Plan gn_plan(int N, int HW, int C, int G, int size, bool bwd) {
     return best;
 }
 
-// rows per chunk: one register load per thread (RPT rows), the chunk count bounded so that its merge stays short
+// rows per chunk: one register load per thread (RPT rows)
 inline int gn_rows(int HW, int C) { return GN_T / (C >> 3) * GN_RPT; }
 inline bool gn_bad(const void* x, int N, int HW, int C, int G) { return !x || N < 1 || HW < 1 || C < 1 || G < 1 || C % G != 0; }
 inline bool gn_limit(int N, int HW, int C) { return C % 8 != 0 || C > GN_MAXC || N > 65535; }
@@ -833,7 +864,7 @@ extern "C" {
 size_t cfl_gn_ws_bytes(int N, int HW, int C, int G) {
     if (N < 1 || HW < 1 || C < 8 || G < 1 || C % G || gn_limit(N, HW, C)) return 0;
     const size_t chunks = cfl_cdiv(HW, gn_rows(HW, C));        // (also enough for the one-workgroup kernels: [N][2][C])
-    return cfl_align256((size_t)N * chunks * G * 2 * 4) + cfl_align256((size_t)N * chunks * C * 2 * 4);
+    return cfl_align256((size_t)N * chunks * G * 2 * 4) + cfl_align256((size_t)N * chunks * C * 2 * 4);      // (second: also the merged [2][N][G])
 }
 
 #define GN_SWITCH(E, LAUNCH)                                                                            \
@@ -884,16 +915,18 @@ int cfl_gn_fwd(const void* x, const void* res, const float* gamma, const float* 
     const int rows = gn_rows(HW, C);
     const dim3 grid(cfl_cdiv(HW, rows), N);
     float* part = (float*)ws;
+    float* stats = (int)grid.x > GN_MERGE ? (float*)((char*)ws + cfl_align256((size_t)N * grid.x * G * 2 * 4)) : nullptr;
 #define GN_FWD(E, A, R)                                                                                                               \
     CFL_LAUNCH(K_GN_APPLY, (cfl_gn_apply_kernel<E, A, R>), grid, dim3(GN_T), 0, stream, (const E*)x, (const E*)res, gamma, beta, part, \
-               HW, C, G, rows, eps, (E*)y, mean, rstd)
+               HW, C, G, rows, eps, (E*)y, mean, rstd, stats)
     if (dtype == 0) {
         CFL_LAUNCH(K_GN_STATS, cfl_gn_stats_kernel<F8>, grid, dim3(GN_T), 0, stream, (const F8*)x, HW, C, G, rows, part);
-        GN_SWITCH(F8, GN_FWD);
     } else {
         CFL_LAUNCH(K_GN_STATS, cfl_gn_stats_kernel<U4>, grid, dim3(GN_T), 0, stream, (const U4*)x, HW, C, G, rows, part);
-        GN_SWITCH(U4, GN_FWD);
     }
+    if (stats)
+        CFL_LAUNCH(K_GN_STATS, cfl_gn_merge_kernel, dim3(N), dim3(1024), 0, stream, part, (int)grid.x, rows, HW, C / G, G, eps, stats);
+    if (dtype == 0) { GN_SWITCH(F8, GN_FWD); } else { GN_SWITCH(U4, GN_FWD); }
 #undef GN_FWD
     return 0;
 }
@@ -934,11 +967,13 @@ int cfl_gn_bwd(const void* dy, const void* dy2, const void* x, const void* res, 
     const dim3 grid(chunks, N);
     float* pg = (float*)ws;
     float* pc = (float*)((char*)ws + cfl_align256((size_t)N * chunks * G * 2 * 4));
+    const int sums = chunks > GN_MERGE ? 1 : chunks;
 #define GN_BWD(E, A, R)                                                                                                                 \
     CFL_LAUNCH(K_GN_BWD_REDUCE, (cfl_gn_bwd_reduce_kernel<E, A, R>), grid, dim3(GN_T), 0, stream, (const E*)x, (const E*)dy,            \
                (const E*)dy2, (const E*)res, gamma, beta, mean, rstd, HW, C, G, rows, pc, pg);                                          \
+    if (chunks > GN_MERGE) CFL_LAUNCH(K_GN_BWD_REDUCE, cfl_gn_bwd_merge_kernel, dim3(G, N), dim3(64), 0, stream, pg, chunks, G);        \
     CFL_LAUNCH(K_GN_BWD_APPLY, (cfl_gn_bwd_apply_kernel<E, A, R>), grid, dim3(GN_T), 0, stream, (const E*)x, (const E*)dy,              \
-               (const E*)dy2, (const E*)res, gamma, beta, mean, rstd, pg, HW, C, G, rows, (E*)dx, want_dres ? (E*)dres : (E*)nullptr)
+               (const E*)dy2, (const E*)res, gamma, beta, mean, rstd, pg, HW, C, G, rows, sums, (E*)dx, want_dres ? (E*)dres : (E*)nullptr)
     if (dtype == 0) { GN_SWITCH(F8, GN_BWD); } else { GN_SWITCH(U4, GN_BWD); }
 #undef GN_BWD
     CFL_LAUNCH(K_GN_BWD_FINAL, cfl_gn_bwd_final_kernel, dim3(cfl_cdiv(C, 16)), dim3(1024), 0, stream, pc, N * chunks, C, dgamma, dbeta);
