@@ -2396,6 +2396,8 @@ def dropout(x, p, seed=None):
         raise _lib.CreamflHipError(f'dropout: p must lie between 0 and 1, got {p}')
     if p == 0.0 or x.numel() == 0:
         return x
+    if _DROPOUT_TICK[0] is not None and _DROPOUT_TICK[0].device != x.device:      # (the kernel adds that device's word to its seed)
+        raise _lib.CreamflHipError(f'dropout: the dropout tick is registered on {_DROPOUT_TICK[0].device}, x is on {x.device}')
     seed = _next_dropout_seed() if seed is None else int(seed) & 0xFFFFFFFF
     return _DropoutFn.apply(x.contiguous(), p, seed, torch.is_grad_enabled() and x.requires_grad)
 

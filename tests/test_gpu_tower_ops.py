@@ -163,6 +163,13 @@ def test_dropout_manner(dev):
             ops.dropout(**{**dict(x=x, p=0.5), **kw})
 
 
+def test_dropout_refuses_a_tick_of_another_device(dev, monkeypatch):
+    from creamfl_amd import _lib, ops
+    monkeypatch.setitem(ops._DROPOUT_TICK, 0, torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(_lib.CreamflHipError, match='tick'):
+        ops.dropout(torch.ones(4, device=dev), 0.5)
+
+
 def test_dropout_backward_uses_the_forwards_tick(dev):
     """The tick moves on between forward and backward: the gradient still follows the mask that the forward drew."""
     from creamfl_amd import ops
