@@ -165,7 +165,7 @@ def test_dropout_manner(dev):
 
 def test_dropout_refuses_a_tick_of_another_device(dev, monkeypatch):
     from creamfl_amd import _lib, ops
-    monkeypatch.setitem(ops._DROPOUT_TICK, 0, torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(ops, '_DROPOUT_TICK', [torch.zeros(1, dtype=torch.int32)])
     with pytest.raises(_lib.CreamflHipError, match='tick'):
         ops.dropout(torch.ones(4, device=dev), 0.5)
 
