@@ -621,7 +621,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
                 for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(s[0][r]) * (dp[0][r] - D);
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) { r0 += s[0][r]; r1 += s[0][r + 1]; }
-                mma_cols(Kt[buf], at, u, s[0], dq);
+                mma_cols<NW == 1>(Kt[buf], at, u, s[0], dq);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (nxt < 0) return true;
