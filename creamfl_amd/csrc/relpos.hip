@@ -654,12 +654,13 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
 // ---- backward, keys: dK, dV and the bias gradient.  A wave owns 32 keys; the staged rows are queries.
 // The bias gradient of a distance is the sum of ds along a diagonal (diag_add, into words of the wave's own; adding every value in LDS took
 // @DQ@ at 32 texts of 512 tokens, 12 heads).  Tiles beyond +-R are summed in registers.  At the end the workgroup's sums per distance go to
-// part [heads][slots][nd], one slot per (text, key block, part), place d + R + BPAD.
+// part [heads][slots][2 R + 1], one slot per (text, key block, part).
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, int nkb) {
     constexpr int NT = NW * 64, U = KT / 32;
     __shared__ __attribute__((aligned(1024))) u16 Qt[NB][KT * 64], Gt[NB][KT * 64];
     __shared__ __attribute__((aligned(16))) float ls[NB][KT], ds[NB][KT];      // -log-sum and -D of the staged queries
+    __shared__ float ends[2];
     extern __shared__ float bl[];
     const int nd = 2 * (a.R + BPAD) + 1, mid = a.R + BPAD;
     float* gone = bl + nd;                                     // [KT] of -inf: what a lane reads whose key does not take part
@@ -672,9 +673,9 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     const int sp = id % a.ns, kb = id / a.ns % nkb, h = id / (a.ns * nkb) % a.heads, b = id / (a.ns * nkb * a.heads);
     const Text t = text_of(a, b);
     if (a.cu && kb == 0) clear_rest<NT>(a, t, b, h, sp, a.dk, a.dv, a.lddk);
-    float* out = a.diag + ((((long long)h * a.B + b) * nkb + kb) * a.ns + sp) * nd;
+    float* out = a.diag + ((((long long)h * a.B + b) * nkb + kb) * a.ns + sp) * (2 * a.R + 1);
     if (kb * NW * 32 >= t.lk) {
-        for (int i = threadIdx.x; i < nd; i += NT) out[i] = 0.f;
+        for (int i = threadIdx.x; i <= 2 * a.R; i += NT) out[i] = 0.f;
         return;
     }
     const Part part = part_of(sp, a.ns, t.lq, KT);
@@ -790,7 +791,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
         tiles(std::true_type{}, min(behind, part.to), 0.f, far_hi);
         tiles(std::false_type{}, part.to, clo, far_lo);
     }
-    // the workgroup's sums per distance
+    // the workgroup's sums per distance; what lies beyond +-R counts as +-R
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
     if (lane == 0) {                                           // (far tiles exist only where the range reaches beyond +-R)
@@ -798,11 +799,21 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
         if (dhi >= a.R) dg[w * nd + mid + a.R] += far_hi;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < nd; i += NT) {
+    for (int side = w; side < 2; side += NW) {
         float x = 0.f;
-        if (i >= dlo + mid && i <= dhi + mid) {
+        for (int d = (side ? a.R + 1 : dlo) + lane; d <= (side ? dhi : -a.R - 1); d += 64)
 #pragma unroll
-            for (int c = 0; c < NW; ++c) x += dg[c * nd + i];
+            for (int c = 0; c < NW; ++c) x += dg[c * nd + d + mid];
+        x = wave_sum(x);
+        if (lane == 0) ends[side] = x;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i <= 2 * a.R; i += NT) {
+        const int d = i - a.R;
+        float x = (i == 0 ? ends[0] : 0.f) + (i == 2 * a.R ? ends[1] : 0.f);
+        if (d >= dlo && d <= dhi) {
+#pragma unroll
+            for (int c = 0; c < NW; ++c) x += dg[c * nd + d + mid];
         }
         out[i] = x;
     }
@@ -1032,8 +1043,15 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
     if (before != gridDim.y - 1) return;
     for (int i = threadIdx.x; i < nb; i += 1024) {
         float y = 0.f;
-        for (int k = 0; k < (int)gridDim.y; ++k)
-            y += __hip_atomic_load(share + ((long long)h * gridDim.y + k) * nb + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int k0 = 0; k0 < (int)gridDim.y; k0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = k0 + k < (int)gridDim.y ? __hip_atomic_load(share + ((long long)h * gridDim.y + k0 + k) * nb + i, __ATOMIC_RELAXED,
+                                                                   __HIP_MEMORY_SCOPE_AGENT) : 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y += v[k];
+        }
         put_dtable(dtable, bf16, (long long)i * heads + h, y);
     }
 }
@@ -1100,7 +1118,7 @@ size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb, 
     const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk), k = rp_shape((long long)B * heads, Lk, Lq ? Lq : Lk);
     const long long rows = Lq ? (long long)B * Lq : T, krows = T ? T : (long long)B * Lk;
     if (p.small) return (size_t)B * heads * 64 * 4;
-    return cfl_align256((size_t)B * heads * k.blocks * k.ns * rp_nd(R) * 4) + cfl_align256((size_t)heads * cfl_cdiv(rp_nd(R), 64) * nb * 4) +
+    return cfl_align256((size_t)B * heads * k.blocks * k.ns * (2 * R + 1) * 4) + cfl_align256((size_t)heads * cfl_cdiv(2 * R + 1, 64) * nb * 4) +
            cfl_align256((size_t)heads * 4) + rp_row_bytes(p, heads, rows) + rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
 }
 
@@ -1159,7 +1177,7 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
                    heads, (float*)nullptr, (u32*)nullptr, dtable, table_bf16);
         return 0;
     }
-    const int nd = rp_nd(R), nshare = cfl_cdiv(nd, 64);
+    const int nd = 2 * R + 1, nshare = cfl_cdiv(nd, 64);
     at += cfl_align256((size_t)B * heads * kp.blocks * kp.ns * nd * 4);
     float* share = (float*)at;
     at += cfl_align256((size_t)heads * nshare * nb * 4);
@@ -1183,7 +1201,7 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
 #define RP_LDS(NW) bl * (1 + (NW)) + 64 * 4
     RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, L, RP_LDS, a, kp.blocks);
 #undef RP_LDS
-    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, nshare), dim3(1024), 0, stream, a.diag, nd, R + BPAD,
+    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, nshare), dim3(1024), 0, stream, a.diag, nd, R,
                (long long)B * kp.blocks * kp.ns, bucket, R, nb, heads, share, a.done, dtable, table_bf16);
     if (kp.ns > 1) {
         const dim3 g((unsigned)((a.krows * heads + 3) / 4));
