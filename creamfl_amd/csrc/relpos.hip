@@ -346,7 +346,6 @@ __device__ __forceinline__ void store_row(const f32x16 (&o)[2], u16* row, int la
             *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
         }
 }
-__device__ __forceinline__ void lds_add(float* p, float v) { __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 // over the two lanes l, l ^ 32 (one VALU instruction instead of a trip through the LDS queue)
 __device__ __forceinline__ float half_max(float v) {
     const u32 u = __float_as_uint(v);
@@ -500,7 +499,12 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
 // Sums of a 32 x 32 block along its diagonals.  Register r of lane (x, half) holds column x and row j = (r & 3) + 8 (r >> 2) + 4 half; the sum
 // over j - x = e is added to dst[-e] in LDS.  With the columns in lanes 32 .. 63 and zeros below, the sums are  t <- (t moved down one
 // lane) + v_j  for j from the highest down: lane i then holds e = 32 - i.  One instruction moves and adds; two chains of 16 rows take turns.
-// The 64 addresses of an LDS addition are distinct and a wave's LDS operations stay in order, so the order of every sum is fixed.
+// The words are the wave's own, an addition's 64 addresses distinct and a wave's LDS operations in order: plain reads and writes, and a fixed
+// order of every sum (LDS atomics, some 50 clocks each, took the dK / dV kernel from 82 to 100 us at 32 texts of 512 tokens, 12 heads).
+__device__ __forceinline__ void add_own(float* p, float v) {
+    *p += v;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");     // (the next addition reads words that other lanes write here)
+}
 __device__ __forceinline__ float down_one(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x130, 0xf, 0xf, true));
 }
@@ -515,8 +519,8 @@ __device__ __forceinline__ void diag_add_apart(const f32x16& v, float* dst, int 
     float a = v[15], b = v[15];
 #pragma unroll
     for (int r = 14; r >= 0; --r) { a = down_one(a) + v[r]; b = down_one_round(b) + v[r]; }
-    lds_add(dst + lane - 32 - 16 * u, a);
-    if (lane >= 49) lds_add(dst + lane - 96 - 16 * u, b - a);
+    add_own(dst + lane - 32 - 16 * u, a);
+    if (lane >= 49) add_own(dst + lane - 96 - 16 * u, b - a);
 }
 __device__ __forceinline__ void diag_add(const f32x16& v, float* dst, int lane) {
     float hi = 0.f, lo = 0.f;
@@ -533,8 +537,8 @@ __device__ __forceinline__ void diag_add(const f32x16& v, float* dst, int lane) 
 #pragma unroll
         for (int k = 3; k >= 0; --k) { hi = down_one(hi) + __uint_as_float(low[k]); lo = down_one(lo) + __uint_as_float(low[k + 4]); }
     }
-    lds_add(dst + lane - 48, hi);
-    lds_add(dst + lane - 32, lo);
+    add_own(dst + lane - 48, hi);
+    add_own(dst + lane - 32, lo);
 }
 
 // ---- backward, queries: dQ and D.  Same ownership as the forward.
@@ -757,6 +761,10 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                         s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], a.scale2, nl[r]));
                         dp[0][r] *= s[0][r];
                     }
+                    if constexpr (APART) mma_cols_apart(Gt[buf], at, u, s[0], dv);
+                    else mma_cols<NB == 1>(Gt[buf], at, 0, s[0], dv);
+                    if constexpr (APART) mma_cols_apart(Qt[buf], at, u, dp[0], dk);
+                    else mma_cols<NB == 1>(Qt[buf], at, 0, dp[0], dk);
                     if constexpr (!near) {
                         float x0 = 0.f, x1 = 0.f;
 #pragma unroll
@@ -766,14 +774,6 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
                         diag_add_apart(dp[0], mine + d0, u, lane);
                     } else {
                         diag_add(dp[0], mine + d0, lane);
-                    }
-                    if constexpr (APART) {
-                        mma_cols_apart(Gt[buf], at, u, s[0], dv);
-                        mma_cols_apart(Qt[buf], at, u, dp[0], dk);
-                    } else {
-                        // (at most 32 queries: the roundings of few products would show, and they cost nothing)
-                        mma_cols<NB == 1>(Gt[buf], at, 0, s[0], dv);
-                        mma_cols<NB == 1>(Qt[buf], at, 0, dp[0], dk);
                     }
                 }
                 if (NB > 1) {
