@@ -15,7 +15,19 @@
 // Matrix instructions: v_mfma_f32_32x32x16_bf16; scores are formed TRANSPOSED (S^T = K Q^T) where a wave owns queries, so a lane owns
 // one query and its keys sit in the lane's registers; registers 8 kk .. 8 kk + 7 are then, packed to bf16, the second operand of the
 // following product (o^T = V^T P^T) whose first operand is read transposed out of LDS in the same key order (ds_read_b64_tr_b16).
-// P and ds are rounded to bf16 there (2^-9 relative, the precision of v and k themselves); sums stay in 32 bits.
+// P and ds are rounded to bf16 there (2^-9 relative, the precision of v and k themselves; two terms where it costs nothing, see below); sums stay
+// in 32 bits.
+//
+// What bounds it: vector instructions.  A score takes 3.5 of them and an exp2 at a quarter of their rate in the forward, 5.5 and one in dQ, 6 to 8
+// and one in dK / dV, against 2, 3 and 4 products of 64: the forward's vector pipes are busy 77 %, its matrix pipes 40 % of the time (counters
+// at 2 texts of 4096 tokens; the clock settles near 1.8 GHz).  Measured, 12 heads, kernel time and rate of the products:
+//                         32 texts of 512 tokens     2 texts of 4096 tokens
+//   forward               41 us    630 TF/s          126 us   818 TF/s
+//   dQ                    57 us    680 TF/s          167 us   926 TF/s
+//   dK / dV / diagonals   83 us    620 TF/s          235 us   877 TF/s
+//   table's last sums      5 us                        5 us
+// Tried, without gain or worse: tiles swizzled without any bank conflict; the log-sums spread by a product with ones; three waves a SIMD for
+// dK / dV (spills: 254 -> 311 us); wave priorities around the products; a loop copy per staging buffer in dK / dV.
 #include <type_traits>
 #include "common.h"
 
@@ -625,7 +637,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
                 for (int r = 0; r < 16; ++r) s[0][r] = __builtin_amdgcn_exp2f(s[0][r]) * (dp[0][r] - D);
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) { r0 += s[0][r]; r1 += s[0][r + 1]; }
-                mma_cols<NW == 1>(Kt[buf], at, u, s[0], dq);
+                mma_cols<NW == 1>(Kt[buf], at, u, s[0], dq);   // (two terms for a few queries: their roundings would show, and cost nothing)
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (nxt < 0) return true;
@@ -656,8 +668,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
 }
 
 // ---- backward, keys: dK, dV and the bias gradient.  A wave owns 32 keys; the staged rows are queries.
-// The bias gradient of a distance is the sum of ds along a diagonal (diag_add, into words of the wave's own; adding every value in LDS took
-// @DQ@ at 32 texts of 512 tokens, 12 heads).  Tiles beyond +-R are summed in registers.  At the end the workgroup's sums per distance go to
+// The bias gradient of a distance is the sum of ds along a diagonal (diag_add, into words of the wave's own; adding every value with an LDS
+// atomic took 240 us more at 32 texts of 512 tokens, 12 heads).  Tiles beyond +-R are summed in registers.  At the end the workgroup's sums per distance go to
 // part [heads][slots][2 R + 1], one slot per (text, key block, part).
 template <int NW, int KT, int NB>
 __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, int nkb) {
@@ -833,7 +845,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
 // operands; K, Q and dO pass through LDS for the products that contract over rows.  D is summed from p and dp themselves, so the
 // rounding of o plays no part; P and ds are taken as two bf16 terms: few products, and waiting for memory bounds this kernel.  The bias gradient's diagonals go to memory as they are: part [heads][B][64], place d + 32.
 // The log-sum is taken off the score as the forward formed it: a row of one key has p = 1 and ds = 0 to the bit.
-// 256 packed captions of 8 to 32 tokens, 12 heads: @B32@ us, against @B32OLD@ with the kernels for long texts.
+// 256 packed captions of 8 to 32 tokens, 12 heads: 23 us (2.0 TB/s), against 45 us with the kernels for long texts.  A wave's chain of loads bounds
+// it: every wave is resident at once, so nothing follows to hide it.
 __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     __shared__ __attribute__((aligned(16))) u16 Kt[32 * TP], Qt[32 * TP], Gt[32 * TP];
     __shared__ float bl[64], dgs[128];
@@ -1056,7 +1069,13 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
     }
 }
 
-// Launch shape for `L` rows that waves own (32 each) against `K` rows that are passed over, for every (text, head).
+// Launch shape for `L` rows that waves own (32 each) against `K` rows that are passed over, for every (text, head).  Each rule with both sides
+// measured, forward / backward in microseconds:
+//   texts of at most 32 tokens by their own backward kernel: 256 x 32 tokens x 12 heads 30 against 52
+//   the long axis split: one text of 8192 tokens, one head 46 / 117 against 171 / 507, of 2048 tokens x 4 heads 22 / 60 against 46 / 135 (until
+//   every SIMD has two waves instead of one: 43 / 116 and 27 / 60)
+//   four waves a workgroup: 32 x 512 x 12 42 / 144 against 65 / 216, one text of 1000 tokens, one head 14.8 / 44 against 15.9 / 49, 64 x 33 x 12 and less
+//   tie; their tiles of 64 rows against 32: 2 x 4096 x 12 129 / 420 against 141 / 466
 struct Shape { int nw, kt, blocks, ns; bool small; };
 inline Shape rp_shape(long long BH, int L, int K) {
     Shape p;
@@ -1067,8 +1086,7 @@ inline Shape rp_shape(long long BH, int L, int K) {
     const int most = K / 256 < 16 ? K / 256 : 16;
     p.ns = (int)(ns > most ? most : ns);
     if (p.ns < 1) p.ns = 1;
-    // four waves share what is staged, where that leaves a workgroup for every CU
-    p.nw = L > 32 && BH * cfl_cdiv(L, 128) * p.ns >= 256 ? 4 : 1;
+    p.nw = L > 32 ? 4 : 1;                                     // four waves share what is staged
     p.kt = p.nw == 1 || K <= 32 ? 32 : 64;
     p.blocks = cfl_cdiv(L, 32 * p.nw);
     return p;
@@ -1086,13 +1104,12 @@ inline int rp_check(const RpArgs& a, int head_dim) {
     return 0;
 }
 
-#define RP_LAUNCH(ID, KERN, P, K, LDS1, ...)                                                                                           \
+#define RP_LAUNCH(ID, KERN, P, LDS1, ...)                                                                                              \
     do {                                                                                                                               \
         const dim3 grid_((unsigned)((long long)a.B * a.heads * (P).blocks * (P).ns));                                                  \
-        if ((P).nw == 4 && (P).kt == 64) { CFL_LAUNCH(ID, (KERN<4, 64, 2>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }         \
-        else if ((P).nw == 4) { CFL_LAUNCH(ID, (KERN<4, 32, 1>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }                    \
-        else if ((K) > 32) { CFL_LAUNCH(ID, (KERN<1, 32, 2>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                        \
-        else { CFL_LAUNCH(ID, (KERN<1, 32, 1>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                                      \
+        if ((P).nw == 1) { CFL_LAUNCH(ID, (KERN<1, 32, 2>), grid_, dim3(64), LDS1(1), stream, __VA_ARGS__); }                          \
+        else if ((P).kt == 64) { CFL_LAUNCH(ID, (KERN<4, 64, 2>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }                   \
+        else { CFL_LAUNCH(ID, (KERN<4, 32, 1>), grid_, dim3(256), LDS1(4), stream, __VA_ARGS__); }                                     \
     } while (0)
 
 inline int rp_nd(int R) { return 2 * (R + BPAD) + 1; }
@@ -1141,7 +1158,10 @@ int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, l
     a.pm = p.ns > 1 ? (float*)((char*)ws + rp_part_bytes(p, heads, a.rows)) : nullptr;
     const size_t lds = (size_t)rp_nd(R) * 4;
 #define RP_LDS(NW) lds
-    RP_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel, p, Lk, RP_LDS, a);
+    if (p.small)
+        CFL_LAUNCH(K_RELPOS_FWD, (cfl_relpos_fwd_kernel<1, 32, 1>), dim3((unsigned)(B * heads)), dim3(64), lds, stream, a);
+    else
+        RP_LAUNCH(K_RELPOS_FWD, cfl_relpos_fwd_kernel, p, RP_LDS, a);
 #undef RP_LDS
     if (p.ns > 1)
         CFL_LAUNCH(K_RELPOS_JOIN, cfl_relpos_join_kernel, dim3((unsigned)((a.rows * heads + 3) / 4)), dim3(256), 0, stream, a.po, a.pm, p.ns, heads,
@@ -1189,7 +1209,7 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     at += rp_part_bytes(p, heads, a.rows);
     a.nqb = p.blocks; a.ns = p.ns;
 #define RP_LDS(NW) bl
-    RP_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel, p, Lk, RP_LDS, a);
+    RP_LAUNCH(K_RELPOS_DQ, cfl_relpos_dq_kernel, p, RP_LDS, a);
 #undef RP_LDS
     const int* qend = cu && !Lq ? cu + B : nullptr;
     if (p.ns > 1)
@@ -1199,7 +1219,7 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     a.pv = (float*)(at + rp_part_bytes(kp, heads, a.krows));
     a.ns = kp.ns;
 #define RP_LDS(NW) bl * (1 + (NW)) + 64 * 4
-    RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, L, RP_LDS, a, kp.blocks);
+    RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, RP_LDS, a, kp.blocks);
 #undef RP_LDS
     CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, nshare), dim3(1024), 0, stream, a.diag, nd, R,
                (long long)B * kp.blocks * kp.ns, bucket, R, nb, heads, share, a.done, dtable, table_bf16);
