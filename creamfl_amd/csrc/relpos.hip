@@ -345,17 +345,17 @@ __device__ __forceinline__ void drop_keys(f32x16& s, u64 bits, int u, int lane) 
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = (in >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[r] : -INFINITY;
 }
-// a lane's 32 values of its row, rounded once
+// a lane's 32 values of its row, rounded once.  The lanes l, l ^ 32 of a row trade halves (one instruction for two values), so that each writes 16
+// bytes in one piece (256 captions, 12 heads: forward 12.6 -> 11.2, backward 30.8 -> 26.6 us).
 __device__ __forceinline__ void store_row(const f32x16 (&o)[2], u16* row, int lane, float c) {
-    u16* op = row + 4 * (lane >> 5);
+    u16* op = row + 8 * (lane >> 5);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            uint2 v;
-            v.x = pack2(o[dt][4 * g] * c, o[dt][4 * g + 1] * c);
-            v.y = pack2(o[dt][4 * g + 2] * c, o[dt][4 * g + 3] * c);
-            *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
+        for (int g = 0; g < 2; ++g) {
+            const auto x = __builtin_amdgcn_permlane32_swap(pack2(o[dt][8 * g] * c, o[dt][8 * g + 1] * c), pack2(o[dt][8 * g + 4] * c, o[dt][8 * g + 5] * c), false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(pack2(o[dt][8 * g + 2] * c, o[dt][8 * g + 3] * c), pack2(o[dt][8 * g + 6] * c, o[dt][8 * g + 7] * c), false, false);
+            *reinterpret_cast<uint4*>(op + 32 * dt + 16 * g) = uint4{x[0], y[0], x[1], y[1]};
         }
 }
 // over the two lanes l, l ^ 32 (one VALU instruction instead of a trip through the LDS queue)
@@ -913,16 +913,8 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     f32x16 out[2];
     const auto store = [&](u16* p, long long ld, bool on, bool live, float c) {
         if (!on) return;
-        u16* op = p + x * ld + 4 * half;
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                uint2 v;
-                v.x = live ? pack2(out[dt][4 * g] * c, out[dt][4 * g + 1] * c) : 0u;
-                v.y = live ? pack2(out[dt][4 * g + 2] * c, out[dt][4 * g + 3] * c) : 0u;
-                *reinterpret_cast<uint2*>(op + 32 * dt + 8 * g) = v;
-            }
+        if (!live) { zero16(out[0]); zero16(out[1]); }
+        store_row(out, p + x * ld, lane, c);
     };
     const auto apply = [&](const u16* tile, const f32x16& w) {
         zero16(out[0]); zero16(out[1]);
