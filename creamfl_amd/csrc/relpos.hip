@@ -68,7 +68,7 @@ struct RpArgs {
     float *po, *pm;                         // the parts' results: [ns][heads][rows][64], and of the forward [ns][heads][rows][2] (maximum, sum)
     float* pr;                              // of dQ [ns][heads][rows]: the rows' sums of ds
     float* pv;                              // dV's
-    u32* done;                              // [heads]: counted by cfl_relpos_dtable_kernel, started at 0 by dQ's kernel
+    u32* done;                              // [heads]: counted by cfl_relpos_dtable_kernel, started at 0 by the kernel before
     long long rows, krows;                  // query rows, key rows in all
 };
 
@@ -860,6 +860,7 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
         if (!a.Lq) clear_rest<64>(a, t, b, h, 0, a.dq, nullptr, a.lddq);
         clear_rest<64>(a, t, b, h, 0, a.dk, a.dv, a.lddk);
     }
+    if (blockIdx.x == 0) for (int i = lane; i < a.heads; i += 64) a.done[i] = 0;
     if (t.lq == 0 || t.lk == 0) {
         part[lane] = 0.f;
         zero_rows<64>(a.dq, a.lddq, h, t.q0, t.q0 + t.lq);
@@ -991,14 +992,14 @@ __global__ __launch_bounds__(256) void cfl_relpos_join_sum_kernel(const float* _
     }
 }
 
-// ---- the bias gradient from part [heads][slots][nd] (place i: distance i - mid): the slots' sums of 64 distances, then of these every
-// bucket's share, in a fixed order.  grid = (heads, ceil(nd / 64)), 64 distances x 16 strands of slots.  One block of distances: that is the
-// table's gradient; more: share [heads][blocks][nb], and the head's last workgroup (whichever it is) adds the blocks up in their order.
+// ---- the bias gradient from part [heads][slots][nd] (place i: distance i - mid): sums of 64 distances over `per` slots, then of these every
+// bucket's share, in a fixed order.  grid = (heads, ceil(nd / 64), ceil(slots / per)), 64 distances x 16 strands of slots.  One workgroup a
+// head: that is the table's gradient; more: share [heads][workgroups][nb], and the head's last one (whichever it is) adds them up in order.
 __device__ __forceinline__ void put_dtable(void* dtable, int bf16, long long at, float v) {
     if (bf16) ((__bf16*)dtable)[at] = (__bf16)v;
     else ((float*)dtable)[at] = v;
 }
-__global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __restrict__ part, int nd, int mid, long long slots,
+__global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __restrict__ part, int nd, int mid, long long slots, int per,
                                                                  const int* __restrict__ bucket, int R, int nb, int heads, float* share, u32* done,
                                                                  void* dtable, int bf16) {
     __shared__ u32 before;
@@ -1009,14 +1010,15 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (i < nd) {
         const float* p = part + (long long)h * slots * nd + i;
-        long long s = strand;
-        for (; s + 112 < slots; s += 128) {
+        const long long last = min(slots, (long long)(blockIdx.z + 1) * per);
+        long long s = (long long)blockIdx.z * per + strand;
+        for (; s + 112 < last; s += 128) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] += p[(s + 16 * k) * nd];
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (s + 16 * k < slots) x[k] += p[(s + 16 * k) * nd];
+            if (s + 16 * k < last) x[k] += p[(s + 16 * k) * nd];
     }
     red[strand][lane] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     __syncthreads();
@@ -1035,7 +1037,7 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
         for (int k = threadIdx.x & (L - 1); k < 64; k += L) y += bk[k] == b ? red[0][k] : 0.f;
         for (int o = L >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
         if (b < nb && (threadIdx.x & (L - 1)) == 0) {
-            if (share) __hip_atomic_store(share + ((long long)h * gridDim.y + blockIdx.y) * nb + b, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (share) __hip_atomic_store(share + (((long long)h * gridDim.z + blockIdx.z) * gridDim.y + blockIdx.y) * nb + b, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             else put_dtable(dtable, bf16, (long long)b * heads + h, y);
         }
     }
@@ -1045,19 +1047,16 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
     __syncthreads();
     if (threadIdx.x == 0) before = __hip_atomic_fetch_add(done + h, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (before != gridDim.y - 1) return;
-    for (int i = threadIdx.x; i < nb; i += 1024) {
+    const int all = (int)(gridDim.y * gridDim.z);
+    if (before != (u32)(all - 1)) return;
+    for (int b0 = 0; b0 < nb; b0 += 1024 / L) {
+        const int b = b0 + threadIdx.x / L;
         float y = 0.f;
-        for (int k0 = 0; k0 < (int)gridDim.y; k0 += 8) {
-            float v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                v[k] = k0 + k < (int)gridDim.y ? __hip_atomic_load(share + ((long long)h * gridDim.y + k0 + k) * nb + i, __ATOMIC_RELAXED,
-                                                                   __HIP_MEMORY_SCOPE_AGENT) : 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y += v[k];
-        }
-        put_dtable(dtable, bf16, (long long)i * heads + h, y);
+        if (b < nb)
+            for (int k = threadIdx.x & (L - 1); k < all; k += L)
+                y += __hip_atomic_load(share + ((long long)h * all + k) * nb + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int o = L >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
+        if (b < nb && (threadIdx.x & (L - 1)) == 0) put_dtable(dtable, bf16, (long long)b * heads + h, y);
     }
 }
 
@@ -1109,6 +1108,15 @@ inline size_t rp_part_bytes(const Shape& p, int heads, long long rows) {
     return p.ns > 1 ? cfl_align256((size_t)p.ns * heads * rows * 64 * 4) : 0;
 }
 
+// slots a workgroup of the table's last sums takes: 512, by at most 1024 workgroups (one query of each of 446 texts of 1959 tokens, one head: 7136
+// slots take 44 us as one)
+inline int rp_per(long long slots) {
+    const long long parts = (slots + 511) / 512;
+    return (int)((slots + (parts < 1024 ? parts : 1024) - 1) / (parts < 1024 ? parts : 1024));
+}
+inline size_t rp_share_bytes(int heads, int nd, long long slots, int nb) {
+    return cfl_align256((size_t)heads * cfl_cdiv(nd, 64) * cfl_cdiv(slots, rp_per(slots)) * nb * 4) + cfl_align256((size_t)heads * 4);
+}
 inline size_t rp_row_bytes(const Shape& p, int heads, long long rows) { return p.ns > 1 ? cfl_align256((size_t)p.ns * heads * rows * 4) : 0; }
 
 }  // namespace
@@ -1126,9 +1134,9 @@ size_t cfl_relpos_bwd_ws_bytes(int B, int Lq, int Lk, int T, int heads, int nb, 
     if (B < 1 || Lq < 0 || Lk < 1 || T < 0 || heads < 1 || nb < 1 || R < 0 || R > MAXR || (Lq == 0 && T == 0)) return 0;
     const Shape p = rp_shape((long long)B * heads, Lq ? Lq : Lk, Lk), k = rp_shape((long long)B * heads, Lk, Lq ? Lq : Lk);
     const long long rows = Lq ? (long long)B * Lq : T, krows = T ? T : (long long)B * Lk;
-    if (p.small) return (size_t)B * heads * 64 * 4;
-    return cfl_align256((size_t)B * heads * k.blocks * k.ns * (2 * R + 1) * 4) + cfl_align256((size_t)heads * cfl_cdiv(2 * R + 1, 64) * nb * 4) +
-           cfl_align256((size_t)heads * 4) + rp_row_bytes(p, heads, rows) + rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
+    if (p.small) return cfl_align256((size_t)B * heads * 64 * 4) + rp_share_bytes(heads, 64, B, nb);
+    return cfl_align256((size_t)B * heads * k.blocks * k.ns * (2 * R + 1) * 4) +
+           rp_share_bytes(heads, 2 * R + 1, (long long)B * k.blocks * k.ns, nb) + rp_row_bytes(p, heads, rows) + rp_part_bytes(p, heads, rows) + 2 * rp_part_bytes(k, heads, krows);
 }
 
 int cfl_relpos_fwd(const void* q, long long ldq, const void* k, const void* v, long long ldk, const unsigned char* mask, const int* cu,
@@ -1182,19 +1190,22 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     const size_t bl = (size_t)rp_nd(R) * 4;
     char* at = (char*)ws;
     a.diag = (float*)at;
+    const int nd = p.small ? 64 : 2 * R + 1;
+    const long long slots = p.small ? B : (long long)B * kp.blocks * kp.ns;
+    const dim3 tg(heads, cfl_cdiv(nd, 64), (unsigned)cfl_cdiv(slots, rp_per(slots)));
+    at += cfl_align256((size_t)heads * slots * nd * 4);
+    float* share = tg.y * tg.z > 1 ? (float*)at : nullptr;
+    a.done = (u32*)(at + rp_share_bytes(heads, nd, slots, nb) - cfl_align256((size_t)heads * 4));
+    at += rp_share_bytes(heads, nd, slots, nb);
+#define RP_TABLE()                                                                                                                             \
+    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, tg, dim3(1024), 0, stream, a.diag, nd, p.small ? 32 : R, slots, rp_per(slots),       \
+               bucket, R, nb, heads, share, a.done, dtable, table_bf16)
     if (p.small) {
         a.ns = 1;
         CFL_LAUNCH(K_RELPOS_BWD32, cfl_relpos_bwd32_kernel, dim3((unsigned)(B * heads)), dim3(64), 0, stream, a);
-        CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, 1), dim3(1024), 0, stream, a.diag, 64, 32, (long long)B, bucket, R, nb,
-                   heads, (float*)nullptr, (u32*)nullptr, dtable, table_bf16);
+        RP_TABLE();
         return 0;
     }
-    const int nd = 2 * R + 1, nshare = cfl_cdiv(nd, 64);
-    at += cfl_align256((size_t)B * heads * kp.blocks * kp.ns * nd * 4);
-    float* share = (float*)at;
-    at += cfl_align256((size_t)heads * nshare * nb * 4);
-    a.done = (u32*)at;
-    at += cfl_align256((size_t)heads * 4);
     a.pr = (float*)at;
     at += rp_row_bytes(p, heads, a.rows);
     a.po = (float*)at;
@@ -1213,8 +1224,8 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
 #define RP_LDS(NW) bl * (1 + (NW)) + 64 * 4
     RP_LAUNCH(K_RELPOS_DKV, cfl_relpos_dkv_kernel, kp, RP_LDS, a, kp.blocks);
 #undef RP_LDS
-    CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, dim3(heads, nshare), dim3(1024), 0, stream, a.diag, nd, R,
-               (long long)B * kp.blocks * kp.ns, bucket, R, nb, heads, share, a.done, dtable, table_bf16);
+    RP_TABLE();
+#undef RP_TABLE
     if (kp.ns > 1) {
         const dim3 g((unsigned)((a.krows * heads + 3) / 4));
         const int* kend = cu ? cu + B : nullptr;

@@ -228,7 +228,7 @@ def check_padded(dev, t, mask, scale=None, heads=None):
 
 
 @pytest.mark.parametrize('B,L,heads', [(1, 1, 1), (3, 2, 2), (2, 17, 3), (2, 31, 4), (3, 32, 12), (2, 33, 2), (2, 63, 1), (2, 64, 2), (1, 65, 3), (2, 96, 2),
-                                       (1, 127, 1), (2, 128, 2), (2, 129, 2), (2, 197, 3), (1, 300, 2), (1, 513, 1), (9, 24, 12), (1, 1025, 1), (40, 160, 8)])
+                                       (1, 127, 1), (2, 128, 2), (2, 129, 2), (2, 197, 3), (1, 300, 2), (1, 513, 1), (9, 24, 12), (1, 1025, 1), (40, 160, 8), (1100, 3, 1), (260, 70, 1)])
 def test_relpos_attention_matches_oracle(dev, B, L, heads):
     check_padded(dev, attn_inputs(B * 1000 + L, B, L, heads), None)
 
