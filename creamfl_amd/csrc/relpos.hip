@@ -22,9 +22,9 @@
 // and one in dK / dV, against 2, 3 and 4 products of 64: the forward's vector pipes are busy 77 %, its matrix pipes 40 % of the time (counters
 // at 2 texts of 4096 tokens; the clock settles near 1.8 GHz).  Measured, 12 heads, kernel time and rate of the products:
 //                         32 texts of 512 tokens     2 texts of 4096 tokens
-//   forward               41 us    630 TF/s          126 us   818 TF/s
+//   forward               39 us    660 TF/s          124 us   830 TF/s
 //   dQ                    57 us    680 TF/s          167 us   926 TF/s
-//   dK / dV / diagonals   83 us    620 TF/s          235 us   877 TF/s
+//   dK / dV / diagonals   78 us    660 TF/s          234 us   880 TF/s
 //   table's last sums      5 us                        5 us
 // Tried, without gain or worse: tiles swizzled without any bank conflict; the log-sums spread by a product with ones; three waves a SIMD for
 // dK / dV (spills: 254 -> 311 us); wave priorities around the products; a loop copy per staging buffer in dK / dV.
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
 // over j - x = e is added to dst[-e] in LDS.  With the columns in lanes 32 .. 63 and zeros below, the sums are  t <- (t moved down one
 // lane) + v_j  for j from the highest down: lane i then holds e = 32 - i.  One instruction moves and adds; two chains of 16 rows take turns.
 // The words are the wave's own, an addition's 64 addresses distinct and a wave's LDS operations in order: plain reads and writes, and a fixed
-// order of every sum (LDS atomics, some 50 clocks each, took the dK / dV kernel from 82 to 100 us at 32 texts of 512 tokens, 12 heads).
+// order of every sum (with LDS atomics, some 50 clocks each, the dK / dV kernel took 100 us instead of 82 at 32 texts of 512 tokens, 12 heads).
 __device__ __forceinline__ void add_own(float* p, float v) {
     *p += v;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");     // (the next addition reads words that other lanes write here)
@@ -845,7 +845,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
 // operands; K, Q and dO pass through LDS for the products that contract over rows.  D is summed from p and dp themselves, so the
 // rounding of o plays no part; P and ds are taken as two bf16 terms: few products, and waiting for memory bounds this kernel.  The bias gradient's diagonals go to memory as they are: part [heads][B][64], place d + 32.
 // The log-sum is taken off the score as the forward formed it: a row of one key has p = 1 and ds = 0 to the bit.
-// 256 packed captions of 8 to 32 tokens, 12 heads: 23 us (2.0 TB/s), against 45 us with the kernels for long texts.  A wave's chain of loads bounds
+// 256 packed captions of 8 to 32 tokens, 12 heads: 21 us (2.2 TB/s), against 40 us with the kernels for long texts.  A wave's chain of loads bounds
 // it: every wave is resident at once, so nothing follows to hide it.
 __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
     __shared__ __attribute__((aligned(16))) u16 Kt[32 * TP], Qt[32 * TP], Gt[32 * TP];
@@ -1062,10 +1062,10 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
 
 // Launch shape for `L` rows that waves own (32 each) against `K` rows that are passed over, for every (text, head).  Each rule with both sides
 // measured, forward / backward in microseconds:
-//   texts of at most 32 tokens by their own backward kernel: 256 x 32 tokens x 12 heads 30 against 52
+//   texts of at most 32 tokens by their own backward kernel: 256 x 32 tokens x 12 heads 30 against 47
 //   the long axis split: one text of 8192 tokens, one head 46 / 117 against 171 / 507, of 2048 tokens x 4 heads 22 / 60 against 46 / 135 (until
 //   every SIMD has two waves instead of one: 43 / 116 and 27 / 60)
-//   four waves a workgroup: 32 x 512 x 12 42 / 144 against 65 / 216, one text of 1000 tokens, one head 14.8 / 44 against 15.9 / 49, 64 x 33 x 12 and less
+//   four waves a workgroup: 32 x 512 x 12 42 / 144 against 65 / 208, one text of 1000 tokens, one head 14.8 / 44 against 15.9 / 49, 64 x 33 x 12 and less
 //   tie; their tiles of 64 rows against 32: 2 x 4096 x 12 129 / 420 against 141 / 466
 struct Shape { int nw, kt, blocks, ns; bool small; };
 inline Shape rp_shape(long long BH, int L, int K) {
