@@ -676,7 +676,6 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     constexpr int NT = NW * 64, U = KT / 32;
     __shared__ __attribute__((aligned(1024))) u16 Qt[NB][KT * 64], Gt[NB][KT * 64];
     __shared__ __attribute__((aligned(16))) float ls[NB][KT], ds[NB][KT];      // -log-sum and -D of the staged queries
-    __shared__ float ends[2];
     extern __shared__ float bl[];
     const int nd = 2 * (a.R + BPAD) + 1, mid = a.R + BPAD;
     float* gone = bl + nd;                                     // [KT] of -inf: what a lane reads whose key does not take part
@@ -708,12 +707,12 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
     const float* dp_ = a.dsum + h * a.rows + t.q0;
     const int k0 = (kb * NW + w) * 32, key = k0 + (lane & 31);
     const bool live = key < t.lk && (!mask || mask[key]);
+    bf16x8 kf[4], vf[4];
+    load_rows(a.k + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, kf);
+    load_rows(a.v + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, vf);
     f32x16 dk[2], dv[2];
     zero16(dk[0]); zero16(dk[1]); zero16(dv[0]); zero16(dv[1]);
     if (__syncthreads_or(live) && part.from < part.to) {       // (else no key of the workgroup takes part: zeros)
-        bf16x8 kf[4], vf[4];
-        load_rows(a.k + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, kf);
-        load_rows(a.v + t.k0 * a.ldk + h * 64, a.ldk, k0, t.lk, lane, vf);
         if (!live) {
             const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -804,25 +803,18 @@ __global__ __launch_bounds__(NW * 64, 2) void cfl_relpos_dkv_kernel(RpArgs a, in
         tiles(std::false_type{}, part.to, clo, far_lo);
     }
     // the workgroup's sums per distance; what lies beyond +-R counts as +-R
+    for (int d = dlo + lane; d < -a.R; d += 64) far_lo += mine[d];
+    for (int d = a.R + 1 + lane; d <= dhi; d += 64) far_hi += mine[d];
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
-    if (lane == 0) {                                           // (far tiles exist only where the range reaches beyond +-R)
-        if (dlo <= -a.R) dg[w * nd + mid - a.R] += far_lo;
-        if (dhi >= a.R) dg[w * nd + mid + a.R] += far_hi;
-    }
-    __syncthreads();
-    for (int side = w; side < 2; side += NW) {
-        float x = 0.f;
-        for (int d = (side ? a.R + 1 : dlo) + lane; d <= (side ? dhi : -a.R - 1); d += 64)
-#pragma unroll
-            for (int c = 0; c < NW; ++c) x += dg[c * nd + d + mid];
-        x = wave_sum(x);
-        if (lane == 0) ends[side] = x;
+    if (lane == 0) {                                           // (these words exist where there was something to add)
+        if (dlo <= -a.R) mine[-a.R] += far_lo;
+        if (dhi >= a.R) mine[a.R] += far_hi;
     }
     __syncthreads();
     for (int i = threadIdx.x; i <= 2 * a.R; i += NT) {
         const int d = i - a.R;
-        float x = (i == 0 ? ends[0] : 0.f) + (i == 2 * a.R ? ends[1] : 0.f);
+        float x = 0.f;
         if (d >= dlo && d <= dhi) {
 #pragma unroll
             for (int c = 0; c < NW; ++c) x += dg[c * nd + d + mid];
