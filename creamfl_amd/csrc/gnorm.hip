@@ -7,13 +7,13 @@
 //
 // Where it sits: the normalisation of the image trunks (src/networks/models/image_encoder.py:27-36, src/networks/resnet_client.py:60-98
 // use BatchNorm there), for federations whose clients' batch statistics do not average.
-// HBM-bound: bf16 256 x 56 x 56 x 256 with a residual moves its maps at 5.7 TB/s in the forward (288 us, x read twice) and 5.4 TB/s in the
-// backward (605 us, everything read twice); fp32 128 x 28 x 28 x 128, read once, 24 and 38 us (4.2 and 4.0 TB/s).  A one-pass form that kept
-// slices of 200 KB in registers, one workgroup a CU, lost: its loads and stores do not overlap (261 against 232 us, with a residual 329
-// against 287).  A sample is a row-major [H W, C] matrix; a thread owns 8 consecutive channels of its rows (one 16-byte access in bf16).
+// HBM-bound: bf16 256 x 56 x 56 x 256 with a residual takes 266 us forward (290 before what fits registers
+// and LDS was kept for the second pass) and 605 backward (everything read twice, 5.4 TB/s); fp32 128 x 28 x 28 x 128, read once, 24 and 38 us (4.2 and 4.0 TB/s).  A one-pass form that kept
+// slices of 200 KB in registers, one workgroup a CU, lost: its loads and stores do not overlap (261 us without, 329 with a residual).  A sample is a row-major [H W, C] matrix; a thread owns 8 consecutive channels of its rows (one 16-byte access in bf16).
 // Statistics: a thread keeps its RPT rows in registers and forms mean and squared deviations of what it holds in two passes; partial
 // (mean, M2) pairs are then merged by sum n (mean - mu)^2, so that a mean much larger than the deviation costs no digits (a running
 // sum of squares would).  Everything is summed in 32 bits and in a fixed order: two runs give the same bits.
+#include <type_traits>
 #include "common.h"
 #include "colmap.h"
 
@@ -357,6 +357,7 @@ constexpr int RES_V16 = 14, RES_V32 = 8;                       // records a thre
 constexpr int RES_B16 = 13, RES_B32 = 9;                       // ... in the backward: x and the 32-bit gradient
 constexpr int RES_F16 = 4, RES_F32 = 3;                        // ... in the variants for few records
 constexpr int STR_T = 1024;                                    // threads of the two-pass kernels
+constexpr int STR_KEEP = 8;                                    // records a thread keeps in the forward of bf16
 constexpr int RES_T = 512;                                     // most threads of the one-pass kernels
 
 // (count, mean, M2) of the workgroup's groups from per-thread pairs in LDS: lds[rsub * slots + slot] = (mean, M2) over cnt(rsub) rows of the
@@ -631,9 +632,11 @@ __global__ __launch_bounds__(V <= 4 ? 256 : RES_T) void cfl_gn_res_bwd_kernel(co
 // slice in the caches (L2 and the 256 MB behind it), and runs from the last row to the first, the most recently read ones.
 // Deviations are summed from the thread's first value of a channel: what that costs in digits is at most the row count times 2^-24 of
 // the squared deviation of that one value, which is itself part of the sum.
-template <class E, int NG, int U>
+// KEEP of a thread's last records stay in registers and `kl` before them in LDS (its own place): the second pass does not read them again (17 of
+// 25 at 56 x 56 x 256 bf16: 290 -> 266 us with a residual; ten in registers 275).
+template <class E, int NG, int U, int KEEP>
 __global__ __launch_bounds__(STR_T) void cfl_gn_str_fwd_kernel(const E* __restrict__ x, const E* __restrict__ res, const float* __restrict__ gamma,
-                                                               const float* __restrict__ beta, int HW, int C, int G, int S, float eps, int act,
+                                                               const float* __restrict__ beta, int HW, int C, int G, int S, float eps, int act, int kl,
                                                                E* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
     extern __shared__ __attribute__((aligned(16))) float gl[];
     const int T = blockDim.x, t = threadIdx.x, cpg = C / G, GS = S / cpg, tpr = S >> 3, rpp = T / tpr, C8 = C >> 3, nsl = C / S;
@@ -642,29 +645,45 @@ __global__ __launch_bounds__(STR_T) void cfl_gn_str_fwd_kernel(const E* __restri
     float2* lds = reinterpret_cast<float2*>(gl + 16);
     float* mu = gl + 16 + 2 * T * NG;
     float* rs = mu + GS;
+    E* kept = reinterpret_cast<E*>(gl + (16 + 2 * T * NG + 2 * GS + 3) / 4 * 4);      // [kl][T]
     const int id = xcd_remap(blockIdx.x, gridDim.x), n = id / nsl, s0 = (id % nsl) * S;
     const int rsub = t / tpr, cl = (t - rsub * tpr) * 8, c0 = s0 + cl;
     const bool active = rsub < rpp;
     const long long step = (long long)rpp * C8;
     const E* px = x + ((long long)n * HW + rsub) * C8 + (c0 >> 3);
     const int cnt = active && rsub < HW ? (HW - rsub + rpp - 1) / rpp : 0;
+    const int tail = max(cnt - KEEP, 0), body = max(tail - kl, 0);       // records from `body` on: LDS, from `tail` on: registers
+    E own[KEEP > 0 ? KEEP : 1];
     if (active) {
         float K[8], s[8], q[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) { s[j] = 0.f; q[j] = 0.f; K[j] = 0.f; }
         if (cnt) unpack8(px[0], K);
-        for (int k0 = 0; k0 < cnt; k0 += U) {
-            E v[U];
+        const auto add = [&](const E& v, bool in) {
+            float f[8];
+            unpack8(v, f);
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = px[min(k0 + u, cnt - 1) * step];
+            for (int j = 0; j < 8; ++j) { const float d = in ? f[j] - K[j] : 0.f; s[j] += d; q[j] = fmaf(d, d, q[j]); }
+        };
+        const auto pass = [&](int from, int to, auto keep) {
+            for (int k0 = from; k0 < to; k0 += U) {
+                E v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float f[8];
-                unpack8(v[u], f);
-                const bool in = k0 + u < cnt;
+                for (int u = 0; u < U; ++u) v[u] = px[min(k0 + u, to - 1) * step];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { const float d = in ? f[j] - K[j] : 0.f; s[j] += d; q[j] = fmaf(d, d, q[j]); }
+                for (int u = 0; u < U; ++u) {
+                    if (keep && k0 + u < to) kept[(k0 + u - from) * T + t] = v[u];
+                    add(v[u], k0 + u < to);
+                }
             }
+        };
+        pass(0, body, std::false_type{});
+        pass(body, tail, std::true_type{});
+        if (KEEP > 0 && cnt) {
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) own[i] = px[min(tail + i, cnt - 1) * step];
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) add(own[i], tail + i < cnt);
         }
         const float inv = cnt ? 1.f / (float)cnt : 0.f;
 #pragma unroll
@@ -696,29 +715,47 @@ __global__ __launch_bounds__(STR_T) void cfl_gn_str_fwd_kernel(const E* __restri
     for (int j = 0; j < 8; ++j) { sc[j] = rs[gi[j]] * gamma[c0 + j]; sh[j] = beta[c0 + j]; mv[j] = mu[gi[j]]; }
     const E* pr = res ? res + (px - x) : nullptr;
     E* py = y + (px - x);
-    for (int k0 = cnt - 1; k0 >= 0; k0 -= U) {
-        E v[U], w[U];
+    const auto put = [&](const E& v, const E& w, int at) {
+        float f[8], h[8];
+        unpack8(v, f);
+        if (res) unpack8(w, h);
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = px[max(k0 - u, 0) * step];
+        for (int j = 0; j < 8; ++j) {
+            float z = fmaf(f[j] - mv[j], sc[j], sh[j]);
+            if (res) z += h[j];
+            f[j] = gn_act(act, z);
+        }
+        gn_store(py + at * step, f);
+    };
+#pragma unroll
+    for (int i0 = 0; i0 < KEEP; i0 += U) {
+        E w[U];
         if (res) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) w[u] = pr[max(k0 - u, 0) * step];
+            for (int u = 0; u < U; ++u) w[u] = pr[min(tail + i0 + u, cnt - 1) * step];
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (k0 - u < 0) break;
-            float f[8], h[8];
-            unpack8(v[u], f);
-            if (res) unpack8(w[u], h);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float z = fmaf(f[j] - mv[j], sc[j], sh[j]);
-                if (res) z += h[j];
-                f[j] = gn_act(act, z);
-            }
-            gn_store(py + (k0 - u) * step, f);
-        }
+        for (int u = 0; u < U; ++u)
+            if (tail + i0 + u < cnt) put(own[i0 + u], w[u], tail + i0 + u);
     }
+    const auto back = [&](int from, int to, auto keep) {           // records to - 1 .. from
+        for (int k0 = to - 1; k0 >= from; k0 -= U) {
+            E v[U], w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = keep ? kept[(max(k0 - u, from) - from) * T + t] : px[max(k0 - u, from) * step];
+            if (res) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) w[u] = pr[max(k0 - u, from) * step];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 - u < from) break;
+                put(v[u], w[u], k0 - u);
+            }
+        }
+    };
+    back(body, tail, std::true_type{});
+    back(0, body, std::false_type{});
 }
 
 template <class E, int U>
@@ -821,9 +858,9 @@ struct Plan { int kind, S, T; bool few; };
 // One pass where a slice of 64 or 128 bytes a row (a narrower one shares its cache lines with its neighbours) fits half a CU's threads at
 // V records each, so that one workgroup's loads run beside another's stores; else two passes where there is a slice for every CU; else
 // (few samples, large maps) chunks.  Measured, forward / forward with residual / backward with residual, microseconds:
-//   bf16 256 x 56 x 56 x 256: one pass 242 / 307 / 684 (32-byte slices), two passes 225 / 288 / 609
+//   bf16 256 x 56 x 56 x 256: one pass 242 / 307 / 684 (32-byte slices), two passes 218 / 266 / 609
 //   bf16 128 x 28 x 28 x 512: one pass 47 / 67 / 139, two passes 64 / 81 / 155;  fp32 128 x 28 x 28 x 128: 23 / 28 / 52, 27 / 34 / 66
-//   bf16 64 x 112 x 112 x 64 (128 slices): two passes 67 / 116 / 247, chunks 86 / 160 / 222
+//   bf16 64 x 112 x 112 x 64 (128 slices): two passes 68 / 113 / 247, chunks 86 / 160 / 222
 inline Plan gn_plan(int N, int HW, int C, int G, int size, bool bwd) {
     const int cpg = C / G, unit = cpg / gn_gcd(cpg, 8) * 8;     // lcm(cpg, 8)
     const int V = bwd ? (size == 2 ? RES_B16 : RES_B32) : (size == 2 ? RES_V16 : RES_V32);
@@ -890,17 +927,25 @@ int cfl_gn_fwd(const void* x, const void* res, const float* gamma, const float* 
     const Plan p = gn_plan(N, HW, C, G, dtype ? 2 : 4, false);
     if (p.kind) {
         const int ng = (C / G) % 8 ? 8 : 1, gs = p.S / (C / G);
-        const size_t lds = (size_t)(16 + 2 * gs) * 4 + (size_t)p.T * ng * 8;
+        size_t lds = (size_t)(16 + 2 * gs) * 4 + (size_t)p.T * ng * 8;
+        int kl = 0;
+        if (p.kind == 2) {                                     // (1024 threads have the CU's LDS for themselves, 512 half of it)
+            lds = (lds + 15) / 16 * 16;
+            const int rows = cfl_cdiv(HW, p.T / (p.S >> 3)) - (dtype ? STR_KEEP : 0), fit = ((160 * 1024 / STR_T) * p.T - (int)lds) / (p.T * (dtype ? 16 : 32));
+            kl = rows < fit ? rows : fit;
+            kl = kl > 0 ? kl : 0;
+            lds += (size_t)kl * p.T * (dtype ? 16 : 32);
+        }
         const dim3 rg((unsigned)(N * (C / p.S)));
-#define GN_ONE(KERN)                                                                                                                     \
+#define GN_ONE(KERN, ...)                                                                                                                \
     do {                                                                                                                                 \
-        CFL_SET_LDS(KERN, 96 * 1024);                                                                                                    \
-        CFL_LAUNCH(K_GN_RES, KERN, rg, dim3(p.T), lds, stream, (const GE*)x, (const GE*)res, gamma, beta, HW, C, G, p.S, eps, act, (GE*)y, \
-                   mean, rstd);                                                                                                          \
+        CFL_SET_LDS(KERN, 160 * 1024);                                                                                                   \
+        CFL_LAUNCH(K_GN_RES, KERN, rg, dim3(p.T), lds, stream, (const GE*)x, (const GE*)res, gamma, beta, HW, C, G, p.S, eps, act,       \
+                   __VA_ARGS__ (GE*)y, mean, rstd);                                                                                      \
     } while (0)
 #define GN_KIND(NG, VF, V)                                                                \
     do {                                                                                  \
-        if (p.kind == 2) { GN_ONE((cfl_gn_str_fwd_kernel<GE, NG, 4>)); }                  \
+        if (p.kind == 2) { GN_ONE((cfl_gn_str_fwd_kernel<GE, NG, 4, sizeof(GE) == 16 ? STR_KEEP : 0>), kl, ); } \
         else if (p.few) { GN_ONE((cfl_gn_res_fwd_kernel<GE, NG, VF>)); }                  \
         else { GN_ONE((cfl_gn_res_fwd_kernel<GE, NG, V>)); }                              \
     } while (0)
