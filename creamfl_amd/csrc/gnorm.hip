@@ -7,9 +7,11 @@
 //
 // Where it sits: the normalisation of the image trunks (src/networks/models/image_encoder.py:27-36, src/networks/resnet_client.py:60-98
 // use BatchNorm there), for federations whose clients' batch statistics do not average.
-// HBM-bound: bf16 256 x 56 x 56 x 256 with a residual takes 266 us forward (290 before what fits registers
-// and LDS was kept for the second pass) and 605 backward (everything read twice, 5.4 TB/s); fp32 128 x 28 x 28 x 128, read once, 24 and 38 us (4.2 and 4.0 TB/s).  A one-pass form that kept
-// slices of 200 KB in registers, one workgroup a CU, lost: its loads and stores do not overlap (261 us without, 329 with a residual).  A sample is a row-major [H W, C] matrix; a thread owns 8 consecutive channels of its rows (one 16-byte access in bf16).
+// HBM-bound: bf16 256 x 56 x 56 x 256 with a residual takes 266 us forward (290 before what fits registers and LDS was kept for the second
+// pass) and 605 backward (everything read twice, 5.4 TB/s; the same keeping there, three records of 25, gave 1 %); fp32 128 x 28 x 28 x 128,
+// read once, 24 and 38 us (4.2 and 4.0 TB/s).  A one-pass form that kept slices of 200 KB in registers, one workgroup a CU, lost: its loads and
+// stores do not overlap (261 us without, 329 with a residual).
+// A sample is a row-major [H W, C] matrix; a thread owns 8 consecutive channels of its rows (one 16-byte access in bf16).
 // Statistics: a thread keeps its RPT rows in registers and forms mean and squared deviations of what it holds in two passes; partial
 // (mean, M2) pairs are then merged by sum n (mean - mu)^2, so that a mean much larger than the deviation costs no digits (a running
 // sum of squares would).  Everything is summed in 32 bits and in a fixed order: two runs give the same bits.

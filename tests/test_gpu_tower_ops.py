@@ -506,3 +506,77 @@ def test_two_captured_graphs_replay(dev):
             torch.cuda.synchronize()
             for a, b in zip(got, step()):
                 assert torch.equal(a, b), k
+
+
+# ------------------------------------------------------------------------------------------------ offsets past 32 bits
+def test_relpos_attention_rows_past_32_bits(dev):
+    """2.2e9 elements of qkv: the last texts' rows, a text of nearly all rows cut to 40, and the rest zero."""
+    from creamfl_amd import ops
+    T, heads, L = 950_000, 12, 40
+    t = attn_inputs(3, 1, 1, heads)
+    qkv = torch.zeros(T, 192 * heads, dtype=torch.bfloat16, device=dev)
+    assert qkv.numel() > 1 << 31
+    g = torch.Generator().manual_seed(6)
+    cu = torch.tensor([0, 30, T - 75, T - 40, T], dtype=torch.int32)
+    ends = [(0, 30), (30, 70), (T - 75, T - 40), (T - 40, T)]      # (what takes part of each text)
+    parts = [torch.randn(b - a, 192 * heads, generator=g).to(torch.bfloat16) for a, b in ends]
+    dos = [torch.randn(b - a, 64 * heads, generator=g).to(torch.bfloat16) for a, b in ends]
+    do = torch.zeros(T, 64 * heads, dtype=torch.bfloat16, device=dev)
+    for (a, b), x, d in zip(ends, parts, dos):
+        qkv[a:b], do[a:b] = x.to(dev), d.to(dev)
+    qkv.requires_grad_(True)
+    o = ops.relpos_attention_varlen(qkv, cu.to(dev), L, t['table'].to(dev), t['buckets'].to(dev), heads)
+    dqkv, = torch.autograd.grad(o, [qkv], do)
+    H = heads * 64
+    for (a, b), x, d in zip(ends, parts, dos):
+        w = text_oracle(x, t['table'], t['buckets'], None, d)
+        within(o[a:b].view(-1, heads, 64), w['o'], 'o from %d' % a)
+        for i, name in enumerate(('dq', 'dk', 'dv')):
+            within(dqkv[a:b, i * H:(i + 1) * H].reshape(-1, heads, 64), w[name], '%s from %d' % (name, a))
+    assert not o[70:T - 75].any() and not dqkv[70:T - 75].any()
+
+
+def test_gn_act_maps_past_32_bits(dev):
+    """2.2e9 elements: the last sample's values and gradients against 64 bits."""
+    from creamfl_amd import ops
+    N, C, G, S = 33, 256, 32, 512
+    x = torch.empty(N, C, S, S, dtype=torch.bfloat16, device=dev, memory_format=torch.channels_last)
+    assert x.numel() > 1 << 31
+    gen = torch.Generator(device=dev).manual_seed(3)
+    for n in range(N):
+        x[n] = torch.randn(C, S, S, device=dev, generator=gen) + n
+    dy = torch.zeros_like(x)
+    dy[-1] = torch.randn(C, S, S, device=dev, generator=gen)
+    ga = (1 + 0.1 * torch.randn(C, device=dev, generator=gen)).requires_grad_(True)
+    be = torch.zeros(C, device=dev, requires_grad=True)
+    y = ops.gn_act(x.requires_grad_(True), ga, be, G)
+    dx, dga, dbe = torch.autograd.grad(y, [x, ga, be], dy)
+    v, d, w = x.detach()[-1].double().reshape(G, -1), dy[-1].double().reshape(G, C // G, -1), ga.detach().double().reshape(G, C // G, 1)
+    mu = v.mean(1, keepdim=True)
+    r = ((v - mu).square().mean(1, keepdim=True) + 1e-5).rsqrt()
+    xh = (v - mu) * r
+    # one rounding of the output, and in 32 bits what a mean of N adds to a deviation of 1: x - mu is exact to 2^-24 of the mean
+    e = 2.0 ** -8
+    want = (xh.reshape(G, C // G, -1) * w).reshape(C, S, S)
+    assert bool(((y.detach()[-1].double() - want).abs() <= e * want.abs() + 64 * N * 2.0 ** -24).all())
+    gg = (d * w).reshape(G, -1)
+    want = (r * (gg - gg.mean(1, keepdim=True) - xh * (gg * xh).mean(1, keepdim=True))).reshape(C, S, S)
+    assert bool(((dx[-1].double() - want).abs() <= e * want.abs() + 64 * N * 2.0 ** -24).all())
+    assert not dx[:-1].any()
+    # sums of 262144 products of about 1: pairwise over threads, at most sqrt(262144) ulps of the largest partial sum
+    want = (d * xh.reshape(G, C // G, -1)).sum(2).reshape(-1)
+    assert bool(((dga.double() - want).abs() <= 2.0 ** -24 * 512 * 64 * (1 + want.abs().max())).all())
+    want = d.sum(2).reshape(-1)
+    assert bool(((dbe.double() - want).abs() <= 2.0 ** -24 * 512 * 64 * (1 + want.abs().max())).all())
+
+
+def test_dropout_elements_past_33_bits(dev):
+    """Elements are counted in pairs by a 64-bit number: behind 2^33 its upper half changes the flags."""
+    from creamfl_amd import ops
+    n, p, seed = (1 << 33) + 5001, 0.25, 77
+    y = ops.dropout(torch.ones(n, dtype=torch.bfloat16, device=dev), p, seed=seed)
+    f = float(torch.tensor(4 / 3).to(torch.bfloat16))
+    for start, s in ((0, seed), (1 << 33, seed + 0x632BE5AB)):
+        got = y[start:start + 5001].float().cpu()
+        assert torch.equal(got, torch.where(ref.keep_flags(s, p, 5001), torch.full_like(got, f), torch.zeros_like(got))), start
+    assert not torch.equal(y[:5001], y[1 << 33:])
