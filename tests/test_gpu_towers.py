@@ -91,12 +91,26 @@ def test_relative_text_tower_padded_packed_and_cls(dev, L):
                     assert off(gg[n], gw[n]) <= BERT_GRAD, (cls, pack is not None, n, off(gg[n], gw[n]))
 
 
-def gate_bound(linear, step):
+def smallest_map(model, x):
+    """Elements of the smallest normalised map in a pass of x."""
+    seen = []
+    hooks = [m.register_forward_hook(lambda m, i, o: seen.append((o[0] if isinstance(o, tuple) else o).numel()))
+             for m in model.modules() if isinstance(m, torch.nn.GroupNorm)]
+    with torch.no_grad():
+        model(x)
+    for h in hooks:
+        h.remove()
+    return min(seen)
+
+
+def gate_bound(linear, step, smallest):
     """The bound of a ResNet-18's gradients: `linear`, and the ReLUs whose inputs are so near zero that rounding decides them.  An input with
     relative noise e (root mean square; the inputs are normalised) has the other sign with probability e / pi: the mean of |noise|, e sqrt(2 / pi),
     times the density at zero, 1 / sqrt(2 pi).  Half the gradients pass, so that flipped gates are 2 e / pi of the gradient's square.  Behind l
-    layers of three roundings of `step` / sqrt(3) each, e = step sqrt(l); 17 layers add up their squares."""
-    return (linear ** 2 + 2 / 3.141592653589793 * step * sum(l ** 0.5 for l in range(1, 18))) ** 0.5
+    layers of three roundings of `step` / sqrt(3) each, e = step sqrt(l); 17 layers add up their squares.  That is what is expected.  Where e is so
+    small that a map has less than one such gate on the mean (23040 inputs, e = 2e-5: 0.15), one is still a gate of the N / 2 that pass: 2 / N of
+    the square.  More than three beyond the mean in one map have a chance below 0.15^4 / 4! = 2e-5, so three in the smallest map are allowed for."""
+    return (linear ** 2 + 2 / 3.141592653589793 * step * sum(l ** 0.5 for l in range(1, 18)) + 3 * 2 / smallest) ** 0.5
 
 
 @pytest.mark.parametrize('half', [False, True], ids=['fp32', 'bf16'])
@@ -122,10 +136,11 @@ def test_group_normed_trunk(dev, half):
     want, gw = run(ref.train(), x)
     (got, gg), names = launched(lambda: run(m, x.to(dev).contiguous(memory_format=torch.channels_last)))
     assert 'gn_res' in names, names
+    small = smallest_map(ref, x)
     bound = 60 * HALF / 3 ** 0.5 if half else 20 * 2.0 ** -24 * 4608 ** 0.5
     assert off(got, want) <= bound, off(got, want)
     for n in gw:
-        assert off(gg[n], gw[n]) <= gate_bound(2 * bound, HALF if half else 2.0 ** -24 * 4608 ** 0.5), (n, off(gg[n], gw[n]))
+        assert off(gg[n], gw[n]) <= gate_bound(2 * bound, HALF if half else 2.0 ** -24 * 4608 ** 0.5, small), (n, off(gg[n], gw[n]))
 
 
 def server(dev, half, dropout=None):
@@ -214,4 +229,4 @@ def test_client_step(dev):
         for a, b in zip(got, want):
             assert off(a, b) <= bound, off(a, b)
         for n in gw:
-            assert off(gg[n], gw[n]) <= gate_bound(2 * bound, 2.0 ** -24 * 4608 ** 0.5), (n, off(gg[n], gw[n]))
+            assert off(gg[n], gw[n]) <= gate_bound(2 * bound, 2.0 ** -24 * 4608 ** 0.5, smallest_map(ref, x)), (n, off(gg[n], gw[n]))
