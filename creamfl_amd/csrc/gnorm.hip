@@ -76,6 +76,14 @@ __device__ __forceinline__ void gn_groups(int cl, int cpg, int (&g)[8]) {
     }
 }
 
+// lanes (a power of two) of a wave for each of G groups of `work` items, GN_T threads in all (one thread a group took 175 us of a map of 64 channels
+// in one group, 32 row phases)
+__device__ __forceinline__ int gn_lanes(int G, int work) {
+    int L = 1;
+    while (L < 64 && 2 * L * G <= GN_T && L < work) L *= 2;
+    return L;
+}
+
 // ---- forward, pass 1: (mean, M2) of every group over a chunk of rows.  grid = (chunks, N); part: [N][chunks][G][2]
 template <class E>
 __global__ __launch_bounds__(GN_T) void cfl_gn_stats_kernel(const E* __restrict__ x, int HW, int C, int G, int rows, float* __restrict__ part) {
@@ -108,25 +116,31 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_stats_kernel(const E* __restrict_
         }
     }
     __syncthreads();
-    const int cpg = C / G;
-    for (int g = threadIdx.x; g < G; g += GN_T) {
-        // rows of phase s: those r0 + s + k rpp below r1
+    // L lanes of a wave to a group, over its (row phase, channel) pairs
+    const int cpg = C / G, pairs = m.rpp * cpg, L = gn_lanes(G, pairs), l = threadIdx.x & (L - 1);
+    for (int g0 = 0; g0 < G; g0 += GN_T / L) {
+        const int g = g0 + threadIdx.x / L;
+        const bool on = g < G;
         float sum = 0.f;
-        for (int s = 0; s < m.rpp; ++s) {
-            const int cnt = (r1 - r0 - s + m.rpp - 1) / m.rpp;
-            if (r1 - r0 > s) for (int c = 0; c < cpg; ++c) sum = fmaf((float)cnt, sm[s * C + g * cpg + c], sum);
+        for (int k = l; on && k < pairs; k += L) {
+            const int s = k / cpg, cnt = (r1 - r0 - s + m.rpp - 1) / m.rpp;      // rows of phase s: those r0 + s + i rpp below r1
+            if (r1 - r0 > s) sum = fmaf((float)cnt, sm[s * C + g * cpg + k - s * cpg], sum);
         }
+        for (int o = L >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         const float mean = sum / (float)((r1 - r0) * cpg);
         float m2 = 0.f;
-        for (int s = 0; s < m.rpp; ++s) {
-            const int cnt = (r1 - r0 - s + m.rpp - 1) / m.rpp;
-            if (r1 - r0 > s) for (int c = 0; c < cpg; ++c) {
-                const float d = sm[s * C + g * cpg + c] - mean;
-                m2 += fmaf((float)cnt * d, d, sq[s * C + g * cpg + c]);
+        for (int k = l; on && k < pairs; k += L) {
+            const int s = k / cpg, cnt = (r1 - r0 - s + m.rpp - 1) / m.rpp, at = s * C + g * cpg + k - s * cpg;
+            if (r1 - r0 > s) {
+                const float d = sm[at] - mean;
+                m2 += fmaf((float)cnt * d, d, sq[at]);
             }
         }
-        float* o = part + (((long long)blockIdx.y * gridDim.x + blockIdx.x) * G + g) * 2;
-        o[0] = mean; o[1] = m2;
+        for (int o = L >> 1; o > 0; o >>= 1) m2 += __shfl_xor(m2, o, 64);
+        if (on && l == 0) {
+            float* o = part + (((long long)blockIdx.y * gridDim.x + blockIdx.x) * G + g) * 2;
+            o[0] = mean; o[1] = m2;
+        }
     }
 }
 
@@ -280,11 +294,13 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_bwd_reduce_kernel(const E* __rest
         sa[c] = a * gamma[c]; sb[c] = b * gamma[c];            // (row phase 0's place: read above by this thread alone)
     }
     __syncthreads();
-    for (int g = threadIdx.x; g < G; g += GN_T) {
+    const int L = gn_lanes(G, cpg), l = threadIdx.x & (L - 1);
+    for (int g0 = 0; g0 < G; g0 += GN_T / L) {
+        const int g = g0 + threadIdx.x / L;
         float a = 0.f, b = 0.f;
-        for (int c = 0; c < cpg; ++c) { a += sa[g * cpg + c]; b += sb[g * cpg + c]; }
-        pg[(blk * G + g) * 2] = a;
-        pg[(blk * G + g) * 2 + 1] = b;
+        for (int c = l; g < G && c < cpg; c += L) { a += sa[g * cpg + c]; b += sb[g * cpg + c]; }
+        for (int o = L >> 1; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+        if (g < G && l == 0) { pg[(blk * G + g) * 2] = a; pg[(blk * G + g) * 2 + 1] = b; }
     }
 }
 

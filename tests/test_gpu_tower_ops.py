@@ -35,7 +35,7 @@ GN_SHAPES = [  # n, c, h, w, groups
     (1, 8, 1, 1, 8), (1, 8, 1, 1, 1), (3, 8, 1, 2, 4), (2, 16, 7, 7, 2), (1, 24, 5, 3, 3), (2, 40, 9, 11, 8), (5, 64, 13, 17, 32), (2, 320, 8, 8, 32),
     (3, 72, 30, 31, 9), (2, 512, 7, 7, 32), (1, 2048, 7, 7, 32), (2, 2048, 2, 3, 2048), (1, 1000, 4, 4, 5), (2, 64, 56, 56, 32), (1, 64, 112, 111, 16),
     (130, 8, 3, 3, 2), (2, 256, 28, 28, 1), (1, 1608, 12, 12, 67),
-    (2, 512, 95, 97, 32), (1, 1000, 41, 40, 5), (1, 2048, 24, 23, 2048)]             # (more than 64 chunks of rows, a ragged last one)
+    (2, 512, 95, 97, 32), (1, 1000, 41, 40, 5), (1, 2048, 24, 23, 2048), (3, 64, 57, 94, 1), (1, 2048, 9, 11, 1)]             # (more than 64 chunks of rows, a ragged last one)
 
 
 @pytest.mark.parametrize('shape', GN_SHAPES, ids=str)
