@@ -913,7 +913,9 @@ inline Plan gn_plan(int N, int HW, int C, int G, int size, bool bwd) {
 // rows per chunk: one register load per thread (RPT rows)
 inline int gn_rows(int HW, int C) { return GN_T / (C >> 3) * GN_RPT; }
 inline bool gn_bad(const void* x, int N, int HW, int C, int G) { return !x || N < 1 || HW < 1 || C < 1 || G < 1 || C % G != 0; }
-inline bool gn_limit(int N, int HW, int C) { return C % 8 != 0 || C > GN_MAXC || N > 65535; }
+// (rows are counted in 32 bits, a step of at most GN_T GN_RPT beyond the last: GN_MAXHW leaves room for it)
+constexpr int GN_MAXHW = 1 << 30;
+inline bool gn_limit(int N, int HW, int C) { return C % 8 != 0 || C > GN_MAXC || N > 65535 || HW > GN_MAXHW; }
 
 }  // namespace
 

@@ -1240,11 +1240,16 @@ def _aligned16(t):
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format)
 
 
+_GN_MAX_POSITIONS = 1 << 30          # H W of a map: the kernels count a sample's rows in 32 bits
+
+
 def gn_act_supported(x, num_channels, groups):
-    """True when `gn_act` takes `x`: [N, C, H, W] on the GPU, channels_last, bf16 or fp32, C a multiple of 8 and of `groups`, C <= 2048."""
+    """True when `gn_act` takes `x`: [N, C, H, W] on the GPU, channels_last, bf16 or fp32, C a multiple of 8 and of `groups`, C <= 2048,
+    H W <= 2^30."""
     return (torch.is_tensor(x) and x.is_cuda and x.dim() == 4 and x.dtype in (torch.bfloat16, torch.float32) and x.numel() > 0
             and x.shape[1] == num_channels and num_channels % 8 == 0 and num_channels <= 2048 and groups >= 1
-            and num_channels % groups == 0 and x.shape[0] <= 65535 and x.is_contiguous(memory_format=torch.channels_last))
+            and num_channels % groups == 0 and x.shape[0] <= 65535 and x.shape[2] * x.shape[3] <= _GN_MAX_POSITIONS
+            and x.is_contiguous(memory_format=torch.channels_last))
 
 
 class _GNActFn(torch.autograd.Function):
@@ -1307,7 +1312,7 @@ def gn_act(x, weight, bias, groups, eps=1e-5, act='none', residual=None, two=Fal
         raise _lib.CreamflHipError('gn_act: expected a CUDA/HIP tensor (no CPU fallback in creamfl_amd)')
     groups = int(groups)
     if not gn_act_supported(x, x.shape[1] if x.dim() == 4 else 0, groups):
-        raise _lib.CreamflHipError(f'gn_act: expected a channels_last bf16 / fp32 [N, C, H, W] map with C % 8 == 0, C % groups == 0, C <= 2048; '
+        raise _lib.CreamflHipError(f'gn_act: expected a channels_last bf16 / fp32 [N, C, H, W] map with C % 8 == 0, C % groups == 0, C <= 2048, H W <= 2^30; '
                                    f'got {tuple(x.shape)} {x.dtype} with {groups} groups')
     for t, name in ((weight, 'weight'), (bias, 'bias')):
         if not torch.is_tensor(t) or tuple(t.shape) != (x.shape[1],) or t.device != x.device:

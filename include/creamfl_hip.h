@@ -203,7 +203,7 @@ int cfl_dropout(const void* x, int dtype, long long n, double p, unsigned seed, 
  * for federations whose clients' batch statistics do not average: x [N][HW][C], G groups of C / G channels, statistics over one
  * sample's HW C / G values;  z = (x - mu) rstd gamma + beta (+ res), y = act(z), act 0 none, 1 relu, 2 silu.
  * dtype: 0 fp32, 1 bf16 (x, res, y, dy, dy2, dx, dres); gamma, beta, their gradients, mean / rstd [N][G] fp32 (both NULL = skip).
- * C % 8 == 0, C <= 2048, N <= 65535, 16-byte aligned activations.  bwd: the gradient is dy + dy2 (dy2 may be NULL); dres = dy act'(z)
+ * C % 8 == 0, C <= 2048, N <= 65535, HW <= 2^30, 16-byte aligned activations.  bwd: the gradient is dy + dy2 (dy2 may be NULL); dres = dy act'(z)
  * where want_dres; `res` as in the forward (NULL = none).  ws: cfl_gn_ws_bytes (forward and backward alike). */
 size_t cfl_gn_ws_bytes(int N, int HW, int C, int G);
 int cfl_gn_fwd(const void* x, const void* res, const float* gamma, const float* beta, int dtype, int N, int HW, int C, int G, float eps,
