@@ -49,10 +49,12 @@ __device__ __forceinline__ float gn_act(int act, float z) {
     if (act == GN_SILU) return z * gn_sigmoid(z);
     return z;
 }
-__device__ __forceinline__ float gn_act_grad(int act, float z) {
-    if (act == GN_RELU) return z > 0.f ? 1.f : 0.f;
-    if (act == GN_SILU) { const float s = gn_sigmoid(z); return s * fmaf(z, 1.f - s, 1.f); }
-    return 1.f;
+// d act'(z).  ReLU selects: where it is closed the result is 0 whatever the gradient holds (a product would make NaN of an infinite one, and
+// the group's sums would carry it into the whole group)
+__device__ __forceinline__ float gn_act_grad(int act, float z, float d) {
+    if (act == GN_RELU) return z > 0.f ? d : 0.f;
+    if (act == GN_SILU) { const float s = gn_sigmoid(z); return d * (s * fmaf(z, 1.f - s, 1.f)); }
+    return d;
 }
 // 8 channels rounded once (hardware conversion, two values an instruction)
 __device__ __forceinline__ void gn_store(U4* p, const float (&f)[8]) {
@@ -243,7 +245,7 @@ __device__ __forceinline__ void gn_dz(const E& xv, const E& rv, const float (&mv
         if (ACT != GN_NONE) {
             float z = fmaf(xh[j], ga[j], be[j]);
             if (RES) z += h[j];
-            dz[j] *= gn_act_grad(ACT, z);
+            dz[j] = gn_act_grad(ACT, z, dz[j]);
         }
     }
 }
@@ -616,7 +618,7 @@ __global__ __launch_bounds__(V <= 4 ? 256 : RES_T) void cfl_gn_res_bwd_kernel(co
                     if (act != GN_NONE) {
                         float z = fmaf(xh[j], ga[j], be[j]);
                         if (res) z += h[j];
-                        dz[k][j] *= gn_act_grad(act, z);
+                        dz[k][j] = gn_act_grad(act, z, dz[k][j]);
                     }
                     a8[j] += dz[k][j];
                     b8[j] = fmaf(dz[k][j], xh[j], b8[j]);
@@ -814,7 +816,7 @@ __global__ __launch_bounds__(STR_T) void cfl_gn_str_bwd_kernel(const E* __restri
             if (act != GN_NONE) {
                 float z = fmaf(xh[j], ga[j], be[j]);
                 if (res) z += h[j];
-                dz[j] *= gn_act_grad(act, z);
+                dz[j] = gn_act_grad(act, z, dz[j]);
             }
         }
     };

@@ -1,0 +1,77 @@
+"""GPU: group norm in each of the ways csrc/gnorm.hip runs it -- one pass over registers, two passes over a slice, chunks of rows -- against
+its 64-bit restatement (oracle/tower_ops.py), on maps as large as the ways' rules ask for.  The statistics are per sample, so the oracle
+takes a few samples of a large batch; the gradient of the others is zero, and so are their shares of dgamma and dbeta."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import tower_ops as ref
+
+pytestmark = pytest.mark.gpu
+DT = {'fp32': torch.float32, 'bf16': torch.bfloat16}
+
+
+@pytest.fixture(scope='module')
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip('needs a GPU')
+    from creamfl_amd import _lib
+    _lib.load()
+    return torch.device('cuda:0')
+
+
+def within(got, want, name):
+    value, bound = want
+    off = (got.detach().double().cpu() - value).abs()
+    bad = ~(off <= bound)
+    assert not bool(bad.any()), '%s: %d of %d outside, worst %.3g of its bound at %s' % (
+        name, int(bad.sum()), bad.numel(), float((off / bound).nan_to_num(nan=np.inf).max()), tuple(bad.nonzero()[0].tolist()))
+
+
+def fmap(shape, dtype, dev, gen, scale=1.0, shift=0.0):
+    return torch.empty(shape, dtype=DT[dtype], device=dev, memory_format=torch.channels_last).normal_(shift, scale, generator=gen)
+
+
+def sample_oracle(x, ga, be, groups, picks, act, res, dy, dtype):
+    p = torch.tensor(picks, device=x.device)
+    return ref.group_norm_act(x[p], ga, be, groups, act=act, residual=None if res is None else res[p], dy=None if dy is None else dy[p],
+                              bf16=dtype == 'bf16')
+
+
+# one pass, one pass of few records, chunks, two passes (of the backward)
+GATE_SHAPES = [((2, 256, 14, 13, 32), 'bf16'), ((2, 64, 13, 17, 32), 'fp32'), ((3, 64, 3, 3, 8), 'bf16'), ((1, 64, 112, 111, 16), 'fp32'),
+               ((1, 64, 112, 111, 16), 'bf16'), ((128, 72, 10, 10, 9), 'bf16'), ((64, 40, 10, 10, 5), 'fp32'), ((64, 40, 10, 10, 40), 'fp32')]
+
+
+@pytest.mark.parametrize('shape,dtype', GATE_SHAPES, ids=str)
+@pytest.mark.parametrize('two', [False, True], ids=['', 'two'])
+def test_gradients_at_closed_gates_do_not_count(dev, shape, dtype, two):
+    """Infinite and NaN gradients where ReLU is closed: zeros, as if nothing had arrived there."""
+    from creamfl_amd import ops
+    n, c, h, w, groups = shape
+    gen = torch.Generator(device=dev).manual_seed(n + c)
+    picks = sorted({0, n // 2, n - 1})
+    x, r = fmap((n, c, h, w), dtype, dev, gen), fmap((n, c, h, w), dtype, dev, gen)
+    ga, be = 1 + 0.3 * torch.randn(c, device=dev, generator=gen), 0.3 * torch.randn(c, device=dev, generator=gen)
+    dy, dy2 = torch.zeros_like(x), torch.zeros_like(x)
+    dy[picks] = fmap((len(picks), c, h, w), dtype, dev, gen)
+    if two:
+        dy2[picks] = fmap((len(picks), c, h, w), dtype, dev, gen)
+    z = torch.nn.functional.group_norm(x.float(), groups, ga, be) + r.float()
+    shut = z < -0.5                                            # (far beyond any rounding of z)
+    g = dy.double() + dy2.double()
+    g[shut] = 0
+    want = sample_oracle(x, ga, be, groups, picks, 'relu', r, g, dtype)
+    k = torch.randint(0, 4, shut.shape, device=dev, generator=gen)
+    for i, bad in enumerate((float('inf'), float('nan'), -float('inf'))):
+        dy[shut & (k == i)] = bad
+    if two:
+        dy2[shut & (k == 0)] = -float('inf')
+    leaves = [t.requires_grad_(True) for t in (x, ga, be, r)]
+    if two:
+        y, y2 = ops.gn_act(x, ga, be, groups, act='relu', residual=r, two=True)
+        grads = torch.autograd.grad([y, y2], leaves, [dy, dy2])
+    else:
+        grads = torch.autograd.grad(ops.gn_act(x, ga, be, groups, act='relu', residual=r), leaves, dy)
+    for name, t in zip(('dx', 'dgamma', 'dbeta', 'dres'), grads):
+        within(t if t.dim() == 1 else t[picks], want[name], name)
