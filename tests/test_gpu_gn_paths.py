@@ -75,3 +75,26 @@ def test_gradients_at_closed_gates_do_not_count(dev, shape, dtype, two):
         grads = torch.autograd.grad(ops.gn_act(x, ga, be, groups, act='relu', residual=r), leaves, dy)
     for name, t in zip(('dx', 'dgamma', 'dbeta', 'dres'), grads):
         within(t if t.dim() == 1 else t[picks], want[name], name)
+
+
+# Maps that run in two passes (a thread of 98 to 512 rows), in one pass and in chunks: the same statistics wherever a far value stands.
+@pytest.mark.parametrize('shape,dtype', [((128, 64, 256, 256, 32), 'bf16'), ((128, 64, 256, 256, 8), 'bf16'), ((128, 64, 128, 128, 32), 'fp32'), ((256, 64, 256, 256, 8), 'fp32'),
+                                         ((40, 64, 32, 32, 8), 'fp32'), ((1, 64, 256, 256, 8), 'fp32'), ((128, 72, 10, 10, 9), 'bf16'), ((64, 40, 52, 52, 40), 'fp32')], ids=str)
+@pytest.mark.parametrize('rest', ['flat', 'noise', 'high'])
+def test_statistics_keep_their_digits_beside_a_far_first_value(dev, shape, dtype, rest):
+    """A first pixel at 30000 (1000.3 beside a flat rest): the variance is nearly all that pixel's, and xh of it sqrt(M) -- every digit of the sum of
+    squares shows.  `high`: a mean of 300 deviations without a far value."""
+    from creamfl_amd import ops
+    n, c, h, w, groups = shape
+    gen = torch.Generator(device=dev).manual_seed(h + groups)
+    x = fmap((n, c, h, w), dtype, dev, gen)
+    if rest == 'flat':
+        x.copy_(torch.linspace(-1, 1, c, device=dev)[None, :, None, None].expand_as(x))
+    if rest == 'high':
+        x.add_(300)
+    else:
+        x[:, :, 0, 0] = 30000.0 if rest == 'noise' else 1000.3
+    ga, be = 1 + 0.3 * torch.randn(c, device=dev, generator=gen), 0.3 * torch.randn(c, device=dev, generator=gen)
+    y = ops.gn_act(x, ga, be, groups)
+    picks = sorted({0, n // 2, n - 1})
+    within(y[picks], sample_oracle(x, ga, be, groups, picks, 'none', None, None, dtype)['y'], 'y')
