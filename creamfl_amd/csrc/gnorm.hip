@@ -828,29 +828,38 @@ __global__ __launch_bounds__(STR_T) void cfl_gn_str_bwd_kernel(const E* __restri
         }
     };
     if (active) {
-        float a8[8], b8[8];
+        float* pa = la + rsub * S + cl;
+        float* pb = lb + rsub * S + cl;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             mv[j] = mean[(long long)n * G + g0 + gi[j]]; rv[j] = rstd[(long long)n * G + g0 + gi[j]];
             ga[j] = gamma[c0 + j]; be[j] = beta[c0 + j];
-            a8[j] = 0.f; b8[j] = 0.f;
+            pa[j] = 0.f; pb[j] = 0.f;
         }
-        for (int k0 = 0; k0 < cnt; k0 += U) {
-            E xv[U], hv[U];
-            float dz[U][8];
+        // sums of 16 records join the thread's in LDS (its own words): equal terms round the same way, and a chain of 512 would be off by up to 127
+        // halves of a last place, of 2048 by 508
+        for (int b0 = 0; b0 < cnt; b0 += 16) {
+            const int to = min(b0 + 16, cnt);
+            float a[8], b[8];
 #pragma unroll
-            for (int u = 0; u < U; ++u) load(min(k0 + u, cnt - 1), xv[u], dz[u], hv[u]);
+            for (int j = 0; j < 8; ++j) { a[j] = 0.f; b[j] = 0.f; }
+            for (int k0 = b0; k0 < to; k0 += U) {
+                E xv[U], hv[U];
+                float dz[U][8];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (k0 + u >= cnt) break;
-                float xh[8];
-                form(xv[u], hv[u], xh, dz[u]);
+                for (int u = 0; u < U; ++u) load(min(k0 + u, to - 1), xv[u], dz[u], hv[u]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { a8[j] += dz[u][j]; b8[j] = fmaf(dz[u][j], xh[j], b8[j]); }
+                for (int u = 0; u < U; ++u) {
+                    if (k0 + u >= to) break;
+                    float xh[8];
+                    form(xv[u], hv[u], xh, dz[u]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { a[j] += dz[u][j]; b[j] = fmaf(dz[u][j], xh[j], b[j]); }
+                }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { la[rsub * S + cl + j] = a8[j]; lb[rsub * S + cl + j] = b8[j]; }
+            for (int j = 0; j < 8; ++j) { pa[j] += a[j]; pb[j] += b[j]; }
+        }
     }
     __syncthreads();
     gn_block_sums(la, lb, ta, tb, s1, s2, T, S, GS, cpg, rpp, HW, gamma + s0, pc + (long long)n * 2 * C + s0, C);

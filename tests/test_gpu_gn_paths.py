@@ -98,3 +98,21 @@ def test_statistics_keep_their_digits_beside_a_far_first_value(dev, shape, dtype
     y = ops.gn_act(x, ga, be, groups)
     picks = sorted({0, n // 2, n - 1})
     within(y[picks], sample_oracle(x, ga, be, groups, picks, 'none', None, None, dtype)['y'], 'y')
+
+
+def test_constant_gradients_sum_without_drift(dev):
+    """Equal gradients at every position (what mean pooling sends): a chain of equal terms rounds the same way at every step.  Two passes, 576 rows a
+    thread; a constant for each of 32 channels."""
+    from creamfl_amd import ops
+    n, c, h, w, groups = 256, 32, 384, 384, 4
+    gen = torch.Generator(device=dev).manual_seed(9)
+    x = fmap((n, c, h, w), 'fp32', dev, gen).requires_grad_(True)
+    ga, be = (1 + 0.3 * torch.randn(c, device=dev, generator=gen)).requires_grad_(True), torch.zeros(c, device=dev, requires_grad=True)
+    picks = [0, n - 1]
+    dy = torch.zeros_like(x, requires_grad=False)
+    dy[picks] = (0.5 + torch.rand(c, device=dev, generator=gen))[None, :, None, None]
+    dx, dga, dbe = torch.autograd.grad(ops.gn_act(x, ga, be, groups), [x, ga, be], dy)
+    want = sample_oracle(x.detach(), ga.detach(), be.detach(), groups, picks, 'none', None, dy, 'fp32')
+    within(dbe, want['dbeta'], 'dbeta')
+    within(dga, want['dgamma'], 'dgamma')
+    within(dx[picks], want['dx'], 'dx')
