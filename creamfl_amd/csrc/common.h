@@ -37,7 +37,7 @@ enum CflKernel {
     K_CONV3_X3, K_CONV3_X3_WGRAD, K_CONV3_X3_WGRAD_REDUCE, K_CONV3_X3_WIMAGE,
     K_PAIR_BWD_REDUCE,
     K_DROPOUT, K_GN_RES, K_GN_STATS, K_GN_APPLY, K_GN_BWD_REDUCE, K_GN_BWD_APPLY, K_GN_BWD_FINAL,
-    K_RELPOS_FWD, K_RELPOS_JOIN, K_RELPOS_BWD32, K_RELPOS_DQ, K_RELPOS_DKV, K_RELPOS_DTABLE,
+    K_RELPOS_FWD, K_RELPOS_JOIN, K_RELPOS_BWD32, K_RELPOS_DQ, K_RELPOS_DKV, K_RELPOS_DTABLE, K_RELPOS_DTABLE_JOIN,
     K_NUM
 };
 

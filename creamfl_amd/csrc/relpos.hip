@@ -25,7 +25,7 @@
 //   forward               39 us    660 TF/s          124 us   830 TF/s
 //   dQ                    57 us    680 TF/s          167 us   926 TF/s
 //   dK / dV / diagonals   78 us    660 TF/s          234 us   880 TF/s
-//   table's last sums      5 us                        5 us
+//   table's last sums    4 + 4 us                    4 + 4 us
 // Tried, without gain or worse: tiles swizzled without any bank conflict; the log-sums spread by a product with ones; three waves a SIMD for
 // dK / dV (spills: 254 -> 311 us); wave priorities around the products; a loop copy per staging buffer in dK / dV.
 #include <type_traits>
@@ -68,7 +68,6 @@ struct RpArgs {
     float *po, *pm;                         // the parts' results: [ns][heads][rows][64], and of the forward [ns][heads][rows][2] (maximum, sum)
     float* pr;                              // of dQ [ns][heads][rows]: the rows' sums of ds
     float* pv;                              // dV's
-    u32* done;                              // [heads]: counted by cfl_relpos_dtable_kernel, started at 0 by the kernel before
     long long rows, krows;                  // query rows, key rows in all
 };
 
@@ -570,7 +569,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
     const Text t = text_of(a, b);
     const Part part = part_of(sp, a.ns, t.lk, KT);
     if (a.cu && !a.Lq && qb == 0) clear_rest<NT>(a, t, b, h, sp, a.dq, nullptr, a.lddq);
-    if (blockIdx.x == 0) for (int i = threadIdx.x; i < a.heads; i += NT) a.done[i] = 0;
     if (qb * NW * 32 >= t.lq) return;
     fill_bias<NT>(a, h, bl, -(t.lq | (NW * 32 - 1)), t.lk | (KT - 1));     // (rows past the end are computed with as well)
     Keys<NW, KT> keys{a.mask ? a.mask + (long long)b * a.Lk : nullptr, part.to, 0, tb, 0};
@@ -852,7 +850,6 @@ __global__ __launch_bounds__(64) void cfl_relpos_bwd32_kernel(RpArgs a) {
         if (!a.Lq) clear_rest<64>(a, t, b, h, 0, a.dq, nullptr, a.lddq);
         clear_rest<64>(a, t, b, h, 0, a.dk, a.dv, a.lddk);
     }
-    if (blockIdx.x == 0) for (int i = lane; i < a.heads; i += 64) a.done[i] = 0;
     if (t.lq == 0 || t.lk == 0) {
         part[lane] = 0.f;
         zero_rows<64>(a.dq, a.lddq, h, t.q0, t.q0 + t.lq);
@@ -986,15 +983,15 @@ __global__ __launch_bounds__(256) void cfl_relpos_join_sum_kernel(const float* _
 
 // ---- the bias gradient from part [heads][slots][nd] (place i: distance i - mid): sums of 64 distances over `per` slots, then of these every
 // bucket's share, in a fixed order.  grid = (heads, ceil(nd / 64), ceil(slots / per)), 64 distances x 16 strands of slots.  One workgroup a
-// head: that is the table's gradient; more: share [heads][workgroups][nb], and the head's last one (whichever it is) adds them up in order.
+// head: that is the table's gradient; more: share [heads][workgroups][nb], which a launch of its own adds up in order (4 us; the last
+// workgroup doing it would need a fence that writes back and drops whole caches, 30 us).
 __device__ __forceinline__ void put_dtable(void* dtable, int bf16, long long at, float v) {
     if (bf16) ((__bf16*)dtable)[at] = (__bf16)v;
     else ((float*)dtable)[at] = v;
 }
 __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __restrict__ part, int nd, int mid, long long slots, int per,
-                                                                 const int* __restrict__ bucket, int R, int nb, int heads, float* share, u32* done,
+                                                                 const int* __restrict__ bucket, int R, int nb, int heads, float* share,
                                                                  void* dtable, int bf16) {
-    __shared__ u32 before;
     __shared__ float red[16][64];
     __shared__ int bk[64];
     const int h = blockIdx.x, lane = threadIdx.x & 63, strand = threadIdx.x >> 6, i = blockIdx.y * 64 + lane;
@@ -1029,24 +1026,22 @@ __global__ __launch_bounds__(1024) void cfl_relpos_dtable_kernel(const float* __
         for (int k = threadIdx.x & (L - 1); k < 64; k += L) y += bk[k] == b ? red[0][k] : 0.f;
         for (int o = L >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
         if (b < nb && (threadIdx.x & (L - 1)) == 0) {
-            if (share) __hip_atomic_store(share + (((long long)h * gridDim.z + blockIdx.z) * gridDim.y + blockIdx.y) * nb + b, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (share) share[(((long long)h * gridDim.z + blockIdx.z) * gridDim.y + blockIdx.y) * nb + b] = y;
             else put_dtable(dtable, bf16, (long long)b * heads + h, y);
         }
     }
-    if (!share) return;
-    // (the shares are written through to memory and read from there: a fence would write back and drop whole caches, 30 us)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(done + h, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    const int all = (int)(gridDim.y * gridDim.z);
-    if (before != (u32)(all - 1)) return;
+}
+// share [heads][all][nb] -> dtable; L lanes of a wave to a bucket, as above
+__global__ __launch_bounds__(1024) void cfl_relpos_dtable_join_kernel(const float* __restrict__ share, int all, int nb, int heads, void* dtable,
+                                                                      int bf16) {
+    const int h = blockIdx.x;
+    int L = 16;
+    while (L > 1 && (long long)nb * L > 1024) L >>= 1;
     for (int b0 = 0; b0 < nb; b0 += 1024 / L) {
         const int b = b0 + threadIdx.x / L;
         float y = 0.f;
         if (b < nb)
-            for (int k = threadIdx.x & (L - 1); k < all; k += L)
-                y += __hip_atomic_load(share + ((long long)h * all + k) * nb + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int k = threadIdx.x & (L - 1); k < all; k += L) y += share[((long long)h * all + k) * nb + b];
         for (int o = L >> 1; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
         if (b < nb && (threadIdx.x & (L - 1)) == 0) put_dtable(dtable, bf16, (long long)b * heads + h, y);
     }
@@ -1107,7 +1102,7 @@ inline int rp_per(long long slots) {
     return (int)((slots + (parts < 1024 ? parts : 1024) - 1) / (parts < 1024 ? parts : 1024));
 }
 inline size_t rp_share_bytes(int heads, int nd, long long slots, int nb) {
-    return cfl_align256((size_t)heads * cfl_cdiv(nd, 64) * cfl_cdiv(slots, rp_per(slots)) * nb * 4) + cfl_align256((size_t)heads * 4);
+    return cfl_align256((size_t)heads * cfl_cdiv(nd, 64) * cfl_cdiv(slots, rp_per(slots)) * nb * 4);
 }
 inline size_t rp_row_bytes(const Shape& p, int heads, long long rows) { return p.ns > 1 ? cfl_align256((size_t)p.ns * heads * rows * 4) : 0; }
 
@@ -1187,11 +1182,13 @@ int cfl_relpos_bwd(const void* q, long long ldq, const void* k, const void* v, l
     const dim3 tg(heads, cfl_cdiv(nd, 64), (unsigned)cfl_cdiv(slots, rp_per(slots)));
     at += cfl_align256((size_t)heads * slots * nd * 4);
     float* share = tg.y * tg.z > 1 ? (float*)at : nullptr;
-    a.done = (u32*)(at + rp_share_bytes(heads, nd, slots, nb) - cfl_align256((size_t)heads * 4));
     at += rp_share_bytes(heads, nd, slots, nb);
 #define RP_TABLE()                                                                                                                             \
     CFL_LAUNCH(K_RELPOS_DTABLE, cfl_relpos_dtable_kernel, tg, dim3(1024), 0, stream, a.diag, nd, p.small ? 32 : R, slots, rp_per(slots),       \
-               bucket, R, nb, heads, share, a.done, dtable, table_bf16)
+               bucket, R, nb, heads, share, dtable, table_bf16);                                                                               \
+    if (share)                                                                                                                                 \
+        CFL_LAUNCH(K_RELPOS_DTABLE_JOIN, cfl_relpos_dtable_join_kernel, dim3(heads), dim3(1024), 0, stream, share, (int)(tg.y * tg.z), nb,     \
+                   heads, dtable, table_bf16)
     if (p.small) {
         a.ns = 1;
         CFL_LAUNCH(K_RELPOS_BWD32, cfl_relpos_bwd32_kernel, dim3((unsigned)(B * heads)), dim3(64), 0, stream, a);

@@ -27,6 +27,7 @@ static const char* const g_kernel_names[K_NUM] = {
     "cfl_dropout_kernel", "cfl_gn_res_kernel", "cfl_gn_stats_kernel", "cfl_gn_apply_kernel", "cfl_gn_bwd_reduce_kernel", "cfl_gn_bwd_apply_kernel",
     "cfl_gn_bwd_final_kernel",
     "cfl_relpos_fwd_kernel", "cfl_relpos_join_kernel", "cfl_relpos_bwd32_kernel", "cfl_relpos_dq_kernel", "cfl_relpos_dkv_kernel", "cfl_relpos_dtable_kernel",
+    "cfl_relpos_dtable_join_kernel",
 };
 
 namespace {
