@@ -2523,7 +2523,8 @@ def relpos_attention(qkv, table, buckets, heads, key_mask=None, scale=None):
 def relpos_attention_varlen(qkv, cu_seqlens, max_len, table, buckets, heads, scale=None):
     """`relpos_attention` on PACKED tokens: qkv [T, 3H], text b = rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1] on the device;
     a text may be empty); max_len: the longest text's length -- a longer one is cut to its first max_len tokens.  Rows that belong to no
-    text, or to a cut one's rest, give zeros.  -> [T, H]."""
+    text, or to a cut one's rest, give zeros.  The offsets must not fall: where they do, texts overlap and the results are undefined (in
+    bounds all the same; the host does not read them).  -> [T, H]."""
     qkv = _aligned16(_bf16c(qkv, 'qkv'))
     heads, max_len = int(heads), int(max_len)
     if qkv.dim() != 2 or qkv.numel() == 0 or max_len < 1:
@@ -2535,7 +2536,7 @@ def relpos_attention_varlen(qkv, cu_seqlens, max_len, table, buckets, heads, sca
 
 def relpos_attention_cls(q, kv, table, buckets, heads, key_mask=None, cu_seqlens=None, max_len=None, scale=None):
     """The single query at position 0 of every text ([CLS]): q [B, H], kv [B, L, 2H] (K | V; key_mask [B, L]) or, packed, [T, 2H] with
-    cu_seqlens and max_len.  -> [B, H]; differentiable in q, kv and table (once)."""
+    cu_seqlens and max_len (as of `relpos_attention_varlen`).  -> [B, H]; differentiable in q, kv and table (once)."""
     q, kv = _aligned16(_bf16c(q, 'q')), _aligned16(_bf16c(kv, 'kv'))
     heads = int(heads)
     packed = cu_seqlens is not None

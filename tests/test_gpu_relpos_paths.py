@@ -54,3 +54,50 @@ def test_the_tables_shares_meet_in_a_launch_of_their_own(dev, B, L, heads):
         dt, et = dt + w[0], et + w[1]
     off = (first.double().cpu() - dt).abs()
     assert bool((off <= et + 2.0 ** -24 * (dt.abs() + et) + 1e-30).all()), float((off / et).max())
+
+
+# A sentinel before and behind every buffer that the entries write, in elements
+GUARD = 4096
+
+
+class Guarded:
+    """A buffer between two stretches of a known value."""
+    def __init__(self, dev, n, dtype):
+        self.whole = torch.full((n + 2 * GUARD,), 7, dtype=dtype, device=dev)
+        self.n = n
+
+    def ptr(self):
+        return self.whole.data_ptr() + GUARD * self.whole.element_size()
+
+    def untouched(self):
+        return bool((self.whole[:GUARD] == 7).all()) and bool((self.whole[GUARD + self.n:] == 7).all())
+
+
+@pytest.mark.parametrize('cu', [[0, 30, 7, 12, -5], [5, -3, 1 << 30, 2], [-2 ** 31, 2 ** 31 - 1], [2 ** 31 - 1, -2 ** 31, 9, 9], [25, 25, 25], [19, 3, 20, 0, 1]], ids=str)
+@pytest.mark.parametrize('T,longest,cls', [(20, 20, False), (20, 20, True), (70, 70, False), (700, 700, False), (700, 700, True)])
+def test_offsets_of_any_kind_leave_everything_else_alone(dev, cu, T, longest, cls):
+    """Offsets that fall or lie outside the rows: the kernels clip them to the rows there are, so that nothing beside the buffers is written, forward
+    and backward, short and long texts, split or not.  (Which values overlapping texts give is undefined.)"""
+    from creamfl_amd import _lib, ops
+    lib = _lib.load()
+    B, H = len(cu) - 1, 64
+    g = torch.Generator(device=dev).manual_seed(T)
+    off = torch.tensor(cu, dtype=torch.int32, device=dev)
+    rows, lq = (B, 1) if cls else (T, 0)
+    q, k, v = (torch.randn(n, H, device=dev, generator=g).to(torch.bfloat16) for n in (rows, T, T))
+    do = torch.randn(rows, H, device=dev, generator=g).to(torch.bfloat16)
+    table, buckets = torch.randn(32, 1, device=dev, generator=g), ops.relpos_buckets(32, 128, dev)
+    o, lse, dsum = Guarded(dev, rows * H, torch.bfloat16), Guarded(dev, rows, torch.float32), Guarded(dev, rows, torch.float32)
+    nf = lib.cfl_relpos_fwd_ws_bytes(B, lq, longest, T, 1)
+    nb = lib.cfl_relpos_bwd_ws_bytes(B, lq, longest, T, 1, 32, 128)
+    wf, wb = Guarded(dev, max(nf, 256), torch.uint8), Guarded(dev, nb, torch.uint8)
+    dq, dk, dv, dt = Guarded(dev, rows * H, torch.bfloat16), Guarded(dev, T * H, torch.bfloat16), Guarded(dev, T * H, torch.bfloat16), Guarded(dev, 32, torch.float32)
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.cfl_relpos_fwd(q.data_ptr(), H, k.data_ptr(), v.data_ptr(), H, None, off.data_ptr(), B, lq, longest, T, 1, 64, 0.125, table.data_ptr(), 0, 32,
+                                  buckets.data_ptr(), 128, o.ptr(), H, lse.ptr(), wf.ptr(), stream), 'fwd')
+    _lib.check(lib.cfl_relpos_bwd(q.data_ptr(), H, k.data_ptr(), v.data_ptr(), H, None, off.data_ptr(), B, lq, longest, T, 1, 64, 0.125, table.data_ptr(), 0, 32,
+                                  buckets.data_ptr(), 128, o.ptr(), do.data_ptr(), H, lse.ptr(), dsum.ptr(), dq.ptr(), H, dk.ptr(), dv.ptr(), H, dt.ptr(),
+                                  wb.ptr(), stream), 'bwd')
+    torch.cuda.synchronize()
+    for name, t in dict(o=o, lse=lse, dsum=dsum, wf=wf, wb=wb, dq=dq, dk=dk, dv=dv, dt=dt).items():
+        assert t.untouched(), name
