@@ -59,6 +59,7 @@ SIGNATURES = {
     'cfl_set_dropout_tick': (c_int, [_P]),
     'cfl_dropout': (c_int, [_P, c_int, c_longlong, c_double, c_uint, _P, _P, _P, _P]),
     'cfl_gn_ws_bytes': (c_size_t, [c_int, c_int, c_int, c_int]),
+    'cfl_gn_plan': (c_int, [c_int, c_int, c_int, c_int, c_int, c_int]),
     'cfl_gn_fwd': (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, _P, _P, _P, _P]),
     'cfl_gn_bwd': (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P]),
     'cfl_relpos_fwd_ws_bytes': (c_size_t, [c_int, c_int, c_int, c_int, c_int]),

@@ -945,6 +945,13 @@ size_t cfl_gn_ws_bytes(int N, int HW, int C, int G) {
     return cfl_align256((size_t)N * chunks * G * 2 * 4) + cfl_align256((size_t)N * chunks * C * 2 * 4);      // (second: also the merged [2][N][G])
 }
 
+int cfl_gn_plan(int N, int HW, int C, int G, int dtype, int bwd) {
+    if (N < 1 || HW < 1 || C < 8 || G < 1 || C % G || dtype < 0 || dtype > 1) return CFL_EINVAL;
+    if (gn_limit(N, HW, C)) return CFL_ELIMIT;
+    const Plan p = gn_plan(N, HW, C, G, dtype ? 2 : 4, bwd != 0);
+    return p.kind | (p.kind && p.few ? 4 : 0) | (p.kind && !bwd && (C / G) % 8 ? 8 : 0) | (p.kind ? p.T << 4 : 0);
+}
+
 #define GN_SWITCH(E, LAUNCH)                                                                            \
     do {                                                                                                \
         if (act == GN_NONE && !res) { LAUNCH(E, GN_NONE, false); }                                      \

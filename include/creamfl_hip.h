@@ -206,6 +206,10 @@ int cfl_dropout(const void* x, int dtype, long long n, double p, unsigned seed, 
  * C % 8 == 0, C <= 2048, N <= 65535, HW <= 2^30, 16-byte aligned activations.  bwd: the gradient is dy + dy2 (dy2 may be NULL); dres = dy act'(z)
  * where want_dres; `res` as in the forward (NULL = none).  ws: cfl_gn_ws_bytes (forward and backward alike). */
 size_t cfl_gn_ws_bytes(int N, int HW, int C, int G);
+/* How the calls of these sizes are run (host arithmetic): bits 0-1: 0 chunks of rows by several launches, 1 one pass over registers, 2 two passes
+ * of one workgroup; bit 2: the one-pass variant for few rows; bit 3: groups that are no whole records of 8 channels (forward); bits 4 up:
+ * threads of a workgroup.  Negative: an error code.  For tests and measurements; a caller needs none of it. */
+int cfl_gn_plan(int N, int HW, int C, int G, int dtype, int bwd);
 int cfl_gn_fwd(const void* x, const void* res, const float* gamma, const float* beta, int dtype, int N, int HW, int C, int G, float eps,
                int act, void* y, float* mean, float* rstd, void* ws, void* stream);
 int cfl_gn_bwd(const void* dy, const void* dy2, const void* x, const void* res, const float* gamma, const float* beta, const float* mean,

@@ -116,3 +116,79 @@ def test_constant_gradients_sum_without_drift(dev):
     within(dbe, want['dbeta'], 'dbeta')
     within(dga, want['dgamma'], 'dgamma')
     within(dx[picks], want['dx'], 'dx')
+
+
+# (n, c, h, w, groups), type, the forward's and the backward's way as cfl_gn_plan names them: kind ('chunks', 'one', 'few', 'two'), threads, whether
+# groups are whole records of 8 channels.  The server's trunk at a batch of 256 takes ('two', 1024) for its stem and first stage, 'one' with 14
+# records a thread behind them; tests/test_tower_ops_limits.py checks on the CPU that every way is in this list.
+PATHS = [
+    ((256, 64, 113, 111, 32), 'bf16', ('two', 1024, False), ('two', 1024)),
+    ((256, 64, 57, 55, 32), 'bf16', ('two', 1024, False), ('two', 1024)),
+    ((256, 128, 57, 55, 8), 'bf16', ('two', 1024, True), ('two', 1024)),
+    ((128, 72, 31, 29, 24), 'bf16', ('two', 512, False), ('two', 512)),
+    ((128, 72, 31, 29, 9), 'bf16', ('two', 512, True), ('two', 512)),
+    ((128, 72, 9, 11, 24), 'bf16', ('two', 256, False), ('two', 256)),
+    ((128, 72, 9, 11, 9), 'bf16', ('two', 256, True), ('two', 256)),
+    ((256, 64, 57, 55, 32), 'fp32', ('two', 1024, False), ('two', 1024)),
+    ((256, 64, 57, 55, 8), 'fp32', ('two', 1024, True), ('two', 1024)),
+    ((64, 40, 52, 53, 40), 'fp32', ('two', 512, False), ('two', 512)),
+    ((64, 40, 52, 53, 5), 'fp32', ('two', 512, True), ('two', 512)),
+    ((64, 40, 9, 11, 40), 'fp32', ('two', 256, False), ('two', 256)),
+    ((64, 40, 9, 11, 5), 'fp32', ('two', 256, True), ('two', 256)),
+    ((128, 512, 29, 27, 32), 'bf16', ('one', 512, True), ('one', 512)),
+    ((256, 256, 14, 14, 32), 'bf16', ('one', 128, True), ('one', 128)),
+    ((256, 128, 29, 27, 32), 'bf16', ('one', 256, False), ('one', 256)),
+    ((128, 128, 29, 27, 32), 'fp32', ('one', 256, False), ('one', 256)),
+    ((128, 256, 14, 14, 32), 'fp32', ('one', 128, True), ('one', 128)),
+    ((128, 512, 7, 7, 32), 'bf16', ('few', 128, True), ('few', 128)),
+    ((128, 64, 16, 16, 32), 'fp32', ('few', 256, False), ('few', 256)),
+    ((128, 512, 7, 7, 32), 'fp32', ('few', 128, True), ('few', 128)),
+    ((66, 64, 16, 16, 32), 'bf16', ('few', 256, False), ('few', 256)),
+    ((1, 64, 113, 111, 32), 'bf16', ('chunks',), ('chunks',)),
+    ((2, 64, 113, 111, 8), 'fp32', ('chunks',), ('chunks',)),
+]
+
+
+def way(shape, dtype, bwd):
+    from creamfl_amd import _lib
+    n, c, h, w, groups = shape
+    p = _lib.load().cfl_gn_plan(n, h * w, c, groups, int(dtype == 'bf16'), int(bwd))
+    assert p >= 0, p
+    kind = ('chunks', 'few' if p & 4 else 'one', 'two')[p & 3]
+    return (kind,) if kind == 'chunks' else (kind, p >> 4) if bwd else (kind, p >> 4, not p & 8)
+
+
+@pytest.mark.parametrize('shape,dtype,fwd,bwd', PATHS, ids=str)
+@pytest.mark.parametrize('act,res,two', [('none', False, False), ('relu', False, False), ('relu', True, True), ('silu', True, False)])
+def test_every_way_matches_oracle(dev, shape, dtype, fwd, bwd, act, res, two):
+    """Values and gradients of the first, the last and a middle sample, in the forms that the trunks call: with and without a residual, with one
+    gradient and with two."""
+    from creamfl_amd import ops
+    assert way(shape, dtype, False) == fwd and way(shape, dtype, True) == bwd, (way(shape, dtype, False), way(shape, dtype, True))
+    n, c, h, w, groups = shape
+    gen = torch.Generator(device=dev).manual_seed(n * 31 + c + h)
+    picks = sorted({0, n // 2, n - 1})
+    x, r = fmap((n, c, h, w), dtype, dev, gen, 1.5, 0.5), fmap((n, c, h, w), dtype, dev, gen) if res else None
+    ga, be = 1 + 0.3 * torch.randn(c, device=dev, generator=gen), 0.3 * torch.randn(c, device=dev, generator=gen)
+    dy, dy2 = torch.zeros_like(x), torch.zeros_like(x) if two else None
+    dy[picks] = fmap((len(picks), c, h, w), dtype, dev, gen)
+    if two:
+        dy2[picks] = fmap((len(picks), c, h, w), dtype, dev, gen)
+    want = sample_oracle(x, ga, be, groups, picks, act, r, dy.double() + dy2.double() if two else dy, dtype)
+    leaves = [t.requires_grad_(True) for t in ((x, ga, be, r) if res else (x, ga, be))]
+    y = ops.gn_act(x, ga, be, groups, act=act, residual=r, two=two)
+    grads = torch.autograd.grad(list(y) if two else [y], leaves, [dy, dy2] if two else [dy])
+    y = y[0] if two else y
+    within(y[picks], want['y'], 'y')
+    for name, t in zip(('dx', 'dgamma', 'dbeta', 'dres'), grads):
+        within(t if t.dim() == 1 else t[picks], want[name], name)
+    rest = torch.ones(n, dtype=torch.bool, device=dev)
+    rest[picks] = False
+    assert bool(torch.isfinite(y[rest]).all()) and not bool((grads[0][rest] != 0).any())
+    with torch.no_grad():                                  # the forward alone, on another stream: the same bits
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            again = ops.gn_act(x, ga, be, groups, act=act, residual=r)
+        torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(again, y)

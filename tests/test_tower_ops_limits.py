@@ -30,3 +30,35 @@ def test_gn_act_refuses_maps_beyond_its_row_counters():
             assert not ops.gn_act_supported(x, 8, 1), (h, w)
             with pytest.raises(_lib.CreamflHipError, match='H W'):
                 ops.gn_act(x, x, x, 1)
+
+
+def test_gn_ways_are_all_tested():
+    """Every way that csrc/gnorm.hip's rule can choose stands in the GPU tests' list, and the rule still sends the listed shapes there: the kinds, both
+    types, both directions, groups of whole records and others, the two-pass kernels' three sizes of a workgroup -- and what the server's and the
+    clients' trunks take at their batches."""
+    import sys
+    import os
+    sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+    from test_gpu_gn_paths import PATHS, way
+    seen = set()
+    for shape, dtype, fwd, bwd in PATHS:
+        assert way(shape, dtype, False) == fwd and way(shape, dtype, True) == bwd, (shape, dtype, way(shape, dtype, False), way(shape, dtype, True))
+        seen |= {(dtype, 'fwd', fwd), (dtype, 'bwd', bwd)}
+
+    def kinds(got):
+        return {(d, way_, w[0] if w[0] != 'two' else w[:2], w[2:]) for d, way_, w in got}
+    for d in ('bf16', 'fp32'):
+        assert {(d, 'fwd', ('chunks',)), (d, 'bwd', ('chunks',))} <= seen
+        for t in (256, 512, 1024):
+            assert (d, 'bwd', ('two', t)) in seen and {(d, 'fwd', ('two', t, True)), (d, 'fwd', ('two', t, False))} <= seen, (d, t)
+        for k in ('one', 'few'):
+            assert any(x[:2] == (d, 'bwd') and x[2][0] == k for x in seen), (d, k)
+            for whole in (False, True):
+                assert any(x[:2] == (d, 'fwd') and x[2][0] == k and x[2][2] == whole for x in seen), (d, k, whole)
+    trunk = [(64, 112), (64, 56), (256, 56), (128, 56), (128, 28), (512, 28), (256, 28), (256, 14), (1024, 14), (512, 14), (512, 7), (2048, 7)]
+    client = [(64, 112), (64, 56), (128, 28), (256, 14), (512, 7)]
+    for d, batches, maps in (('bf16', (128, 256), trunk), ('fp32', (128,), client)):
+        for n in batches:
+            for c, s in maps:
+                got = {(d, 'fwd', way((n, c, s, s, 32), d, False)), (d, 'bwd', way((n, c, s, s, 32), d, True))}
+                assert kinds(got) <= kinds(seen), (n, c, s, got)
