@@ -15,8 +15,9 @@
 // Matrix instructions: v_mfma_f32_32x32x16_bf16; scores are formed TRANSPOSED (S^T = K Q^T) where a wave owns queries, so a lane owns
 // one query and its keys sit in the lane's registers; registers 8 kk .. 8 kk + 7 are then, packed to bf16, the second operand of the
 // following product (o^T = V^T P^T) whose first operand is read transposed out of LDS in the same key order (ds_read_b64_tr_b16).
-// P and ds are rounded to bf16 there (2^-9 relative, the precision of v and k themselves; two terms where it costs nothing, see below); sums stay
-// in 32 bits.
+// P and ds are rounded to bf16 there (by up to 2^-8 relative, as v and k are): o is then 2.3e-3 off at 512 tokens, its own rounding being 1.7e-3.
+// Where a text has at most 32 queries they are taken as two bf16 terms, and o is off by its own rounding alone: captions 9.6 -> 10.0 us, 128 texts'
+// [CLS] over 512 tokens 28.2 -> 29.6.  For long texts that would cost 40 -> 48 us at 32 x 512 tokens, 127 -> 178 at 2 x 4096.  Sums stay in 32 bits.
 //
 // What bounds it: vector instructions.  A score takes 3.5 of them and an exp2 at a quarter of their rate in the forward, 5.5 and one in dQ, 6 to 8
 // and one in dK / dV, against 2, 3 and 4 products of 64: the forward's vector pipes are busy 77 %, its matrix pipes 40 % of the time (counters
@@ -479,7 +480,7 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
                     l0 += s[u][r];
                     l1 += s[u][r + 1];
                 }
-                mma_cols(Vt[buf], at, u, s[u], o);
+                mma_cols<NW == 1>(Vt[buf], at, u, s[u], o);    // (two terms for a few queries)
             }
             if (nxt < 0) return true;
             if (NB == 1) {

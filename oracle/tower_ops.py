@@ -74,10 +74,10 @@ def keep_flags(seed, p, n):
     return torch.from_numpy(bits.astype(np.int64) >= int(round(65536 * p)))
 
 
-def relpos_attention_text(q, k, v, table, buckets, keep=None, scale=0.125, do=None):
+def relpos_attention_text(q, k, v, table, buckets, keep=None, scale=0.125, do=None, terms=1):
     """One text: q [Lq, heads, 64], k, v [Lk, heads, 64], table [nb, heads], buckets [2 R + 1], keep [Lk] flags.  Returns {name: (value,
     bound)} for o and, with do [Lq, heads, 64], dq, dk, dv and (in the bound without the output's own rounding) dtable.
-    Bounds count: p and ds rounded to bf16 before they meet v, k, q, do; o rounded before D = do . o is formed (but for dtable); outputs rounded."""
+    Bounds count: p (in `terms` bf16 terms where it meets v) and ds rounded to bf16 before they meet v, k, q, do; o rounded before D = do . o is formed (but for dtable); outputs rounded."""
     q, k, v, table = (t.detach().cpu().double() for t in (q, k, v, table))
     buckets = buckets.detach().cpu().long()
     lq, heads, hd = q.shape
@@ -97,7 +97,7 @@ def relpos_attention_text(q, k, v, table, buckets, keep=None, scale=0.125, do=No
     es = 80 * U32 * (abs(scale) * qh.abs() @ kh.abs().transpose(1, 2) + table.abs().max() + s.abs() + 8)
     ep = p * (4 * es + 1e-6)
     o = p @ vh
-    eo = (U16 * p + ep) @ vh.abs()
+    eo = (U16 ** terms * p + ep) @ vh.abs()
 
     def rows(t, extra=0.0):
         return t.permute(1, 0, 2)

@@ -101,3 +101,28 @@ def test_offsets_of_any_kind_leave_everything_else_alone(dev, cu, T, longest, cl
     torch.cuda.synchronize()
     for name, t in dict(o=o, lse=lse, dsum=dsum, wf=wf, wb=wb, dq=dq, dk=dk, dv=dv, dt=dt).items():
         assert t.untouched(), name
+
+
+@pytest.mark.parametrize('B,L,heads,form', [(5, 1, 2, 'padded'), (3, 17, 4, 'padded'), (9, 32, 12, 'padded'), (7, 31, 3, 'packed'), (4, 32, 2, 'cls'), (3, 513, 3, 'cls'),
+                                            (2, 2100, 1, 'cls'), (300, 200, 12, 'cls')])
+def test_few_queries_are_off_by_the_outputs_rounding_alone(dev, B, L, heads, form):
+    """p enters its product with v in two bf16 terms where a text has at most 32 queries: what they leave is 2^-16 of it."""
+    from creamfl_amd import ops
+    g = torch.Generator().manual_seed(B * 100 + L)
+    H = heads * 64
+    qkv = torch.randn(B, L, 3 * H, generator=g).to(torch.bfloat16)
+    table, buckets = torch.randn(32, heads, generator=g), ops.relpos_buckets(32, 128)
+    keep = torch.rand(B, L, generator=g) < 0.8
+    if form == 'packed':
+        cu = torch.arange(0, (B + 1) * L, L, dtype=torch.int32, device=dev)
+        o = ops.relpos_attention_varlen(qkv.view(B * L, 3 * H).to(dev), cu, L, table.to(dev), buckets.to(dev), heads).view(B, L, H)
+    elif form == 'cls':
+        o = ops.relpos_attention_cls(qkv[:, 0, :H].contiguous().to(dev), qkv[:, :, H:].contiguous().to(dev), table.to(dev), buckets.to(dev), heads,
+                                     key_mask=keep.to(dev)).view(B, 1, H)
+    else:
+        o = ops.relpos_attention(qkv.to(dev), table.to(dev), buckets.to(dev), heads, key_mask=keep.to(dev))
+    for b in range(min(B, 9)):
+        q, k, v = (t.reshape(L, heads, 64) for t in qkv[b].split(H, 1))
+        value, bound = ref.relpos_attention_text(q[:o.shape[1]], k, v, table, buckets, None if form == 'packed' else keep[b], 0.125, terms=2)['o']
+        off = (o[b].double().cpu().view(-1, heads, 64) - value).abs()
+        assert bool((off <= bound).all()), (b, float((off / bound).max()))
