@@ -282,9 +282,7 @@ __device__ __forceinline__ void fill_bias(const RpArgs& a, int h, float* bl, int
     }
 }
 // A tile of 32 rows that a wave owns against `n` staged ones, d0 = (first key) - (first query): whether it touches |d| < R
-__device__ __forceinline__ bool tile_near(int R, int d0, int n, bool key_lane) {
-    return key_lane ? d0 - n + 1 < R && d0 + 31 > -R : d0 - 31 < R && d0 + n - 1 > -R;
-}
+__device__ __forceinline__ bool tile_near(int R, int d0, int n) { return d0 - 31 < R && d0 + n - 1 > -R; }
 // ... and, where it does not, the one bias it has
 __device__ __forceinline__ float far_bias(const float* bl, int R, int d0) { return bl[(d0 > 0 ? R : -R) + R + BPAD]; }
 // S += A B^T of U blocks of 32 staged rows against a wave's 32; the blocks' chains of four take turns.  The lane's operand: its row's d
@@ -432,7 +430,7 @@ __global__ __launch_bounds__(NW * 64, 3) void cfl_relpos_fwd_kernel(RpArgs a) {
 #pragma unroll
             for (int u = 0; u < U; ++u) zero16(s[u]);
             mma_rows<U>(Kt[buf], at, qf, s);
-            if (tile_near(a.R, d0, KT, false)) {
+            if (tile_near(a.R, d0, KT)) {
                 const float* bp = bl + a.R + BPAD + d0 + 4 * (lane >> 5) - (lane & 31);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -615,7 +613,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 2) void cfl_relpos_dq_kernel
             Tile<NW, KT>::landed(Vt[buf], bits, w, lane);
             __syncthreads();                                   // (this tile for every wave; the other buffer's readers are done)
             if (NB > 1 && nxt >= 0) copy(nxt, buf ^ 1);
-            const bool near = tile_near(a.R, d0, KT, false);
+            const bool near = tile_near(a.R, d0, KT);
             const float* bp = bl + mid + (near ? d0 : 0) + 4 * (lane >> 5) - (lane & 31);
             const float c = far_bias(bl, a.R, near ? 0 : d0) - lse;
 #pragma unroll

@@ -126,3 +126,59 @@ def test_few_queries_are_off_by_the_outputs_rounding_alone(dev, B, L, heads, for
         value, bound = ref.relpos_attention_text(q[:o.shape[1]], k, v, table, buckets, None if form == 'packed' else keep[b], 0.125, terms=2)['o']
         off = (o[b].double().cpu().view(-1, heads, 64) - value).abs()
         assert bool((off <= bound).all()), (b, float((off / bound).max()))
+
+
+@pytest.mark.parametrize('lq,lk', [(40, 100), (100, 40), (5, 300), (300, 5), (33, 32), (32, 33), (20, 7), (1000, 64), (64, 1000), (1500, 33), (3, 1300)])
+@pytest.mark.parametrize('packed', [False, True], ids=['padded', 'packed'])
+def test_queries_and_keys_of_different_lengths(dev, lq, lk, packed):
+    """The entries' own form: Lq query rows a text against other numbers of keys, both counted from position 0; padded with a mask, or packed keys with an
+    empty text among them and rows behind the last one."""
+    from creamfl_amd import _lib, ops
+    lib = _lib.load()
+    B, heads = 3, 2
+    H = heads * 64
+    g = torch.Generator().manual_seed(lq * 7 + lk)
+    lens = [lk, 0, max(lk - 3, 1)] if packed else [lk] * 3
+    T = sum(lens) + 2 if packed else 0
+    keep = torch.rand(B, lk, generator=g) < 0.7
+    keep[:, 0] = True
+    rows = T if packed else B * lk
+    q, k, v = (torch.randn(n, H, generator=g).to(torch.bfloat16) for n in (B * lq, rows, rows))
+    do = torch.randn(B * lq, H, generator=g).to(torch.bfloat16)
+    table, buckets = torch.randn(32, heads, generator=g), ops.relpos_buckets(32, 128)
+    cu = torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32)
+    dq_, dk_, dv_, do_, dt_, db_ = (t.to(dev) for t in (q, k, v, do, table, buckets))
+    dm, dc = keep.to(torch.uint8).to(dev), cu.to(dev)
+    mask, off = (None, dc.data_ptr()) if packed else (dm.data_ptr(), None)
+    o = torch.full((B * lq, H), 7, dtype=torch.bfloat16, device=dev)
+    lse, dsum = torch.empty(heads, B * lq, device=dev), torch.empty(heads, B * lq, device=dev)
+    gq, gk, gv, gt = torch.full_like(o, 7), torch.full_like(dk_, 7), torch.full_like(dk_, 7), torch.full_like(dt_, 7)
+    wf = torch.empty(max(lib.cfl_relpos_fwd_ws_bytes(B, lq, lk, T, heads), 256), dtype=torch.uint8, device=dev)
+    wb = torch.empty(lib.cfl_relpos_bwd_ws_bytes(B, lq, lk, T, heads, 32, 128), dtype=torch.uint8, device=dev)
+    s = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.cfl_relpos_fwd(dq_.data_ptr(), H, dk_.data_ptr(), dv_.data_ptr(), H, mask, off, B, lq, lk, T, heads, 64, 0.125, dt_.data_ptr(), 0, 32,
+                                  db_.data_ptr(), 128, o.data_ptr(), H, lse.data_ptr(), wf.data_ptr(), s), 'fwd')
+    _lib.check(lib.cfl_relpos_bwd(dq_.data_ptr(), H, dk_.data_ptr(), dv_.data_ptr(), H, mask, off, B, lq, lk, T, heads, 64, 0.125, dt_.data_ptr(), 0, 32,
+                                  db_.data_ptr(), 128, o.data_ptr(), do_.data_ptr(), H, lse.data_ptr(), dsum.data_ptr(), gq.data_ptr(), H, gk.data_ptr(),
+                                  gv.data_ptr(), H, gt.data_ptr(), wb.data_ptr(), s), 'bwd')
+    torch.cuda.synchronize()
+
+    def ok(got, want, name):
+        value, bound = want
+        off_ = (got.double().cpu().view(value.shape) - value).abs()
+        assert bool((off_ <= bound).all()), (name, float((off_ / bound).nan_to_num(nan=np.inf).max()))
+    dt, et = torch.zeros(32, heads, dtype=torch.float64), torch.zeros(32, heads, dtype=torch.float64)
+    for b in range(B):
+        a, n = (int(cu[b]), lens[b]) if packed else (b * lk, lk)
+        qs = slice(b * lq, (b + 1) * lq)
+        if n == 0:
+            assert not o[qs].any() and not gq[qs].any()
+            continue
+        w = ref.relpos_attention_text(q[qs].view(lq, heads, 64), k[a:a + n].view(n, heads, 64), v[a:a + n].view(n, heads, 64), table, buckets,
+                                      None if packed else keep[b], 0.125, do[qs].view(lq, heads, 64))
+        for t, name in ((o[qs], 'o'), (gq[qs], 'dq'), (gk[a:a + n], 'dk'), (gv[a:a + n], 'dv')):
+            ok(t, w[name], '%s of text %d' % (name, b))
+        dt, et = dt + w['dtable'][0], et + w['dtable'][1]
+    ok(gt, (dt, et + 2.0 ** -24 * (dt.abs() + et) + 1e-30), 'dtable')
+    if packed:
+        assert not gk[T - 2:].any() and not gv[T - 2:].any()
