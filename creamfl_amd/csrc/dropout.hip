@@ -6,7 +6,8 @@
 // `transformers`, restated from its published definition).  The backward is the same map on the gradient, with the seed the forward
 // used: a launch may draw its seed from the device (the captured steps' tick, cfl_set_dropout_tick), so the forward leaves the
 // effective seed in a word of memory and the backward reads it from there -- also when the tick has moved on in between.
-// HBM-bound: one read and one write per element; 131072 x 768 bf16 in 72 us (5.6 TB/s, what a large copy reaches), 24 x 256 in 4.5 us of launch.
+// HBM-bound: one read and one write per element; 131072 x 768 bf16 in 72 us (5.6 TB/s; 5.75 at two to eight times the size, where a library copy
+// reaches 5.0 to 5.4), 24 x 256 in 4 us of launch.
 #include "common.h"
 #include "colmap.h"
 #include "rng.h"

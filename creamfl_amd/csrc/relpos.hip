@@ -19,14 +19,18 @@
 // Where a text has at most 32 queries they are taken as two bf16 terms, and o is off by its own rounding alone: captions 9.6 -> 10.0 us, 128 texts'
 // [CLS] over 512 tokens 28.2 -> 29.6.  For long texts that would cost 40 -> 48 us at 32 x 512 tokens, 127 -> 178 at 2 x 4096.  Sums stay in 32 bits.
 //
-// What bounds it: vector instructions.  A score takes 3.5 of them and an exp2 at a quarter of their rate in the forward, 5.5 and one in dQ, 6 to 8
-// and one in dK / dV, against 2, 3 and 4 products of 64: the forward's vector pipes are busy 77 %, its matrix pipes 40 % of the time (counters
-// at 2 texts of 4096 tokens; the clock settles near 1.8 GHz).  Measured, 12 heads, kernel time and rate of the products:
-//                         32 texts of 512 tokens     2 texts of 4096 tokens
-//   forward               39 us    660 TF/s          124 us   830 TF/s
-//   dQ                    57 us    680 TF/s          167 us   926 TF/s
-//   dK / dV / diagonals   78 us    660 TF/s          234 us   880 TF/s
-//   table's last sums    4 + 4 us                    4 + 4 us
+// What bounds it.  A score takes 3.5 vector instructions and an exp2 at a quarter of their rate in the forward, 5.5 and one in dQ, 6 to 8 and one in
+// dK / dV, against 2, 3 and 4 products of 64.  At 2 texts of 4096 tokens the vector pipes are busy 0.64 / 0.63 / 0.48 of the CUs' busy time in the
+// forward / dQ / dK dV, the matrix pipes 0.40 / 0.47 / 0.42 (the clock settles near 1.8 GHz): the first two are near their vector pipes' pace, while in
+// dK / dV neither pipe bounds -- its registers allow two waves a SIMD, and a wave's products, exponentials and products follow one another.  At 512
+// tokens both pipes wait more (vector 0.57 / 0.44 / 0.42, matrix 0.24 / 0.24 / 0.26): few tiles a workgroup behind its bias and first loads, texts of
+// unequal length.  Measured, 12 heads, kernel time and rate of the products of pairs that count:
+//                         32 texts of 128 to 512 tokens,   2 texts of 4096 tokens
+//                         two empty, padded to 512
+//   forward               38 us    440 TF/s                121 us   850 TF/s
+//   dQ                    58 us    440 TF/s                164 us   940 TF/s
+//   dK / dV / diagonals   74 us    450 TF/s                225 us   920 TF/s
+//   table's last sums    4 + 4 us                         4 + 4 us
 // Tried, without gain or worse: tiles swizzled without any bank conflict; the log-sums spread by a product with ones; three waves a SIMD for
 // dK / dV (spills: 254 -> 311 us); wave priorities around the products; a loop copy per staging buffer in dK / dV.
 #include <type_traits>
@@ -281,7 +285,7 @@ __device__ __forceinline__ void fill_bias(const RpArgs& a, int h, float* bl, int
         for (int i = 0; i < 4; ++i) if (d + i * NT <= last) bl[d + i * NT + mid] = bias_of(t[i]);
     }
 }
-// A tile of 32 rows that a wave owns against `n` staged ones, d0 = (first key) - (first query): whether it touches |d| < R
+// A tile of 32 queries that a wave owns against `n` staged keys, d0 = (first key) - (first query): whether it touches |d| < R
 __device__ __forceinline__ bool tile_near(int R, int d0, int n) { return d0 - 31 < R && d0 + n - 1 > -R; }
 // ... and, where it does not, the one bias it has
 __device__ __forceinline__ float far_bias(const float* bl, int R, int d0) { return bl[(d0 > 0 ? R : -R) + R + BPAD]; }

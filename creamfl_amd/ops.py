@@ -2510,7 +2510,9 @@ def relpos_attention(qkv, table, buckets, heads, key_mask=None, scale=None):
     """softmax_j(scale q_i . k_j + table[bucket of j - i, head]) V per text and head for a fused projection qkv [B, L, 3H] (Q | K | V along
     the last axis), head dim 64, any length (csrc/relpos.hip).  table: [num_buckets, heads], bf16 or fp32; buckets: `relpos_buckets`, or
     any int32 [2 R + 1] map of the clipped distance; key_mask [B, L] (True = the key takes part; what stands at a dropped key does not
-    matter), scale 1 / 8 by default.  A bias of -1e30 or less drops its keys too; a row without a key gives zeros.  Differentiable in qkv and table (once).  -> [B, L, H] bf16."""
+    matter), scale 1 / 8 by default.  A bias of -1e30 or less drops its keys too; a row without a key gives zeros.  Differentiable in qkv and
+    table (once).  Computed in bf16: another type of qkv is rounded to it first (its gradient comes back in its own type, rounded once); a text
+    of more than 32 tokens has its softmax and score gradients rounded to bf16 where they enter a product.  -> [B, L, H] bf16."""
     qkv = _aligned16(_bf16c(qkv, 'qkv'))
     heads = int(heads)
     if qkv.dim() != 3 or qkv.numel() == 0:
