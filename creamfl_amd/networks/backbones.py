@@ -695,16 +695,17 @@ class BertModel(nn.Module):
         if not lens or min(lens) < 1 or max(lens) > min(L, longest):
             return None
         B = len(lens)
-        cu = [0]
-        for n in lens:
-            cu.append(cu[-1] + n)
-        tok = torch.tensor([b * L + t for b, n in enumerate(lens) for t in range(n)], dtype=torch.int64)
+        n = torch.tensor(lens, dtype=torch.int64)
+        cu = torch.zeros(B + 1, dtype=torch.int64)
+        torch.cumsum(n, 0, out=cu[1:])
+        # (whole arrays: a Python loop over the tokens of 256 texts of 512 takes 24 ms of every fresh batch)
+        pos = torch.arange(int(cu[-1])) - torch.repeat_interleave(cu[:-1], n)
         plan = PackPlan()
-        plan.B, plan.L, plan.T = B, L, cu[-1]
-        plan.tok_idx = tok.to(device)
-        plan.pos_ids = (tok % L).to(device)
-        plan.cu = torch.tensor(cu, dtype=torch.int32).to(device)
-        plan.cls_rows = torch.tensor(cu[:-1], dtype=torch.int64).to(device)
+        plan.B, plan.L, plan.T = B, L, int(cu[-1])
+        plan.tok_idx = (torch.repeat_interleave(torch.arange(B) * L, n) + pos).to(device)
+        plan.pos_ids = pos.to(device)
+        plan.cu = cu.to(torch.int32).to(device)
+        plan.cls_rows = cu[:-1].clone().to(device)
         return plan
 
     def forward(self, input_ids, attention_mask=None, token_type_ids=None, cls_only=False, pack=None, **_):

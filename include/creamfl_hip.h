@@ -226,7 +226,8 @@ int cfl_gn_bwd(const void* dy, const void* dy2, const void* x, const void* res, 
  * query rows b Lq ..; Lk is the longest text's length (a longer one is cut to its first Lk rows).  Rows that belong to no text, and a cut
  * text's others, get zeros in o and in the gradients.  Offsets must not fall (cu[b] <= cu[b + 1]): they are clipped to 0 .. T, so nothing outside
  * the T rows is read or written whatever they hold, but where they fall texts overlap, and what the rows and dtable then hold is undefined.
- * Query i of a text stands at position i.  A row without a key has o = 0 and no gradient.
+ * Query i of a text stands at position i.  A bias of -1e30 or less drops its keys as the mask does.  A row without a key has o = 0 and no
+ * gradient.
  * lse (fp32 [heads][query rows]) is written by fwd (NULL = skip) and read by bwd; dsum: scratch of the same size; dtable as table.
  * All ld % 8 == 0, 16-byte aligned bases.
  * ws: cfl_relpos_fwd_ws_bytes (0: may be NULL) / cfl_relpos_bwd_ws_bytes (T = 0: padded). */

@@ -62,3 +62,21 @@ def test_gn_ways_are_all_tested():
             for c, s in maps:
                 got = {(d, 'fwd', way((n, c, s, s, 32), d, False)), (d, 'bwd', way((n, c, s, s, 32), d, True))}
                 assert kinds(got) <= kinds(seen), (n, c, s, got)
+
+
+def test_pack_plan_lists_the_real_tokens():
+    """The packed run's indexes against their definition, token by token; lengths that do not fit give no plan."""
+    import random
+    from creamfl_amd.networks.backbones import BertModel
+    r = random.Random(3)
+    for B, L, longest in ((1, 1, 32), (7, 24, 32), (256, 32, 32), (33, 300, 1 << 30), (5, 700, 1 << 30)):
+        lens = [r.randint(1, min(L, longest)) for _ in range(B)]
+        plan = BertModel.pack_plan(lens, L, 'cpu', longest)
+        pairs = [(b, t) for b, n in enumerate(lens) for t in range(n)]
+        assert (plan.B, plan.L, plan.T) == (B, L, len(pairs))
+        assert plan.tok_idx.dtype == torch.int64 and plan.tok_idx.tolist() == [b * L + t for b, t in pairs]
+        assert plan.pos_ids.dtype == torch.int64 and plan.pos_ids.tolist() == [t for _, t in pairs]
+        assert plan.cu.dtype == torch.int32 and plan.cu.tolist() == [sum(lens[:i]) for i in range(B + 1)]
+        assert plan.cls_rows.dtype == torch.int64 and plan.cls_rows.tolist() == plan.cu.tolist()[:-1] and plan.cls_rows.is_contiguous()
+    assert BertModel.pack_plan([3, 33], 40, 'cpu') is None and BertModel.pack_plan([3, 33], 40, 'cpu', 1 << 30) is not None
+    assert BertModel.pack_plan([], 40, 'cpu') is None and BertModel.pack_plan([0, 3], 40, 'cpu') is None and BertModel.pack_plan([41], 40, 'cpu', 1 << 30) is None
