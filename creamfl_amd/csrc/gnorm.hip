@@ -289,8 +289,14 @@ __global__ __launch_bounds__(GN_T) void cfl_gn_bwd_reduce_kernel(const E* __rest
     __syncthreads();
     const long long blk = (long long)n * gridDim.x + blockIdx.x;
     for (int c = threadIdx.x; c < C; c += GN_T) {
-        float a = 0.f, b = 0.f;
-        for (int s = 0; s < m.rpp; ++s) { a += sa[s * C + c]; b += sb[s * C + c]; }
+        float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};      // (four chains: one of 256 equal terms is off by up to 64 halves of a last place)
+        int s = 0;
+        for (; s + 3 < m.rpp; s += 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { p[i] += sa[(s + i) * C + c]; q[i] += sb[(s + i) * C + c]; }
+        }
+        for (; s < m.rpp; ++s) { p[0] += sa[s * C + c]; q[0] += sb[s * C + c]; }
+        const float a = (p[0] + p[1]) + (p[2] + p[3]), b = (q[0] + q[1]) + (q[2] + q[3]);
         pc[blk * 2 * C + c] = a;
         pc[blk * 2 * C + C + c] = b;
         sa[c] = a * gamma[c]; sb[c] = b * gamma[c];            // (row phase 0's place: read above by this thread alone)

@@ -192,3 +192,20 @@ def test_every_way_matches_oracle(dev, shape, dtype, fwd, bwd, act, res, two):
             again = ops.gn_act(x, ga, be, groups, act=act, residual=r)
         torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(again, y)
+
+
+@pytest.mark.parametrize('shape', [(1, 8, 1000, 1000, 1), (1, 8, 300, 300, 1), (1, 64, 512, 512, 8), (130, 8, 100, 100, 1), (40, 64, 32, 32, 8)], ids=str)
+def test_constant_gradients_sum_without_drift_in_chunks_and_in_one_pass(dev, shape):
+    """dbeta of a constant gradient, 24 constants a channel; the bound is the oracle's for a sum (64 halves of a last place).  Eight channels have 256
+    row phases to a chunk."""
+    from creamfl_amd import ops
+    n, c, h, w, groups = shape
+    for seed in range(24):
+        gen = torch.Generator(device=dev).manual_seed(seed)
+        x = fmap((n, c, h, w), 'fp32', dev, gen).requires_grad_(True)
+        ga, be = torch.ones(c, device=dev, requires_grad=True), torch.zeros(c, device=dev, requires_grad=True)
+        k = 0.5 + torch.rand(c, device=dev, generator=gen)
+        dy = k[None, :, None, None].expand(n, c, h, w).contiguous(memory_format=torch.channels_last)
+        dbe = torch.autograd.grad(ops.gn_act(x, ga, be, groups), [x, ga, be], dy)[2]
+        want = k.double().cpu() * (n * h * w)
+        within(dbe, (want, 64 * 2.0 ** -24 * want), 'dbeta, seed %d' % seed)
