@@ -182,3 +182,34 @@ def test_queries_and_keys_of_different_lengths(dev, lq, lk, packed):
     ok(gt, (dt, et + 2.0 ** -24 * (dt.abs() + et) + 1e-30), 'dtable')
     if packed:
         assert not gk[T - 2:].any() and not gv[T - 2:].any()
+
+
+@pytest.mark.parametrize('L,B,heads', [(20, 3, 2), (32, 2, 2), (70, 2, 2), (300, 2, 2), (1000, 1, 1), (1300, 1, 1), (600, 8, 12)])
+@pytest.mark.parametrize('kind', ['x30', 'x1000', 'rising', 'falling'])
+def test_sharp_scores(dev, L, B, heads, kind):
+    """Scores up to 10^8: rows that one key takes whole; maxima that rise with every tile, or stand in the first one."""
+    from creamfl_amd import ops
+    g = torch.Generator().manual_seed(L + B)
+    H = heads * 64
+    x = torch.randn(B, L, 3 * H, generator=g)
+    if kind[0] == 'x':
+        x[:, :, :2 * H] *= float(kind[1:])
+    else:
+        x[:, :, :H] = x[:, :, :H].abs() * 4
+        x[:, :, H:2 * H] = torch.linspace(-20, 20, L)[None, :, None] * (1 if kind == 'rising' else -1) + 0.1 * x[:, :, H:2 * H]
+    qkv, do = x.to(torch.bfloat16), torch.randn(B, L, H, generator=g).to(torch.bfloat16)
+    table, buckets = torch.randn(32, heads, generator=g), ops.relpos_buckets(32, 128)
+    leaves = [qkv.to(dev).requires_grad_(True), table.to(dev).requires_grad_(True)]
+    o = ops.relpos_attention(leaves[0], leaves[1], buckets.to(dev), heads)
+    dqkv, dtable = torch.autograd.grad(o, leaves, do.to(dev))
+    dt, et = torch.zeros(32, heads, dtype=torch.float64), torch.zeros(32, heads, dtype=torch.float64)
+    for b in range(B):
+        q, k, v = (t.reshape(L, heads, 64) for t in qkv[b].split(H, 1))
+        w = ref.relpos_attention_text(q, k, v, table, buckets, None, 0.125, do[b].view(L, heads, 64))
+        for t, name in ((o[b], 'o'), *zip(dqkv[b].split(H, 1), ('dq', 'dk', 'dv'))):
+            off = (t.double().cpu().reshape(L, heads, 64) - w[name][0]).abs()
+            assert bool((off <= w[name][1]).all()), (b, name, float((off / w[name][1]).nan_to_num(nan=np.inf).max()))
+        dt, et = dt + w['dtable'][0], et + w['dtable'][1]
+    # (a block's sums over diagonals hold to 2^-24 of the largest of them, over at most 2 x 16 additions and the difference of two)
+    off, bound = (dtable.double().cpu() - dt).abs(), et + 64 * 2.0 ** -24 * (et.max(0).values + dt.abs().max(0).values) + 1e-30
+    assert bool((off <= bound).all()), float((off / bound).max())
